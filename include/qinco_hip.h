@@ -301,6 +301,60 @@ QINCO_API int qinco_rerank(const float* xq, const float* cand, int64_t nq, int32
                  const int32_t* codes_in, int32_t Mc, int64_t* pos_out, float* dist_out, int64_t* ids_out, int32_t* codes_out,
                  void* stream);
 
+/* ---- codes drawn from a model's logits, and rows grouped by inverted list -------------------------------------------
+ * Element types of logits, rows and weights.  Sums, softmax statistics and products are held in 32 bits or more whatever the type. */
+enum { QINCO_T_F32 = 0, QINCO_T_F16 = 1, QINCO_T_BF16 = 2 };
+
+/* One code per row of logits (n, V), rows `row_stride` elements apart, 1 <= V <= 2^24: a prior over a codebook (V = K) or over the
+ * inverted lists (V = ivf_K); the codes are what qinco_decode and qinco_lut_decode take.  Codes are ordered by (logit descending, index ascending), NaN and
+ * -inf are never drawn; with e_i = exp((z_i - max z) / T) the kept ones are the first top_k of the order, of these every one with less
+ * than top_p of their mass before it (the first always), of these those with e_i >= min_p.  codes_out[r] = the lowest kept index at
+ * which the kept mass, summed in index order, exceeds u[r] times its total; logp_out[r] (nullable) its log probability among the kept.
+ * T <= 0: the largest logit's lowest index, log probability 0.  A row with nothing to draw: -1 and -inf.  u: (n) in [0, 1), values
+ * outside are taken as the nearest end, NaN as 0.  All decisions are taken on whole-number sums of 64-bit exponentials: the same
+ * inputs give the same codes, whatever the launch.
+ * The settings: arrays of one value per row, or NULL and the scalar.  top_k <= 0 or >= V, top_p >= 1, min_p <= 0 switch a cut off.
+ * workspace: qinco_sample_workspace(n, V) bytes of device memory that no other running call uses.  Device pointers, asynchronous. */
+typedef struct {
+  int32_t struct_bytes;            /* sizeof(qinco_sample_params) */
+  int32_t top_k;
+  double temperature, top_p, min_p;
+  const float* temperature_rows;   /* device (n), or NULL */
+  const int32_t* top_k_rows;
+  const float* top_p_rows;
+  const float* min_p_rows;
+} qinco_sample_params;
+QINCO_API int64_t qinco_sample_workspace(int64_t n, int64_t V);
+QINCO_API int qinco_sample_codes(const void* logits, int dtype, int64_t row_stride, int64_t n, int64_t V, const void* u, int u_is_f64,
+                                 const qinco_sample_params* params, void* codes_out, int code_dtype, float* logp_out, void* workspace,
+                                 int64_t workspace_bytes, void* stream);
+
+/* n rows with k list ids each (code_dtype, rows `row_stride` elements apart: the IVF column of a code matrix, or the ids that
+ * qinco_knn_search found) -> their n k entries (entry = row * k + j) in list order, stable:
+ *   order   (n k)          entry in each slot; -1 behind the last used slot
+ *   place   (n, k)         slot of each entry; -1 if it has no list (id < 0)
+ *   offsets (n_lists + 1)  first slot of each list; offsets[n_lists] = slots in use
+ *   bad     nullable       set to 1 if an id is >= n_lists (never cleared here); such an entry counts as having no list
+ * 1 <= n_lists <= 2^24, n k < 2^31.  workspace: qinco_group_workspace(n k, n_lists) bytes.  Device pointers, asynchronous. */
+QINCO_API int64_t qinco_group_workspace(int64_t entries, int64_t n_lists);
+QINCO_API int qinco_group_rows(const void* lists, int code_dtype, int64_t row_stride, int64_t n, int32_t k, int64_t n_lists, int32_t* order,
+                               int32_t* place, int32_t* offsets, int32_t* bad, void* workspace, int64_t workspace_bytes, void* stream);
+/* Rows of any type into list order: out[place[r, j]] = x[r]; slots behind *end (= offsets + n_lists) get zeros.  x rows are
+ * x_stride_bytes apart, out is (n k) rows of row_bytes. */
+QINCO_API int qinco_group_gather(const void* x, int64_t x_stride_bytes, int64_t row_bytes, const int32_t* place, const int32_t* end,
+                                 int64_t n, int32_t k, void* out, void* stream);
+/* ... and back: out[r] = sum_j w[r, j] y[place[r, j]] over the entries that have a slot (a row without one: zeros), in 32 bits in the
+ * order of j, rounded once.  weights (n, k) of w_dtype or NULL (ones: this is the gradient of the gather).  y (n k) rows of D elements,
+ * y_stride elements apart; out (n, D).  A weight of an entry without a slot is not read. */
+QINCO_API int qinco_group_combine(const void* y, int dtype, int64_t y_stride, int32_t D, const void* weights, int w_dtype,
+                                  const int32_t* place, int64_t n, int32_t k, void* out, void* stream);
+/* Gradients of the weighted sum: dy[place[r, j]] = w[r, j] dout[r] (zeros behind *end), dw[r, j] = <dout[r], y[place[r, j]]> (0 for an
+ * entry without a slot).  dout rows are dout_stride elements apart (0: one row for all); dy (n k, D) and dw (n, k) of weights' type, either
+ * of them may be NULL. */
+QINCO_API int qinco_group_combine_grad(const void* dout, int64_t dout_stride, const void* y, int64_t y_stride, int dtype, int32_t D,
+                                       const void* weights, int w_dtype, const int32_t* place, const int32_t* end, int64_t n, int32_t k,
+                                       void* dy, void* dw, void* stream);
+
 /* Device self-test of the in-wave sort / top-T selection primitives the table and beam kernels are built on, against a host
  * computation (random data, heavy ties, NaN / inf).  QINCO_OK, or QINCO_ERR_HIP with the first discrepancy in
  * qinco_last_error().  Runs on the current device; synchronous. */

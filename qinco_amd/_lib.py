@@ -14,6 +14,7 @@ FLAG_NORMALISED = 1
 CREATE_SPLIT_F16, CREATE_IVF_FP32, CREATE_TABLE_VALU, CREATE_DECODE_FOLDED, CREATE_TABLE_NO_COOP = 1, 2, 4, 8, 16
 CREATE_SPLIT_NO_CALIBRATION, CREATE_NO_PRESEL_FUSION, CREATE_NO_SMALL_LAUNCH, CREATE_EPILOGUE_SELECT = 32, 64, 128, 256
 CREATE_NO_EPILOGUE_SELECT = 512
+T_F32, T_F16, T_BF16 = 0, 1, 2
 
 # every symbol include/qinco_hip.h declares (tests check the library exports all of them)
 API_SYMBOLS = [
@@ -22,6 +23,7 @@ API_SYMBOLS = [
     "qinco_flops_per_vector_decode", "qinco_shape_supported", "qinco_last_error", "qinco_version",
     "qinco_lut_create", "qinco_lut_destroy", "qinco_lut_decode", "qinco_lut_decode_host",
     "qinco_ivf_last_stats", "qinco_check", "qinco_selftest", "qinco_knn_create", "qinco_knn_destroy", "qinco_knn_search", "qinco_knn_search_host", "qinco_knn_set_option", "qinco_knn_last_stats", "qinco_knn_roles_stats", "qinco_sqerr_sum", "qinco_rerank",
+    "qinco_sample_workspace", "qinco_sample_codes", "qinco_group_workspace", "qinco_group_rows", "qinco_group_gather", "qinco_group_combine", "qinco_group_combine_grad",
 ]
 
 
@@ -29,6 +31,12 @@ class QincoDesc(C.Structure):
     _fields_ = [("D", C.c_int32), ("De", C.c_int32), ("Dh", C.c_int32), ("L", C.c_int32), ("M", C.c_int32),
                 ("K", C.c_int32), ("A", C.c_int32), ("B", C.c_int32), ("qinco1_mode", C.c_int32),
                 ("ivf_K", C.c_int32), ("max_batch", C.c_int64)]
+
+
+class QincoSampleParams(C.Structure):
+    _fields_ = [("struct_bytes", C.c_int32), ("top_k", C.c_int32), ("temperature", C.c_double), ("top_p", C.c_double),
+                ("min_p", C.c_double), ("temperature_rows", C.c_void_p), ("top_k_rows", C.c_void_p), ("top_p_rows", C.c_void_p),
+                ("min_p_rows", C.c_void_p)]
 
 
 class QincoOptions(C.Structure):
@@ -150,6 +158,20 @@ def load() -> C.CDLL:
     lib.qinco_sqerr_sum.argtypes = [vp, vp, i64, C.POINTER(dbl), vp]
     lib.qinco_rerank.argtypes = [vp, vp, i64, C.c_int32, C.c_int32, C.c_int32, vp, vp, C.c_int32, vp, vp, vp, vp, vp]
     lib.qinco_rerank.restype = C.c_int
+    lib.qinco_sample_workspace.argtypes = [i64, i64]
+    lib.qinco_sample_workspace.restype = i64
+    lib.qinco_sample_codes.argtypes = [vp, i32, i64, i64, i64, vp, i32, C.POINTER(QincoSampleParams), vp, i32, vp, vp, i64, vp]
+    lib.qinco_sample_codes.restype = C.c_int
+    lib.qinco_group_workspace.argtypes = [i64, i64]
+    lib.qinco_group_workspace.restype = i64
+    lib.qinco_group_rows.argtypes = [vp, i32, i64, i64, C.c_int32, i64, vp, vp, vp, vp, vp, i64, vp]
+    lib.qinco_group_rows.restype = C.c_int
+    lib.qinco_group_gather.argtypes = [vp, i64, i64, vp, vp, i64, C.c_int32, vp, vp]
+    lib.qinco_group_gather.restype = C.c_int
+    lib.qinco_group_combine.argtypes = [vp, i32, i64, C.c_int32, vp, i32, vp, i64, C.c_int32, vp, vp]
+    lib.qinco_group_combine.restype = C.c_int
+    lib.qinco_group_combine_grad.argtypes = [vp, i64, vp, i64, i32, C.c_int32, vp, i32, vp, vp, i64, C.c_int32, vp, vp, vp]
+    lib.qinco_group_combine_grad.restype = C.c_int
     for name in ("qinco_lut_create", "qinco_lut_destroy", "qinco_lut_decode", "qinco_lut_decode_host"):
         getattr(lib, name).restype = C.c_int
     lib.qinco_last_error.restype = C.c_char_p

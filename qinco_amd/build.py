@@ -22,6 +22,7 @@ INST = PKG / "_instances"      # kernel instances built on demand (ensure_instan
 ARCH = "gfx950"
 FLAGS = ["-O3", "-std=c++20", "-fPIC", f"--offload-arch={ARCH}", "-Wall", "-Wno-unused-function",
          "-fvisibility=hidden"]
+NO_PACKED_F32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]   # two-wide fp32 instructions off (csrc/lists_hip.hip)
 
 
 def shapes() -> list[tuple[int, int, int, int, int]]:
@@ -108,6 +109,8 @@ def build(force: bool = False, verbose: bool = False, jobs: int | None = None) -
     for name in ("search_hip", "comm_hip"):
         o = OBJ / f"{name}.o"
         want(o, [cc, *FLAGS, "-c", str(CSRC / f"{name}.hip"), "-o", str(o)])
+    o = OBJ / "lists_hip.o"
+    want(o, [cc, *FLAGS, *NO_PACKED_F32, "-c", str(CSRC / "lists_hip.hip"), "-o", str(o)])
     if tasks:
         if verbose:
             print(f"[qinco_amd.build] compiling {len(tasks)} object(s) for {ARCH}", file=sys.stderr)

@@ -1,0 +1,506 @@
+// Rows grouped by inverted list (the router's dispatch): n rows with k list ids each -> the n k entries sorted by list, stably, and the
+// rows carried into that order and back with weights.  The ids are the IVF column of a code matrix (k = 1: filling an index,
+// reference qinco/search/search_utils.py:121-162) or the k nearest centroids of qinco_knn_search (multi-probe).
+//
+// SORT.  key_i = list of entry i; order = stable sort of the entries by key, a radix sort by digits of at most 11 bits, lowest digit
+// first.  Every pass is stable and free of atomics whose order shows: a tile of entries counts its digits (histogram), the counts are
+// summed down the tiles (scan), and every tile ranks its entries again and writes them to base[digit] + rank (scatter).  The rank of an
+// entry = the entries of the same digit before it: inside a wave by ballots over the digit's bits, across waves by a table in LDS.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace qinco {
+
+constexpr int kGroupThreads = 512, kGroupWaves = kGroupThreads / 64;
+constexpr int kGroupIpt = 8;                              // entries per thread
+constexpr int kGroupTile = kGroupThreads * kGroupIpt;     // 4096 entries per workgroup
+constexpr int kGroupMaxBits = 11, kGroupMaxBins = 1 << kGroupMaxBits;
+constexpr unsigned kGroupNone = 0xFFFFFFFFu;              // key of an entry without a list
+constexpr int kGroupSmallOffsets = 4096;                  // lists up to which the one-workgroup kernel writes the offsets itself
+
+struct GroupKeys {
+  const void* lists;   // (n, k) of code_dtype, rows `stride` elements apart
+  int code_dtype;      // QINCO_CODE_*
+  long stride;
+  unsigned k, N, E;    // N = n k entries
+};
+
+__device__ __forceinline__ unsigned group_key(const GroupKeys& g, unsigned i, bool& bad) {
+  const unsigned row = g.k == 1 ? i : i / g.k;
+  const long o = (long)row * g.stride + (i - row * g.k);
+  long v;
+  if (g.code_dtype == 0) v = (long)reinterpret_cast<const long long*>(g.lists)[o];
+  else if (g.code_dtype == 1) v = reinterpret_cast<const int*>(g.lists)[o];
+  else v = reinterpret_cast<const unsigned char*>(g.lists)[o];
+  bad = v >= (long)g.E;
+  return (v < 0 || bad) ? kGroupNone : (unsigned)v;
+}
+
+struct GroupPass {
+  GroupKeys in;             // first pass: the lists
+  const unsigned* key_in;   // later passes: keys and entries as the pass before left them, `*total` of them
+  const int* idx_in;
+  unsigned* key_out;        // sorted keys (null: nobody needs them)
+  int* idx_out;             // entries in this pass's order; the last pass: `order`
+  int* place;               // last pass: place[entry] = slot; first pass: -1 for entries without a list
+  int* offsets;             // written by a sort of one pass (E + 1), else null
+  unsigned* counts;         // [tile][bin], after the scan: entries of that bin in earlier tiles
+  unsigned* totals;         // [bin]
+  unsigned* total;          // entries that have a list
+  int* bad;                 // nullable: set to 1 if an id is >= E
+  int shift, bits, first, last;
+};
+
+// one wave's counter of a digit in LDS: read and bumped by lanes of the same wave, whose LDS accesses execute in order
+__device__ __forceinline__ unsigned group_seen(const unsigned short& c) { return __hip_atomic_load(&c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
+__device__ __forceinline__ void group_bump(unsigned short& c, unsigned v) { __hip_atomic_store(&c, (unsigned short)v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP); }
+
+// entries of digit d before this one in the wave: the lanes whose d agrees, by one ballot per bit
+__device__ __forceinline__ unsigned long long group_match(unsigned d, bool valid, int bits) {
+  unsigned long long m = __ballot(valid);
+  for (int b = 0; b < bits; ++b) {
+    const bool s = (d >> b) & 1;
+    const unsigned long long bb = __ballot(s);
+    m &= s ? bb : ~bb;
+  }
+  return m;
+}
+
+__global__ void __launch_bounds__(kGroupThreads) group_hist_kernel(GroupPass a) {
+  __shared__ unsigned hist[kGroupMaxBins];
+  const int bins = 1 << a.bits;
+  for (int b = threadIdx.x; b < bins; b += kGroupThreads) hist[b] = 0;
+  __syncthreads();
+  const unsigned N = a.first ? a.in.N : *a.total;
+  const unsigned mask = bins - 1;
+  bool any_bad = false;
+#pragma unroll
+  for (int r = 0; r < kGroupIpt; ++r) {
+    const unsigned i = blockIdx.x * (unsigned)kGroupTile + r * kGroupThreads + threadIdx.x;
+    if (i < N) {
+      bool bad = false;
+      const unsigned key = a.first ? group_key(a.in, i, bad) : a.key_in[i];
+      any_bad |= bad;
+      if (key != kGroupNone) atomicAdd(&hist[(key >> a.shift) & mask], 1u);
+    }
+  }
+  if (any_bad && a.bad) *a.bad = 1;
+  __syncthreads();
+  for (int b = threadIdx.x; b < bins; b += kGroupThreads) a.counts[(size_t)blockIdx.x * bins + b] = hist[b];
+}
+
+// counts[tile][bin] -> entries of the bin in earlier tiles; totals[bin].  A workgroup owns 64 bins, its 16 waves a run of tiles each.
+__global__ void __launch_bounds__(1024) group_scan_kernel(unsigned* counts, unsigned* totals, int tiles, int bins) {
+  __shared__ unsigned part[16][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int bin = blockIdx.x * 64 + lane;
+  const int per = (tiles + 15) / 16;
+  const int t0 = w * per, t1 = t0 + per < tiles ? t0 + per : tiles;
+  unsigned sum = 0;
+  if (bin < bins)
+    for (int t = t0; t < t1; ++t) sum += counts[(size_t)t * bins + bin];
+  part[w][lane] = sum;
+  __syncthreads();
+  unsigned run = 0, all = 0;
+  for (int v = 0; v < 16; ++v) {
+    const unsigned p = part[v][lane];
+    run += v < w ? p : 0;
+    all += p;
+  }
+  if (bin < bins) {
+    for (int t = t0; t < t1; ++t) {
+      const size_t o = (size_t)t * bins + bin;
+      const unsigned c = counts[o];
+      counts[o] = run;
+      run += c;
+    }
+    if (w == 0) totals[bin] = all;
+  }
+}
+
+// exclusive scan of v over the workgroup's threads; *all = the sum.  Ends with a barrier behind its last read of tmp.
+__device__ __forceinline__ unsigned group_block_scan(unsigned v, unsigned* tmp, unsigned* all) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  unsigned s = v;
+  for (int d = 1; d < 64; d <<= 1) {
+    const unsigned o = __shfl_up(s, d, 64);
+    if (lane >= d) s += o;
+  }
+  if (lane == 63) tmp[w] = s;
+  __syncthreads();
+  unsigned before = 0, sum = 0;
+  for (int i = 0; i < kGroupWaves; ++i) {
+    const unsigned t = tmp[i];
+    before += i < w ? t : 0;
+    sum += t;
+  }
+  __syncthreads();
+  *all = sum;
+  return before + s - v;
+}
+
+__global__ void __launch_bounds__(kGroupThreads) group_scatter_kernel(GroupPass a) {
+  __shared__ unsigned short whist[kGroupWaves][kGroupMaxBins];   // entries of a digit in the wave so far, then in earlier waves
+  __shared__ unsigned base[kGroupMaxBins];
+  __shared__ unsigned tmp[kGroupWaves];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int bins = 1 << a.bits;
+  const unsigned mask = bins - 1;
+  for (int b = tid; b < bins; b += kGroupThreads)
+    for (int v = 0; v < kGroupWaves; ++v) whist[v][b] = 0;
+  const unsigned N = a.first ? a.in.N : *a.total;
+  const unsigned tile0 = blockIdx.x * (unsigned)kGroupTile;
+  unsigned key[kGroupIpt], rank[kGroupIpt];
+  int idx[kGroupIpt];
+#pragma unroll
+  for (int r = 0; r < kGroupIpt; ++r) {
+    const unsigned i = tile0 + w * (64 * kGroupIpt) + r * 64 + lane;
+    key[r] = kGroupNone;
+    idx[r] = (int)i;
+    if (i < N) {
+      bool bad;
+      if (a.first) {
+        key[r] = group_key(a.in, i, bad);
+        if (key[r] == kGroupNone) a.place[i] = -1;
+      } else {
+        key[r] = a.key_in[i];
+        idx[r] = a.idx_in[i];
+      }
+    }
+  }
+  // the first slot of every digit: totals summed over the digits, plus the digit's entries in earlier tiles
+  const int bpt = (bins + kGroupThreads - 1) / kGroupThreads;   // 1 .. 4 neighbouring bins per thread
+  unsigned mine[kGroupMaxBins / kGroupThreads], s = 0;
+#pragma unroll
+  for (int j = 0; j < kGroupMaxBins / kGroupThreads; ++j) {
+    const int b = tid * bpt + j;
+    mine[j] = (j < bpt && b < bins) ? a.totals[b] : 0;
+    s += mine[j];
+  }
+  unsigned all;
+  unsigned start = group_block_scan(s, tmp, &all);   // (its barriers also stand between the clearing of whist and its use)
+#pragma unroll
+  for (int j = 0; j < kGroupMaxBins / kGroupThreads; ++j) {
+    const int b = tid * bpt + j;
+    if (j < bpt && b < bins) {
+      if (blockIdx.x == 0 && a.offsets && (unsigned)b < a.in.E) a.offsets[b] = (int)start;
+      base[b] = start + a.counts[(size_t)blockIdx.x * bins + b];
+      start += mine[j];
+    }
+  }
+  if (blockIdx.x == 0 && tid == 0) {
+    if (a.offsets) a.offsets[a.in.E] = (int)all;
+    if (a.first) *a.total = all;
+  }
+#pragma unroll
+  for (int r = 0; r < kGroupIpt; ++r) {
+    const bool valid = key[r] != kGroupNone;
+    const unsigned d = (key[r] >> a.shift) & mask;
+    const unsigned long long m = group_match(d, valid, a.bits);
+    const unsigned below = __builtin_popcountll(m & ((1ull << lane) - 1));
+    if (valid) {
+      const unsigned seen = group_seen(whist[w][d]);
+      rank[r] = seen + below;
+      if (below == 0) group_bump(whist[w][d], seen + __builtin_popcountll(m));
+    }
+  }
+  __syncthreads();
+  for (int b = tid; b < bins; b += kGroupThreads) {
+    unsigned run = 0;
+    for (int v = 0; v < kGroupWaves; ++v) {
+      const unsigned c = whist[v][b];
+      whist[v][b] = (unsigned short)run;
+      run += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < kGroupIpt; ++r) {
+    if (key[r] != kGroupNone) {
+      const unsigned d = (key[r] >> a.shift) & mask;
+      const unsigned dst = base[d] + whist[w][d] + rank[r];
+      a.idx_out[dst] = idx[r];
+      if (a.key_out) a.key_out[dst] = key[r];
+      if (a.last) a.place[idx[r]] = (int)dst;
+    }
+  }
+  if (a.last) {
+    for (int r = 0; r < kGroupIpt; ++r) {
+      const unsigned p = tile0 + r * kGroupThreads + tid;
+      if (p >= all && p < a.in.N) a.idx_out[p] = -1;
+    }
+  }
+}
+
+// offsets[e] = entries whose key is below e: a binary search in the sorted keys per list
+__global__ void __launch_bounds__(256) group_offsets_kernel(const unsigned* keys, const unsigned* total, int* offsets, unsigned E) {
+  const unsigned n = *total;
+  for (unsigned long e = blockIdx.x * 256ul + threadIdx.x; e <= E; e += gridDim.x * 256ul) {
+    unsigned lo = 0, hi = n;
+    while (lo < hi) {
+      const unsigned mid = lo + (hi - lo) / 2;
+      if (keys[mid] < e) lo = mid + 1;
+      else hi = mid;
+    }
+    offsets[e] = (int)lo;
+  }
+}
+
+// Up to one tile of entries: every pass in one workgroup, keys and entries in LDS between the passes.
+__global__ void __launch_bounds__(kGroupThreads) group_small_kernel(GroupPass a, int passes) {
+  __shared__ unsigned skey[kGroupTile];
+  __shared__ unsigned short sidx[kGroupTile];
+  __shared__ unsigned short whist[kGroupWaves][kGroupMaxBins];
+  __shared__ unsigned base[kGroupMaxBins];
+  __shared__ unsigned tmp[kGroupWaves];
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+  const int bins = 1 << a.bits;
+  const unsigned mask = bins - 1;
+  const int rounds = (int)((a.in.N + kGroupThreads - 1) / kGroupThreads);   // entries per thread, the same for every wave
+  unsigned n = a.in.N;
+  unsigned key[kGroupIpt], rank[kGroupIpt];
+  int idx[kGroupIpt];
+  bool any_bad = false;
+  for (int pass = 0; pass < passes; ++pass) {
+    const int shift = pass * a.bits;
+    for (int b = tid; b < bins; b += kGroupThreads)
+      for (int v = 0; v < kGroupWaves; ++v) whist[v][b] = 0;
+#pragma unroll
+    for (int r = 0; r < kGroupIpt; ++r) {
+      const unsigned i = (w * rounds + r) * 64 + lane;
+      key[r] = kGroupNone;
+      idx[r] = (int)i;
+      if (r < rounds && i < n) {
+        if (pass == 0) {
+          bool bad;
+          key[r] = group_key(a.in, i, bad);
+          any_bad |= bad;
+          if (key[r] == kGroupNone) a.place[i] = -1;
+        } else {
+          key[r] = skey[i];
+          idx[r] = sidx[i];
+        }
+      }
+    }
+    __syncthreads();
+  #pragma unroll
+    for (int r = 0; r < kGroupIpt; ++r) {
+      if (r < rounds) {
+        const bool valid = key[r] != kGroupNone;
+        const unsigned d = (key[r] >> shift) & mask;
+        const unsigned long long m = group_match(d, valid, a.bits);
+        const unsigned below = __builtin_popcountll(m & ((1ull << lane) - 1));
+        if (valid) {
+          const unsigned seen = group_seen(whist[w][d]);
+          rank[r] = seen + below;
+          if (below == 0) group_bump(whist[w][d], seen + __builtin_popcountll(m));
+        }
+      }
+    }
+    __syncthreads();
+    const int bpt = (bins + kGroupThreads - 1) / kGroupThreads;
+    unsigned mine[kGroupMaxBins / kGroupThreads], s = 0;
+#pragma unroll
+    for (int j = 0; j < kGroupMaxBins / kGroupThreads; ++j) {
+      const int b = tid * bpt + j;
+      mine[j] = 0;
+      if (j < bpt && b < bins) {
+        unsigned run = 0;
+        for (int v = 0; v < kGroupWaves; ++v) {
+          const unsigned c = whist[v][b];
+          whist[v][b] = (unsigned short)run;
+          run += c;
+        }
+        mine[j] = run;
+      }
+      s += mine[j];
+    }
+    unsigned all;
+    unsigned start = group_block_scan(s, tmp, &all);
+#pragma unroll
+    for (int j = 0; j < kGroupMaxBins / kGroupThreads; ++j) {
+      const int b = tid * bpt + j;
+      if (j < bpt && b < bins) {
+        base[b] = start;
+        start += mine[j];
+      }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kGroupIpt; ++r) {
+      if (r < rounds && key[r] != kGroupNone) {
+        const unsigned d = (key[r] >> shift) & mask;
+        const unsigned dst = base[d] + whist[w][d] + rank[r];
+        skey[dst] = key[r];
+        sidx[dst] = (unsigned short)idx[r];
+      }
+    }
+    n = all;
+    __syncthreads();
+  }
+  if (any_bad && a.bad) *a.bad = 1;
+  for (unsigned p = tid; p < a.in.N; p += kGroupThreads) {
+    if (p < n) {
+      const int i = sidx[p];
+      a.idx_out[p] = i;
+      a.place[i] = (int)p;
+      if (a.key_out) a.key_out[p] = skey[p];
+    } else {
+      a.idx_out[p] = -1;
+    }
+  }
+  if (tid == 0 && a.total) *a.total = n;
+  if (a.offsets)
+    for (unsigned e = tid; e <= a.in.E; e += kGroupThreads) {
+      unsigned lo = 0, hi = n;
+      while (lo < hi) {
+        const unsigned mid = (lo + hi) / 2;
+        if (skey[mid] < e) lo = mid + 1;
+        else hi = mid;
+      }
+      a.offsets[e] = (int)lo;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Rows.  All of these are bound by HBM: a row is read or written once, in the widest units that its width, strides and base allow
+// (16 bytes down to 1); `lanes` (a power of two up to 64) lanes share a row and step through its units, so no index is divided.
+// ---------------------------------------------------------------------------------------------------------------------
+struct GroupRows {
+  const int* place;    // (n, k)
+  const int* end;      // = offsets + E: slots in use
+  long n, N;           // rows, entries = n k
+  int k;
+  int units;           // units per row
+  int lanes_log2;
+};
+
+template <typename U>
+__global__ void __launch_bounds__(256) group_gather_kernel(GroupRows g, const char* x, long x_stride, char* out, long row_bytes) {
+  const int lanes = 1 << g.lanes_log2;
+  const int u0 = threadIdx.x & (lanes - 1);
+  const long per = 256 >> g.lanes_log2;
+  const long first = (long)blockIdx.x * per + (threadIdx.x >> g.lanes_log2), step = (long)gridDim.x * per;
+  for (long r = first; r < g.n; r += step) {
+    const int* pl = g.place + r * g.k;
+    const U* src = reinterpret_cast<const U*>(x + r * x_stride);
+    for (int u = u0; u < g.units; u += lanes) {
+      const U v = src[u];
+      for (int j = 0; j < g.k; ++j) {
+        const int p = pl[j];
+        if (p >= 0) reinterpret_cast<U*>(out + (long)p * row_bytes)[u] = v;
+      }
+    }
+  }
+  for (long s = *g.end + first; s < g.N; s += step)
+    for (int u = u0; u < g.units; u += lanes) reinterpret_cast<U*>(out + s * row_bytes)[u] = U{};
+}
+
+template <typename T> struct GroupNum;
+template <> struct GroupNum<float> {
+  static __device__ __forceinline__ float get(float v) { return v; }
+  static __device__ __forceinline__ float put(float v) { return v; }
+};
+template <> struct GroupNum<_Float16> {
+  static __device__ __forceinline__ float get(_Float16 v) { return (float)v; }
+  static __device__ __forceinline__ _Float16 put(float v) { return (_Float16)v; }
+};
+template <> struct GroupNum<__bf16> {
+  static __device__ __forceinline__ float get(__bf16 v) { return (float)v; }
+  static __device__ __forceinline__ __bf16 put(float v) { return (__bf16)v; }
+};
+
+template <typename T, int E> struct alignas(sizeof(T) * E) GroupVec { T v[E]; };
+
+// weight of entry i in 32 bits (w_dtype: QINCO_T_*; no weights: 1)
+__device__ __forceinline__ float group_weight(const void* w, int w_dtype, long i) {
+  if (!w) return 1.f;
+  if (w_dtype == 0) return reinterpret_cast<const float*>(w)[i];
+  if (w_dtype == 1) return (float)reinterpret_cast<const _Float16*>(w)[i];
+  return (float)reinterpret_cast<const __bf16*>(w)[i];
+}
+
+// out[r] = sum_j w[r, j] y[place[r, j]]: sums in 32 bits in the order of j, rounded once.  The gradient of the gather is this with
+// weights of one.
+template <typename T, int E>
+__global__ void __launch_bounds__(256) group_combine_kernel(GroupRows g, const T* y, long y_stride, const void* wt, int w_dtype, T* out) {
+  using V = GroupVec<T, E>;
+  const int lanes = 1 << g.lanes_log2;
+  const int u0 = threadIdx.x & (lanes - 1);
+  const long per = 256 >> g.lanes_log2;
+  const long first = (long)blockIdx.x * per + (threadIdx.x >> g.lanes_log2), step = (long)gridDim.x * per;
+  for (long r = first; r < g.n; r += step) {
+    for (int u = u0; u < g.units; u += lanes) {
+      float acc[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = 0.f;
+      for (int j = 0; j < g.k; ++j) {
+        const int p = g.place[r * g.k + j];
+        if (p >= 0) {
+          const float w = group_weight(wt, w_dtype, r * g.k + j);
+          const V v = reinterpret_cast<const V*>(y + (long)p * y_stride)[u];
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[e] = fmaf(w, GroupNum<T>::get(v.v[e]), acc[e]);
+        }
+      }
+      V o;
+#pragma unroll
+      for (int e = 0; e < E; ++e) o.v[e] = GroupNum<T>::put(acc[e]);
+      reinterpret_cast<V*>(out + r * (long)g.units * E)[u] = o;
+    }
+  }
+}
+
+// dy[place[r, j]] = w[r, j] dout[r], dw[r, j] = <dout[r], y[place[r, j]]> in one pass over y and dout; rows of dy no entry owns: zeros
+template <typename T, int E, typename W>
+__global__ void __launch_bounds__(256) group_combine_grad_kernel(GroupRows g, const T* dout, long dout_stride, const T* y, long y_stride,
+                                                                 const W* wt, T* dy, W* dw) {
+  using V = GroupVec<T, E>;
+  constexpr int J = 8;   // entries of a row taken together: their dot products are summed over the row's lanes at the end
+  const int lanes = 1 << g.lanes_log2;
+  const int u0 = threadIdx.x & (lanes - 1);
+  const long per = 256 >> g.lanes_log2;
+  const long first = (long)blockIdx.x * per + (threadIdx.x >> g.lanes_log2), step = (long)gridDim.x * per;
+  const long row_elems = (long)g.units * E;
+  for (long r = first; r < g.n; r += step) {
+    const V* d = reinterpret_cast<const V*>(dout + r * dout_stride);
+    for (int j0 = 0; j0 < g.k; j0 += J) {
+      int p[J];
+      float w[J], dot[J];
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        p[j] = j0 + j < g.k ? g.place[r * g.k + j0 + j] : -1;
+        w[j] = p[j] >= 0 ? GroupNum<W>::get(wt[r * g.k + j0 + j]) : 0.f;
+        dot[j] = 0.f;
+      }
+      for (int u = u0; u < g.units; u += lanes) {
+        const V dv = d[u];
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          if (p[j] >= 0) {
+            const V v = reinterpret_cast<const V*>(y + (long)p[j] * y_stride)[u];
+            V o;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+              const float x = GroupNum<T>::get(dv.v[e]);
+              dot[j] = fmaf(x, GroupNum<T>::get(v.v[e]), dot[j]);
+              o.v[e] = GroupNum<T>::put(w[j] * x);
+            }
+            if (dy) reinterpret_cast<V*>(dy + (long)p[j] * row_elems)[u] = o;
+          }
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        for (int m = lanes >> 1; m > 0; m >>= 1) dot[j] += __shfl_xor(dot[j], m, 64);
+        if (dw && u0 == 0 && j0 + j < g.k) dw[r * g.k + j0 + j] = GroupNum<W>::put(dot[j]);
+      }
+    }
+  }
+  if (!dy) return;
+  for (long s = *g.end + first; s < g.N; s += step)
+    for (int u = u0; u < g.units; u += lanes) reinterpret_cast<V*>(dy + s * row_elems)[u] = V{};
+}
+
+}  // namespace qinco

@@ -1,0 +1,273 @@
+// C ABI of the operators between a model that answers in codes and the codec (include/qinco_hip.h): codes drawn from logits
+// (sample_kernel.hpp) and rows grouped by inverted list (group_kernel.hpp).  None of them keeps state: outputs and workspace are the
+// caller's, every argument is checked on the host before anything is launched, and nothing is synchronised.
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+#include <initializer_list>
+#include <type_traits>
+
+#include "abi_util.hpp"
+#include "group_kernel.hpp"
+#include "sample_kernel.hpp"
+
+using namespace qinco;
+#define fail qinco::abi_fail
+
+static constexpr int64_t kMaxLists = (int64_t)1 << 24;
+
+static int bits_of(uint64_t v) {   // bits that hold 0 .. v - 1
+  int b = 0;
+  while (b < 63 && ((uint64_t)1 << b) < v) ++b;
+  return b;
+}
+
+static bool known(int dtype) { return dtype == QINCO_T_F32 || dtype == QINCO_T_F16 || dtype == QINCO_T_BF16; }
+static int size_of(int dtype) { return dtype == QINCO_T_F32 ? 4 : 2; }
+
+// ---------------------------------------------------------------------------------------------
+// sampling
+// ---------------------------------------------------------------------------------------------
+extern "C" int64_t qinco_sample_workspace(int64_t n, int64_t V) {
+  if (n < 0 || V < 1 || V > kMaxLists) return 0;
+  return 0;
+}
+
+extern "C" int qinco_sample_codes(const void* logits, int dtype, int64_t row_stride, int64_t n, int64_t V, const void* u, int u_is_f64,
+                                  const qinco_sample_params* params, void* codes_out, int code_dtype, float* logp_out, void* workspace,
+                                  int64_t workspace_bytes, void* stream) {
+  if (!params || params->struct_bytes != (int32_t)sizeof(qinco_sample_params))
+    return fail(QINCO_ERR_INVALID, "qinco_sample_codes: params missing, or struct_bytes is not sizeof(qinco_sample_params)");
+  if (!known(dtype)) return fail(QINCO_ERR_INVALID, "qinco_sample_codes: unknown element type %d", dtype);
+  if (code_dtype != QINCO_CODE_I64 && code_dtype != QINCO_CODE_I32)
+    return fail(QINCO_ERR_INVALID, "qinco_sample_codes: codes are int64 or int32 (a row with nothing to draw answers -1)");
+  if (V < 1 || V > kMaxLists) return fail(QINCO_ERR_INVALID, "qinco_sample_codes: need 1 <= V <= 2^24 (V=%lld)", (long long)V);
+  if (n < 0 || n > INT32_MAX) return fail(QINCO_ERR_INVALID, "qinco_sample_codes: need 0 <= n < 2^31 (n=%lld)", (long long)n);
+  if (row_stride < 0) return fail(QINCO_ERR_INVALID, "qinco_sample_codes: negative row stride");
+  if (n == 0) return QINCO_OK;
+  if (!logits || !u || !codes_out) return fail(QINCO_ERR_INVALID, "qinco_sample_codes: null buffer");
+  const int64_t need = qinco_sample_workspace(n, V);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return fail(QINCO_ERR_INVALID, "qinco_sample_codes: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  const int lv = bits_of((uint64_t)V);
+  SampleArgs a{logits, (long)row_stride, (long)n, (int)V, u, u_is_f64 != 0, params->temperature_rows, params->temperature, params->top_k_rows,
+               params->top_k, params->top_p_rows, params->top_p, params->min_p_rows, params->min_p, codes_out,
+               code_dtype == QINCO_CODE_I64, logp_out, 62 - lv < 51 ? 62 - lv : 51};
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const dim3 grid((unsigned)(n < 65536 ? n : 65536)), block(kSampleThreads);
+  if (dtype == QINCO_T_F32) hipLaunchKernelGGL(sample_row_kernel<float>, grid, block, 0, st, a);
+  else if (dtype == QINCO_T_F16) hipLaunchKernelGGL(sample_row_kernel<_Float16>, grid, block, 0, st, a);
+  else hipLaunchKernelGGL(sample_row_kernel<__bf16>, grid, block, 0, st, a);
+  HIP_TRY(hipGetLastError());
+  return QINCO_OK;
+}
+
+// ---------------------------------------------------------------------------------------------
+// grouping
+// ---------------------------------------------------------------------------------------------
+namespace {
+struct GroupPlan {
+  int bits, passes;     // bits of one digit (the same for every pass)
+  int64_t tiles;
+  // workspace, in 32-bit words: total | totals | counts | key and entry buffers of the passes
+  int64_t totals, counts, buf, words;
+  int buffers;          // arrays of N words behind `buf`
+};
+}  // namespace
+
+static GroupPlan group_plan(int64_t N, int64_t E) {
+  GroupPlan p{};
+  const int all = bits_of((uint64_t)E);
+  p.passes = all <= kGroupMaxBits ? 1 : (all + kGroupMaxBits - 1) / kGroupMaxBits;
+  p.bits = (all + p.passes - 1) / p.passes;
+  p.tiles = (N + kGroupTile - 1) / kGroupTile;
+  const int64_t bins = (int64_t)1 << p.bits;
+  const bool small = p.tiles <= 1;
+  // two passes: key + entry of the first, sorted keys of the second; three: the same, and the second's entries
+  p.buffers = small ? (E > kGroupSmallOffsets ? 1 : 0) : (p.passes == 1 ? 0 : p.passes == 2 ? 3 : 4);
+  p.totals = 16;
+  p.counts = p.totals + (small ? 0 : bins);
+  p.buf = p.counts + (small ? 0 : p.tiles * bins);
+  p.words = p.buf + p.buffers * N;
+  return p;
+}
+
+extern "C" int64_t qinco_group_workspace(int64_t entries, int64_t n_lists) {
+  if (entries < 0 || entries > INT32_MAX || n_lists < 1 || n_lists > kMaxLists) return 0;
+  return group_plan(entries, n_lists).words * 4;
+}
+
+extern "C" int qinco_group_rows(const void* lists, int code_dtype, int64_t row_stride, int64_t n, int32_t k, int64_t n_lists, int32_t* order,
+                                int32_t* place, int32_t* offsets, int32_t* bad, void* workspace, int64_t workspace_bytes, void* stream) {
+  if (code_dtype != QINCO_CODE_I64 && code_dtype != QINCO_CODE_I32 && code_dtype != QINCO_CODE_U8)
+    return fail(QINCO_ERR_INVALID, "qinco_group_rows: unknown code type %d", code_dtype);
+  if (n_lists < 1 || n_lists > kMaxLists)
+    return fail(QINCO_ERR_INVALID, "qinco_group_rows: need 1 <= n_lists <= 2^24 (n_lists=%lld)", (long long)n_lists);
+  if (n < 0 || k < 1 || n > INT32_MAX / k) return fail(QINCO_ERR_INVALID, "qinco_group_rows: need n >= 0, k >= 1, n k < 2^31");
+  if (row_stride < 0) return fail(QINCO_ERR_INVALID, "qinco_group_rows: negative row stride");
+  const int64_t N = n * k;
+  if (!offsets || (N > 0 && (!lists || !order || !place))) return fail(QINCO_ERR_INVALID, "qinco_group_rows: null buffer");
+  const GroupPlan p = group_plan(N, n_lists);
+  if (!workspace || workspace_bytes < p.words * 4)
+    return fail(QINCO_ERR_INVALID, "qinco_group_rows: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)p.words * 4);
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  unsigned* ws = reinterpret_cast<unsigned*>(workspace);
+  const unsigned E = (unsigned)n_lists;
+  GroupPass a{};
+  a.in = GroupKeys{lists, code_dtype, (long)row_stride, (unsigned)k, (unsigned)N, E};
+  a.place = place;
+  a.total = ws;
+  a.totals = ws + p.totals;
+  a.counts = ws + p.counts;
+  a.bad = bad;
+  a.bits = p.bits;
+  a.first = a.last = 1;
+  a.idx_out = order;
+  unsigned* sorted = nullptr;   // keys in slot order, where the offsets are searched in them
+  if (p.tiles <= 1) {
+    if (p.buffers) sorted = ws + p.buf;
+    a.key_out = sorted;
+    a.offsets = sorted ? nullptr : offsets;
+    hipLaunchKernelGGL(group_small_kernel, dim3(1), dim3(kGroupThreads), 0, st, a, p.passes);
+    HIP_TRY(hipGetLastError());
+  } else {
+    unsigned* buf = ws + p.buf;
+    unsigned* keys[2] = {buf, buf + N};
+    int* idx[2] = {reinterpret_cast<int*>(buf + 2 * N), reinterpret_cast<int*>(buf + 3 * N)};
+    const int bins = 1 << p.bits;
+    for (int pass = 0; pass < p.passes; ++pass) {
+      a.shift = pass * p.bits;
+      a.first = pass == 0;
+      a.last = pass == p.passes - 1;
+      a.key_in = pass ? keys[(pass - 1) & 1] : nullptr;
+      a.idx_in = pass ? idx[(pass - 1) & 1] : nullptr;
+      a.key_out = p.passes > 1 ? keys[pass & 1] : nullptr;
+      a.idx_out = a.last ? order : idx[pass & 1];
+      a.offsets = p.passes == 1 ? offsets : nullptr;
+      if (a.last && p.passes > 1) sorted = a.key_out;
+      hipLaunchKernelGGL(group_hist_kernel, dim3((unsigned)p.tiles), dim3(kGroupThreads), 0, st, a);
+      HIP_TRY(hipGetLastError());
+      hipLaunchKernelGGL(group_scan_kernel, dim3((unsigned)((bins + 63) / 64)), dim3(1024), 0, st, a.counts, a.totals, (int)p.tiles, bins);
+      HIP_TRY(hipGetLastError());
+      hipLaunchKernelGGL(group_scatter_kernel, dim3((unsigned)p.tiles), dim3(kGroupThreads), 0, st, a);
+      HIP_TRY(hipGetLastError());
+    }
+  }
+  if (sorted) {
+    long g = ((long)n_lists + 256) / 256;
+    if (g > 4096) g = 4096;
+    hipLaunchKernelGGL(group_offsets_kernel, dim3((unsigned)g), dim3(256), 0, st, sorted, a.total, offsets, E);
+    HIP_TRY(hipGetLastError());
+  }
+  return QINCO_OK;
+}
+
+// rows of `bytes` bytes at these addresses and strides: the widest unit they all are multiples of
+static int unit_of(int64_t bytes, std::initializer_list<int64_t> strides, std::initializer_list<const void*> ptrs) {
+  uint64_t all = (uint64_t)bytes | 16;
+  for (int64_t s : strides) all |= (uint64_t)s;
+  for (const void* p : ptrs) all |= reinterpret_cast<uintptr_t>(p);
+  return (int)(all & (~all + 1));
+}
+
+static GroupRows group_rows_of(const int32_t* place, const int32_t* end, int64_t n, int32_t k, int64_t units) {
+  int l = 0;
+  while (l < 6 && (1 << l) < units) ++l;
+  return GroupRows{place, end, (long)n, (long)n * k, k, (int)units, l};
+}
+
+static dim3 group_grid(const GroupRows& g) {
+  const long per = 256 >> g.lanes_log2;
+  long b = (g.n + per - 1) / per;
+  if (b > 65536) b = 65536;
+  return dim3((unsigned)b);
+}
+
+extern "C" int qinco_group_gather(const void* x, int64_t x_stride_bytes, int64_t row_bytes, const int32_t* place, const int32_t* end,
+                                  int64_t n, int32_t k, void* out, void* stream) {
+  if (n < 0 || k < 1 || n > INT32_MAX / k || row_bytes < 1 || row_bytes > INT32_MAX || x_stride_bytes < 0)
+    return fail(QINCO_ERR_INVALID, "qinco_group_gather: need n >= 0, k >= 1, n k < 2^31, 1 <= row_bytes < 2^31, a stride >= 0");
+  if (n == 0) return QINCO_OK;
+  if (!x || !place || !end || !out) return fail(QINCO_ERR_INVALID, "qinco_group_gather: null buffer");
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  const int unit = unit_of(row_bytes, {x_stride_bytes}, {x, out});
+  const GroupRows g = group_rows_of(place, end, n, k, row_bytes / unit);
+  const dim3 grid = group_grid(g), block(256);
+  const char* xs = reinterpret_cast<const char*>(x);
+  char* o = reinterpret_cast<char*>(out);
+  switch (unit) {
+    case 16: hipLaunchKernelGGL(group_gather_kernel<uint4>, grid, block, 0, st, g, xs, (long)x_stride_bytes, o, (long)row_bytes); break;
+    case 8: hipLaunchKernelGGL(group_gather_kernel<uint2>, grid, block, 0, st, g, xs, (long)x_stride_bytes, o, (long)row_bytes); break;
+    case 4: hipLaunchKernelGGL(group_gather_kernel<unsigned>, grid, block, 0, st, g, xs, (long)x_stride_bytes, o, (long)row_bytes); break;
+    case 2: hipLaunchKernelGGL(group_gather_kernel<unsigned short>, grid, block, 0, st, g, xs, (long)x_stride_bytes, o, (long)row_bytes); break;
+    default: hipLaunchKernelGGL(group_gather_kernel<unsigned char>, grid, block, 0, st, g, xs, (long)x_stride_bytes, o, (long)row_bytes);
+  }
+  HIP_TRY(hipGetLastError());
+  return QINCO_OK;
+}
+
+// f(T{}, element count of a unit as std::integral_constant) for the unit of `bytes` bytes
+template <typename T, typename F>
+static void with_unit(int bytes, F f) {
+  if (bytes >= 16) f(T{}, std::integral_constant<int, 16 / sizeof(T)>{});
+  else if (bytes >= 8) f(T{}, std::integral_constant<int, 8 / sizeof(T)>{});
+  else if (sizeof(T) == 2 && bytes >= 4) f(T{}, std::integral_constant<int, sizeof(T) == 2 ? 2 : 1>{});
+  else f(T{}, std::integral_constant<int, 1>{});
+}
+
+template <typename F>
+static void with_type(int dtype, int unit, F f) {
+  if (dtype == QINCO_T_F32) with_unit<float>(unit, f);
+  else if (dtype == QINCO_T_F16) with_unit<_Float16>(unit, f);
+  else with_unit<__bf16>(unit, f);
+}
+
+static int check_rows(const char* who, int dtype, int w_dtype, bool weights, int64_t n, int32_t k, int32_t D) {
+  if (!known(dtype)) return fail(QINCO_ERR_INVALID, "%s: unknown element type %d", who, dtype);
+  if (weights && w_dtype != QINCO_T_F32 && w_dtype != dtype)
+    return fail(QINCO_ERR_INVALID, "%s: weights are fp32 or of the rows' type", who);
+  if (n < 0 || k < 1 || n > INT32_MAX / k || D < 1) return fail(QINCO_ERR_INVALID, "%s: need n >= 0, k >= 1, n k < 2^31, D >= 1", who);
+  return QINCO_OK;
+}
+
+extern "C" int qinco_group_combine(const void* y, int dtype, int64_t y_stride, int32_t D, const void* weights, int w_dtype,
+                                   const int32_t* place, int64_t n, int32_t k, void* out, void* stream) {
+  if (int rc = check_rows("qinco_group_combine", dtype, w_dtype, weights != nullptr, n, k, D)) return rc;
+  if (y_stride < 0) return fail(QINCO_ERR_INVALID, "qinco_group_combine: negative stride");
+  if (n == 0) return QINCO_OK;
+  if (!y || !place || !out) return fail(QINCO_ERR_INVALID, "qinco_group_combine: null buffer");
+  const int size = size_of(dtype), unit = unit_of((int64_t)D * size, {y_stride * size}, {y, out});
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  with_type(dtype, unit, [&](auto t, auto e) {
+    using T = decltype(t);
+    constexpr int E = decltype(e)::value;
+    const GroupRows g = group_rows_of(place, nullptr, n, k, D / E);
+    hipLaunchKernelGGL((group_combine_kernel<T, E>), group_grid(g), dim3(256), 0, st, g, (const T*)y, (long)y_stride, weights, w_dtype, (T*)out);
+  });
+  HIP_TRY(hipGetLastError());
+  return QINCO_OK;
+}
+
+extern "C" int qinco_group_combine_grad(const void* dout, int64_t dout_stride, const void* y, int64_t y_stride, int dtype, int32_t D,
+                                        const void* weights, int w_dtype, const int32_t* place, const int32_t* end, int64_t n, int32_t k,
+                                        void* dy, void* dw, void* stream) {
+  if (int rc = check_rows("qinco_group_combine_grad", dtype, w_dtype, true, n, k, D)) return rc;
+  if (y_stride < 0 || dout_stride < 0) return fail(QINCO_ERR_INVALID, "qinco_group_combine_grad: negative stride");
+  if (n == 0) return QINCO_OK;
+  if (!dout || !y || !weights || !place || !end || (!dy && !dw)) return fail(QINCO_ERR_INVALID, "qinco_group_combine_grad: null buffer");
+  const int size = size_of(dtype), unit = unit_of((int64_t)D * size, {y_stride * size, dout_stride * size}, {dout, y, dy});
+  hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+  with_type(dtype, unit, [&](auto t, auto e) {
+    using T = decltype(t);
+    constexpr int E = decltype(e)::value;
+    const GroupRows g = group_rows_of(place, end, n, k, D / E);
+    if (w_dtype == QINCO_T_F32)
+      hipLaunchKernelGGL((group_combine_grad_kernel<T, E, float>), group_grid(g), dim3(256), 0, st, g, (const T*)dout, (long)dout_stride,
+                         (const T*)y, (long)y_stride, (const float*)weights, (T*)dy, (float*)dw);
+    else
+      hipLaunchKernelGGL((group_combine_grad_kernel<T, E, T>), group_grid(g), dim3(256), 0, st, g, (const T*)dout, (long)dout_stride,
+                         (const T*)y, (long)y_stride, (const T*)weights, (T*)dy, (T*)dw);
+  });
+  HIP_TRY(hipGetLastError());
+  return QINCO_OK;
+}

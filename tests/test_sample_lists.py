@@ -1,0 +1,552 @@
+"""Codes drawn from logits (qinco_amd.sample) and rows grouped by inverted list (qinco_amd.lists) against plain statements of both in 64
+bits; their refusals; and a run of them together with the look-up decoder and the k-nearest-list search."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+gpu = pytest.mark.gpu
+HALF = {"float32": 2.0 ** -24, "float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}   # half a step relative to the value
+
+
+# ------------------------------------------------------------------------------------------------ plain statements
+def draw_codes(z, u, T, k, p, m):
+    """z (n, V) float64; settings per row.  -> codes, log probabilities in 64 bits."""
+    n, V = z.shape
+    codes, logps = np.full(n, -1, np.int64), np.full(n, -np.inf)
+    T, k, p, m = (np.broadcast_to(np.asarray(v, np.float64), (n,)) for v in (T, k, p, m))
+    for r in range(n):
+        at = np.flatnonzero(z[r] > -np.inf)        # (NaN compares false)
+        if not len(at):
+            continue
+        at = at[np.argsort(-z[r][at], kind="stable")]
+        if T[r] <= 0:
+            codes[r], logps[r] = at[0], 0.0
+            continue
+        if 0 < k[r] < V:
+            at = at[: int(k[r])]
+        top = z[r][at[0]]
+        with np.errstate(invalid="ignore", over="ignore"):
+            e = np.where(z[r][at] == top, 1.0, np.exp((z[r][at] - top) / T[r]))
+        mass = np.cumsum(e)
+        if p[r] < 1:
+            before = np.concatenate([[0.0], mass[:-1]])
+            stay = before < p[r] * mass[-1]
+            stay[0] = True
+            at, e = at[stay], e[stay]
+        at, e = at[e >= min(m[r], 1.0)], e[e >= min(m[r], 1.0)]
+        back = np.argsort(at)
+        at, e = at[back], e[back]
+        mass = np.cumsum(e)
+        i = min(int(np.searchsorted(mass, min(max(u[r], 0.0), 1.0) * mass[-1], side="right")), int(np.flatnonzero(e).max()))
+        codes[r], logps[r] = at[i], np.log(e[i] / mass[-1])
+    return codes, logps
+
+
+def sort_entries(ids, E):
+    """ids (n, k) -> order, place, offsets by definition."""
+    flat = np.asarray(ids).astype(np.int64).reshape(-1)
+    entries = np.flatnonzero((flat >= 0) & (flat < E))
+    entries = entries[np.argsort(flat[entries], kind="stable")]
+    order, place = np.full(flat.size, -1, np.int64), np.full(flat.size, -1, np.int64)
+    order[: len(entries)] = entries
+    place[entries] = np.arange(len(entries))
+    return order, place.reshape(np.shape(ids)), np.searchsorted(flat[entries], np.arange(E + 1))
+
+
+def to64(t):
+    return t.detach().double().cpu().numpy()
+
+
+# ------------------------------------------------------------------------------------------------ CPU: refusals, sizes
+@pytest.fixture(scope="module")
+def lib():
+    from qinco_amd import _lib, build
+    build.build()
+    return _lib.load()
+
+
+def test_sample_refusals_are_decided_on_the_host(lib):
+    from qinco_amd import _lib
+    P = _lib.QincoSampleParams
+    buf = (C.c_char * 64)()
+    at = C.addressof(buf)
+
+    def call(dtype=0, stride=8, n=1, V=8, params=None, codes=0, logits=at, u=at, out=at):
+        params = P(struct_bytes=C.sizeof(P), temperature=1.0, top_p=1.0) if params is None else params
+        return lib.qinco_sample_codes(logits, dtype, stride, n, V, u, 0, C.byref(params), out, codes, None, None, 0, None)
+    assert call(n=0) == 0                                        # nothing to do: no launch
+    for bad in (dict(dtype=3), dict(V=0), dict(V=(1 << 24) + 1), dict(n=-1), dict(n=1 << 31), dict(stride=-1), dict(codes=_lib.CODE_U8),
+                dict(logits=None), dict(u=None), dict(out=None), dict(params=P(struct_bytes=8))):
+        assert call(**bad) == -1, bad
+        assert b"qinco_sample_codes" in lib.qinco_last_error()
+    assert lib.qinco_sample_workspace(-1, 8) == 0 and lib.qinco_sample_workspace(4, 0) == 0
+    assert lib.qinco_sample_codes(at, 0, 8, 1, 8, at, 0, None, at, 0, None, None, 0, None) == -1
+
+
+def test_group_refusals_are_decided_on_the_host(lib):
+    buf = (C.c_char * 64)()
+    at = C.addressof(buf)
+
+    def call(code=0, stride=1, n=4, k=1, E=8, lists=at, order=at, place=at, offsets=at, ws=at, ws_bytes=1 << 30):
+        return lib.qinco_group_rows(lists, code, stride, n, k, E, order, place, offsets, None, ws, ws_bytes, None)
+    for bad in (dict(code=3), dict(n=-1), dict(k=0), dict(n=1 << 30, k=4), dict(E=0), dict(E=(1 << 24) + 1), dict(stride=-1), dict(lists=None),
+                dict(order=None), dict(place=None), dict(offsets=None), dict(ws=None), dict(ws_bytes=8)):
+        assert call(**bad) == -1, bad
+        assert b"qinco_group_rows" in lib.qinco_last_error()
+    assert lib.qinco_group_workspace(-1, 8) == 0 and lib.qinco_group_workspace(4, 0) == 0 and lib.qinco_group_workspace(4, 1 << 25) == 0
+    assert lib.qinco_group_workspace(0, 1) > 0
+
+    def gather(x=at, xs=4, rb=4, place=at, end=at, n=2, k=2, out=at):
+        return lib.qinco_group_gather(x, xs, rb, place, end, n, k, out, None)
+    assert gather(n=0) == 0
+    for bad in (dict(x=None), dict(xs=-1), dict(rb=0), dict(rb=1 << 31), dict(place=None), dict(end=None), dict(n=-1), dict(k=0), dict(out=None),
+                dict(n=1 << 30, k=2)):
+        assert gather(**bad) == -1, bad
+
+    def combine(y=at, dt=0, ys=4, D=4, w=at, wdt=0, place=at, n=2, k=2, out=at):
+        return lib.qinco_group_combine(y, dt, ys, D, w, wdt, place, n, k, out, None)
+    assert combine(n=0) == 0
+    for bad in (dict(y=None), dict(dt=5), dict(ys=-1), dict(D=0), dict(wdt=1), dict(dt=1, wdt=2), dict(place=None), dict(n=-1), dict(k=0),
+                dict(out=None)):
+        assert combine(**bad) == -1, bad
+
+    def grad(d=at, ds=4, y=at, ys=4, dt=0, D=4, w=at, wdt=0, place=at, end=at, n=2, k=2, dy=at, dw=at):
+        return lib.qinco_group_combine_grad(d, ds, y, ys, dt, D, w, wdt, place, end, n, k, dy, dw, None)
+    assert grad(n=0) == 0
+    for bad in (dict(d=None), dict(ds=-1), dict(y=None), dict(ys=-1), dict(dt=3), dict(D=0), dict(w=None), dict(wdt=2), dict(place=None),
+                dict(end=None), dict(n=-1), dict(k=0), dict(dy=None, dw=None)):
+        assert grad(**bad) == -1, bad
+
+
+def test_host_tensors_are_refused():
+    import torch
+    from qinco_amd import RowGroups, group_rows, sample_codes
+    with pytest.raises(ValueError, match="logits must be a torch CUDA tensor"):
+        sample_codes(torch.zeros(2, 8), torch.zeros(2))
+    with pytest.raises(ValueError, match="lists must be a torch CUDA tensor"):
+        group_rows(torch.zeros(4, dtype=torch.int64), 8)
+    with pytest.raises(ValueError, match="order must be a torch CUDA tensor"):
+        RowGroups(*(torch.zeros(s, dtype=torch.int32) for s in ((4,), (4, 1), (9,))))
+
+
+# ------------------------------------------------------------------------------------------------ sampling
+def check_sample(z, u, *, T=1.0, k=0, p=1.0, m=0.0, code_dtype=np.int64):
+    """z: CUDA (n, V); settings numbers or numpy arrays (n,).  The drawn codes equal the plain statement's; the log probabilities are
+    theirs within the rounding to 32 bits (the 64-bit value itself is good to V 2^-42 of the mass)."""
+    import torch
+    from qinco_amd import sample_codes
+    rows = {}
+    for name, v, dt in (("temperature", T, torch.float32), ("top_k", k, torch.int32), ("top_p", p, torch.float32), ("min_p", m, torch.float32)):
+        rows[name] = torch.as_tensor(v).to("cuda", dt) if isinstance(v, np.ndarray) else v
+    codes, logp = sample_codes(z, u, code_dtype=code_dtype, return_logp=True, **rows)
+    assert codes.dtype == (torch.int64 if code_dtype is np.int64 else torch.int32) and logp.dtype == torch.float32
+    plain = [to64(v) if torch.is_tensor(v) else v for v in rows.values()]
+    want, want_logp = draw_codes(to64(z), to64(u), *plain)
+    got = codes.cpu().numpy()
+    assert np.array_equal(got, want), (np.flatnonzero(got != want)[:5], got[got != want][:5], want[got != want][:5])
+    gl, fin = to64(logp), np.isfinite(want_logp)
+    assert np.array_equal(gl[~fin], want_logp[~fin])
+    assert np.all(np.abs(gl[fin] - want_logp[fin]) <= 2.0 ** -24 * np.abs(want_logp[fin]) + z.shape[1] * 2.0 ** -42 + 1e-12)
+    return codes
+
+
+SETTINGS = [dict(), dict(T=0.7, k=5), dict(p=0.9), dict(m=0.05), dict(T=1.3, k=50, p=0.8, m=0.01), dict(T=0.0), dict(k=1), dict(p=0.0), dict(m=1.0),
+            dict(p=1e-6), dict(T=1e-3, k=3, p=0.99)]
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("n,V", [(1, 1), (3, 2), (5, 63), (4, 64), (4, 65), (300, 256), (7, 257), (3, 1000), (5, 1024), (5, 1025), (6, 4099),
+                                 (2, 16384), (2, 16385), (2, 32769), (2, 70001), (1, (1 << 20) + 3)])
+def test_sample_sizes_and_settings(dtype, n, V):
+    import torch
+    g = torch.Generator("cuda").manual_seed(n * 1000003 + V)
+    for i, s in enumerate(SETTINGS if V < 100000 else SETTINGS[:5]):
+        z = (torch.randn(n, V, generator=g, device="cuda") * 2.5).to(getattr(torch, dtype))
+        check_sample(z, torch.rand(n, generator=g, device="cuda"), **s)
+
+
+@gpu
+def test_sample_masks_infinities_nan_and_ties():
+    import torch
+    g = torch.Generator("cuda").manual_seed(5)
+    inf, low = float("inf"), torch.finfo(torch.float32).min
+    for V in (2, 64, 200, 256, 1500, 40000):
+        z = torch.randn(40, V, generator=g, device="cuda")
+        z[0] = -inf                                    # nothing left
+        z[1] = float("nan")
+        z[2] = low                                     # the type's lowest value everywhere: a uniform row
+        z[3] = low
+        z[3, V // 2] = 0.0                             # ... everywhere but at one place
+        z[4] = -inf
+        z[4, V - 1] = -7.0                             # one code left
+        z[5, ::2] = float("nan")
+        z[6, 1::2] = -inf
+        z[7, V // 2] = inf                             # all the mass at infinity, once
+        z[8] = inf                                     # ... and everywhere
+        z[9] = 0.0
+        z[9, ::2] = -0.0                               # equal logits: -0 is 0
+        z[10] = torch.randint(0, 3, (V,), generator=g, device="cuda").float()      # ties everywhere
+        z[11] = 3e38
+        z[11, 0] = -3e38
+        z[12] = torch.randint(0, 100, (V,), generator=g, device="cuda") * 1.4e-45  # denormal logits
+        z[13] = -inf
+        z[13, 0] = low
+        z[14] = torch.arange(V, device="cuda").float()
+        z[15] = -torch.arange(V, device="cuda").float()
+        z[16:24] = torch.randint(-2, 3, (8, V), generator=g, device="cuda").float()
+        z[24:28, : V // 2] = -inf
+        for s in SETTINGS:
+            u = torch.rand(40, generator=g, device="cuda")
+            u[20:24] = torch.tensor([0.0, 1.0 - 2.0 ** -24, 0.5, 2.0 ** -30])
+            check_sample(z, u, **s)
+
+
+@gpu
+def test_sample_borders_fall_on_the_exact_side():
+    """256 equal logits: the running mass passes u = j / 256 only behind code j; a distribution drawn at evenly spaced numbers has every
+    code as often as its mass says, to within one."""
+    import torch
+    from qinco_amd import sample_codes
+    for dt in (torch.float64, torch.float32):
+        u = torch.arange(256, device="cuda", dtype=dt) / 256
+        got = sample_codes(torch.zeros(256, 256, device="cuda"), u)
+        assert got.tolist() == list(range(256))
+    assert sample_codes(torch.zeros(5, 256, device="cuda"), torch.tensor([-1.0, float("nan"), 1.0, 7.0, float("inf")], device="cuda")).tolist() == [0, 0, 255, 255, 255]
+    n = 20000
+    z = torch.randn(1, 100, generator=torch.Generator("cuda").manual_seed(1), device="cuda")
+    got = np.bincount(sample_codes(z.expand(n, 100), (torch.arange(n, device="cuda", dtype=torch.float64) + 0.5) / n).cpu().numpy(), minlength=100)
+    e = np.exp(to64(z)[0] - to64(z).max())
+    assert np.all(np.abs(got - n * e / e.sum()) <= 1.0)
+
+
+@gpu
+def test_sample_settings_per_row_strides_and_types():
+    import torch
+    from qinco_amd import sample_codes
+    rs = np.random.RandomState(3)
+    g = torch.Generator("cuda").manual_seed(3)
+    for n, V in ((70, 256), (9, 3000), (3, 50001)):
+        T = rs.uniform(0.2, 2, n).astype(np.float32)
+        T[0], T[1] = 0.0, -1.0
+        k = rs.randint(-1, 60, n).astype(np.int32)
+        p = rs.uniform(0.1, 1.2, n).astype(np.float32)
+        m = rs.uniform(-0.1, 0.3, n).astype(np.float32)
+        wide = torch.randn(n, V + 7, generator=g, device="cuda") * 3
+        z = wide[:, 3:3 + V]                                        # rows that start anywhere
+        u = torch.rand(2 * n, generator=g, device="cuda", dtype=torch.float64)[::2]
+        a = check_sample(z, u, T=T, k=k, p=p, m=m)
+        b = check_sample(z.T.contiguous().T, u, T=T, k=k, p=p, m=m, code_dtype=np.int32)   # neighbouring codes far apart
+        assert torch.equal(a, b.long())
+        one = torch.cat([sample_codes(z[i:i + 1], u[i:i + 1], temperature=torch.from_numpy(T[i:i + 1]).cuda(),
+                                      top_k=torch.from_numpy(k[i:i + 1]).cuda(), top_p=torch.from_numpy(p[i:i + 1]).cuda(),
+                                      min_p=torch.from_numpy(m[i:i + 1]).cuda()) for i in range(n)])
+        assert torch.equal(a, one)                                  # a row's code does not depend on its batch
+    assert sample_codes(torch.zeros(0, 16, device="cuda"), torch.zeros(0, device="cuda")).shape == (0,)
+
+
+@gpu
+def test_sample_refuses():
+    import torch
+    from qinco_amd import sample_codes
+    z, u = torch.zeros(4, 8, device="cuda"), torch.zeros(4, device="cuda")
+    for bad in (dict(temperature=-1.0), dict(temperature=math.inf), dict(temperature=math.nan), dict(top_p=math.nan), dict(min_p=1.5),
+                dict(code_dtype=np.uint8), dict(top_k=torch.zeros(4, device="cuda")), dict(top_p=torch.zeros(3, device="cuda")),
+                dict(temperature=torch.ones(4)), dict(min_p=torch.zeros(4, device="cuda", dtype=torch.float64))):
+        with pytest.raises(ValueError):
+            sample_codes(z, u, **bad)
+    for args in ((z[0], u), (z.long(), u), (z.double(), u), (z[:, :0], u), (z, u[:3]), (z, u.half()), (z, u.cpu())):
+        with pytest.raises(ValueError):
+            sample_codes(*args)
+
+
+# ------------------------------------------------------------------------------------------------ grouping
+def check_group(ids, E, **kw):
+    from qinco_amd import group_rows
+    g = group_rows(ids, E, **kw)
+    order, place, offsets = sort_entries(ids.cpu().numpy() if ids.dim() == 2 else ids.cpu().numpy()[:, None], E)
+    assert np.array_equal(g.order.cpu().numpy(), order)
+    assert np.array_equal(g.place.cpu().numpy(), place)
+    assert np.array_equal(g.offsets.cpu().numpy(), offsets)
+    assert np.array_equal(g.counts().cpu().numpy(), np.diff(offsets))
+    return g
+
+
+@gpu
+@pytest.mark.parametrize("N", [0, 1, 63, 64, 65, 511, 513, 4095, 4096, 4097, 8193, 100003])
+def test_group_sizes(N):
+    import torch
+    g = torch.Generator("cuda").manual_seed(N)
+    for E in (1, 2, 255, 256, 257, 2047, 2048, 2049, 4096, 4097, 65536, 1 << 20, (1 << 22) + 1, 1 << 24):
+        if E > 1 << 20 and N not in (65, 4097, 100003):
+            continue
+        ids = torch.randint(0, E, (N,), generator=g, device="cuda")
+        check_group(ids, E)
+        if N:
+            ids[torch.rand(N, generator=g, device="cuda") < 0.2] = -1 - E
+            check_group(ids.int(), E)
+    if N:
+        check_group(torch.full((N,), 300, device="cuda"), 512)                       # one list takes all
+        check_group(torch.full((N,), -1, device="cuda"), 70000)                      # nothing has a list
+        check_group(torch.full((N,), 99999, device="cuda"), 100000)
+        check_group(torch.arange(N, device="cuda").flip(0), N)
+        check_group(torch.randint(0, 256, (N,), generator=g, device="cuda").to(torch.uint8), 256)
+
+
+@gpu
+def test_group_matrices_columns_and_bad_ids():
+    import torch
+    from qinco_amd import group_rows
+    g = torch.Generator("cuda").manual_seed(2)
+    for n, k, E in ((1, 1, 1), (7, 3, 5), (1000, 8, 1024), (2049, 16, 77), (30000, 5, 1 << 18)):
+        ids = torch.randint(-1, E, (n, k), generator=g, device="cuda")
+        check_group(ids, E)
+        wide = torch.randint(0, E, (n, k + 4), generator=g, device="cuda")
+        check_group(wide[:, 2:2 + k], E)                                             # rows further apart than their ids
+        check_group(wide[:, 1], E)                                                   # a column of a code matrix
+        check_group(wide[:, ::2], E)
+        check_group(wide[:1].expand(n, -1), E)
+    ids = torch.tensor([[0, 5], [9, -1], [1 << 40, 2]], device="cuda")
+    with pytest.raises(IndexError, match="n_lists"):
+        group_rows(ids, 9)
+    check_group(ids, 9, check=False)                                                 # ... or counts as having no list
+    for args in ((ids.float(), 9), (ids, 0), (ids, (1 << 24) + 1), (ids[None], 9), (ids[:, :0], 9), (ids.cpu(), 9)):
+        with pytest.raises(ValueError):
+            group_rows(*args)
+
+
+def make_groups(g, n, k, E, drop):
+    import torch
+    ids = torch.randint(0, E, (n, k), generator=g, device="cuda")
+    if drop:
+        ids[torch.rand(n, k, generator=g, device="cuda") < 0.3] = -1
+        ids[n // 2] = -1                                                             # a row without any list
+    from qinco_amd import group_rows
+    return group_rows(ids, E)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+@pytest.mark.parametrize("n,k,D", [(1, 1, 1), (5, 1, 3), (33, 2, 8), (64, 3, 96), (100, 8, 128), (77, 9, 101), (300, 16, 100), (50, 4, 768),
+                                   (20, 17, 1023), (3000, 2, 256), (9, 33, 2)])
+def test_gather_and_combine_with_gradients(dtype, n, k, D):
+    """Against the formulas in 64 bits.  A sum of k products in 32 bits, in order: (k + 1) 2^-24 of the sum of absolute products; a dot
+    product of D: D 2^-24 of the same; a product: 2^-24 of itself; and half a step of the type at the end (for fp16 2^-25 below its
+    normal range)."""
+    import torch
+    g = torch.Generator("cuda").manual_seed(n * 131 + k * 17 + D)
+    dt, half = getattr(torch, dtype), HALF[dtype]
+    tiny = 2.0 ** -25 if dtype == "float16" else 0.0
+    for drop in (False, True):
+        gr = make_groups(g, n, k, 50, drop)
+        place = gr.place.cpu().numpy()
+        used = place >= 0
+        at = np.where(used, place, 0)
+        x = torch.randn(n, D, generator=g, device="cuda").to(dt).requires_grad_()
+        out = gr.gather(x)
+        want = np.zeros((n * k, D))
+        want[place[used]] = np.repeat(to64(x), k, 0)[used.reshape(-1)]
+        assert np.array_equal(to64(out), want)
+        dout = torch.randn(n * k, D, generator=g, device="cuda").to(dt)
+        dx, = torch.autograd.grad(out, x, dout)
+        terms = np.where(used[:, :, None], to64(dout)[at], 0.0)
+        assert dx.dtype == dt and np.all(np.abs(to64(dx) - terms.sum(1)) <= (k + 1) * 2.0 ** -24 * np.abs(terms).sum(1) + half * np.abs(terms.sum(1)) + tiny)
+        for wdt in {torch.float32, dt}:
+            y = torch.randn(n * k, D, generator=g, device="cuda").to(dt)
+            y[gr.order < 0] = float("nan")                                           # rows no entry owns: whatever was there
+            w = torch.softmax(torch.randn(n, k, generator=g, device="cuda"), 1).to(wdt)
+            w[gr.place < 0] = float("nan")
+            y.requires_grad_(), w.requires_grad_()
+            out = gr.combine(y, w)
+            y64, w64 = np.where(used[:, :, None], to64(y)[at], 0.0), np.where(used, to64(w), 0.0)
+            terms = w64[:, :, None] * y64
+            assert out.dtype == dt and np.all(np.abs(to64(out) - terms.sum(1)) <= (k + 1) * 2.0 ** -24 * np.abs(terms).sum(1) + half * np.abs(terms.sum(1)) + tiny)
+            d = torch.randn(n, D, generator=g, device="cuda").to(dt)
+            dy, dw = torch.autograd.grad(out, (y, w), d, retain_graph=True)
+            d64 = to64(d)
+            want = np.zeros((n * k, D))
+            want[place[used]] = (w64[:, :, None] * d64[:, None])[used]
+            assert dy.dtype == dt and np.all(np.abs(to64(dy) - want) <= (half + 2.0 ** -24) * np.abs(want) * (1 + 2.0 ** -20) + tiny)
+            terms = d64[:, None] * y64
+            tol = D * 2.0 ** -24 * np.abs(terms).sum(2) + (HALF[str(wdt)[6:]] if wdt != torch.float32 else 2.0 ** -24) * np.abs(terms.sum(2)) + (2.0 ** -25 if wdt == torch.float16 else 0)
+            assert dw.dtype == wdt and np.all(np.abs(to64(dw) - terms.sum(2)) <= tol)
+            assert torch.equal(torch.autograd.grad(out, y, d, retain_graph=True)[0], dy) and torch.equal(torch.autograd.grad(out, w, d)[0], dw)
+        y = torch.randn(n * k, D, generator=g, device="cuda").to(dt).requires_grad_()
+        out = gr.combine(y)
+        terms = np.where(used[:, :, None], to64(y)[at], 0.0)
+        assert np.all(np.abs(to64(out) - terms.sum(1)) <= (k + 1) * 2.0 ** -24 * np.abs(terms).sum(1) + half * np.abs(terms.sum(1)) + tiny)
+        dy, = torch.autograd.grad(out, y, d)
+        want = np.zeros((n * k, D))
+        want[place[used]] = np.repeat(d64, k, 0)[used.reshape(-1)]
+        assert np.array_equal(to64(dy), want)
+
+
+@gpu
+def test_gradients_against_differences():
+    """Both operators are linear in the rows and in the weights: the difference over a step of 1 along a direction is the gradient's
+    product with it, up to the rounding of two sums of some thousand terms of size 1 in 32 bits."""
+    import torch
+    g = torch.Generator("cuda").manual_seed(8)
+    gr = make_groups(g, 60, 4, 30, True)
+    rand = lambda *s: torch.randn(*s, generator=g, device="cuda")          # noqa: E731
+    x, y, w, c, ck = rand(60, 40), rand(240, 40), rand(60, 4), rand(60, 40), rand(240, 40)
+    for f, t in ((lambda v: (gr.gather(v).double() * ck).sum(), x), (lambda v: (gr.combine(v, w).double() * c).sum(), y),
+                 (lambda v: (gr.combine(y, v).double() * c).sum(), w)):
+        v = t.clone().requires_grad_()
+        grad, = torch.autograd.grad(f(v), v)
+        step = rand(*t.shape)
+        diff = float(f(t + step) - f(t))
+        assert abs(diff - float((grad.double() * step).sum())) <= 1e-2, diff
+
+
+@gpu
+def test_rows_of_any_type_stride_and_broadcast_gradients():
+    import torch
+    g = torch.Generator("cuda").manual_seed(4)
+    n, k = 501, 3
+    gr = make_groups(g, n, k, 40, True)
+    order = gr.order.cpu().numpy()
+    for dt in (torch.uint8, torch.int32, torch.int64, torch.float64, torch.bool):
+        for D in (1, 7, 8, 9, 16, 33):
+            x = torch.randint(0, 100, (n, D + 5), generator=g, device="cuda").to(dt)
+            for v in (x[:, :D], x[:, 2:2 + D], x.T.contiguous().T[:, :D], x[:1, :D].expand(n, D)):
+                got = gr.gather(v).cpu().numpy()
+                want = np.where((order >= 0)[:, None], v.cpu().numpy()[order // k], np.zeros((), got.dtype))
+                assert np.array_equal(got, want)
+    y = torch.randn(n * k, 24, generator=g, device="cuda")
+    w = torch.rand(n, k, generator=g, device="cuda")
+    base = gr.combine(y[:, 3:19].contiguous(), w)
+    assert torch.equal(gr.combine(y[:, 3:19], w), base)                              # rows off their natural alignment: the same bits
+    assert torch.equal(gr.combine(y.T.contiguous().T[:, 3:19], w.T.contiguous().T), base)
+    leaf = y.clone().requires_grad_()
+    gr.combine(leaf[:, 3:19], w).sum().backward()                                    # a gradient broadcast from one number
+    want = np.zeros((n * k, 24))
+    want[:, 3:19] = np.where((order >= 0)[:, None], to64(w).reshape(-1)[order][:, None], 0.0)
+    assert np.array_equal(to64(leaf.grad), want)
+    x = torch.randn(n, 16, generator=g, device="cuda", requires_grad=True)
+    gr.gather(x).sum().backward()
+    assert np.array_equal(to64(x.grad), np.repeat((gr.place.cpu().numpy() >= 0).sum(1)[:, None], 16, 1))
+    shared = torch.randn(1, 16, generator=g, device="cuda", requires_grad=True)      # one row for all
+    gr.gather(shared.expand(n, 16)).sum().backward()
+    assert np.array_equal(to64(shared.grad)[0], np.full(16, float((gr.place >= 0).sum())))
+    with pytest.raises(ValueError):
+        gr.gather(torch.randn(n, 4, device="cuda", dtype=torch.float64, requires_grad=True))
+    for call in (lambda: gr.gather(x[:-1]), lambda: gr.gather(x[:, :0]), lambda: gr.gather(x.cpu()), lambda: gr.combine(y[:-1]),
+                 lambda: gr.combine(y.double()), lambda: gr.combine(y, w[:-1]), lambda: gr.combine(y, w.half()), lambda: gr.combine(y, w.cpu())):
+        with pytest.raises(ValueError):
+            call()
+
+
+@gpu
+def test_no_rows():
+    import torch
+    from qinco_amd import group_rows
+    gr = group_rows(torch.zeros(0, 3, dtype=torch.int64, device="cuda"), 17)
+    assert gr.offsets.tolist() == [0] * 18
+    x = torch.zeros(0, 5, device="cuda", requires_grad=True)
+    out = gr.combine(gr.gather(x), torch.zeros(0, 3, device="cuda"))
+    assert out.shape == (0, 5)
+    out.sum().backward()
+    assert x.grad.shape == (0, 5)
+
+
+# ------------------------------------------------------------------------------------------------ streams, graphs, together
+@gpu
+def test_streams_and_two_calls_at_once():
+    import torch
+    from qinco_amd import group_rows, sample_codes
+    g = torch.Generator("cuda").manual_seed(6)
+    jobs = []
+    for i, (n, V, E) in enumerate(((3000, 256, 1 << 20), (2, 300000, 700), (40, 5000, 5000))):
+        z, u = torch.randn(n, V, generator=g, device="cuda") * 3, torch.rand(n, generator=g, device="cuda")
+        ids = torch.randint(0, E, (20000 + i, 2), generator=g, device="cuda")
+        jobs.append((z, u, ids, E))
+    work = lambda z, u, ids, E: (sample_codes(z, u, top_k=100, top_p=0.9), *(lambda q: (q.order, q.place, q.offsets))(group_rows(ids, E, check=False)))  # noqa: E731
+    want = [work(*j) for j in jobs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for _ in range(3):
+        got = []
+        for s, j in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                got.append(work(*j))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for x, y in zip(got, want) for a, b in zip(x, y))
+
+
+@gpu
+def test_two_graphs_replay_the_eager_results():
+    """Two captured runs of everything, replayed in turn with new inputs and eager work between them."""
+    import torch
+    from qinco_amd import group_rows, sample_codes
+    g = torch.Generator("cuda").manual_seed(7)
+    sizes = ((600, 256, 4, 16), (5, 150000, 3, 100))
+
+    def inputs(n, V, k, D):
+        return (torch.randn(n, V, generator=g, device="cuda") * 2, torch.rand(n, generator=g, device="cuda"),
+                torch.randint(-1, 5000, (n * 50, k), generator=g, device="cuda"), torch.randn(n * 50, D, generator=g, device="cuda"))
+
+    def work(z, u, ids, x):
+        codes = sample_codes(z, u, top_k=40, top_p=0.9, min_p=0.001)
+        gr = group_rows(ids, 5000, check=False)
+        rows = gr.gather(x)
+        return codes, gr.order, gr.offsets, rows, gr.combine(rows, torch.ones_like(ids, dtype=torch.float32))
+    static = [inputs(*s) for s in sizes]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for s in static:
+            work(*s)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for s in static:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(work(*s))
+        graphs.append(graph)
+    for _ in range(4):
+        for i in (0, 1):
+            for t, v in zip(static[i], inputs(*sizes[i])):
+                t.copy_(v)
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        for i in (0, 1):
+            assert all(torch.equal(a, b) for a, b in zip(outs[i], work(*static[i])))
+
+
+@gpu
+def test_together_with_the_search_and_the_look_up_decoder():
+    """Codes drawn step by step from a prior's logits, decoded by the look-up decoder, the reconstructions sent to their two nearest lists
+    (k-nearest-list search), scaled there and brought back with weights."""
+    import torch
+    from qinco_amd import group_rows, sample_codes
+    from qinco_amd.lut import LutDecoder
+    from qinco_amd.search import KnnSearcher
+    g = torch.Generator("cuda").manual_seed(9)
+    n, M, K, D, E = 700, 4, 256, 32, 100
+    u = torch.rand(M, n, generator=g, device="cuda")
+    logits = torch.randn(M, n, K, generator=g, device="cuda") * 2
+    codes = torch.stack([sample_codes(logits[s], u[s], top_p=0.9) for s in range(M)], 1)
+    tables = torch.randn(M, K, D, generator=g, device="cuda")
+    dec = LutDecoder(tables.cpu().numpy(), a=np.arange(M))
+    x = dec(codes)
+    want = sum(to64(tables)[s][codes[:, s].cpu().numpy()] for s in range(M))
+    assert np.abs(to64(x) - want).max() <= M * 2.0 ** -24 * np.abs(to64(tables)).max() * M
+    centroids = torch.randn(E, D, generator=g, device="cuda")
+    knn = KnnSearcher(D)
+    ids, dist = knn.search(centroids, x, k=2, return_dist=True)
+    gr = check_group(ids, E)
+    scale = torch.rand(E, generator=g, device="cuda") + 0.5
+    w = torch.softmax(-dist, 1)
+    rows = gr.gather(x)
+    of_list = torch.repeat_interleave(torch.arange(E, device="cuda"), gr.counts().long())
+    out = gr.combine(rows * scale[of_list][:, None], w)
+    factor = (to64(w) * to64(scale)[ids.cpu().numpy()]).sum(1)
+    assert np.abs(to64(out) - factor[:, None] * to64(x)).max() <= 8 * 2.0 ** -24 * np.abs(factor[:, None] * to64(x)).max()
+    first = check_group(codes[:, 0], K)                                              # an index's rows by their first code
+    moved = first.gather(codes.to(torch.uint8))
+    assert bool((moved[:, 0].diff().int() >= 0).all())
+    knn.close(), dec.close()
