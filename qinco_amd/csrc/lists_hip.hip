@@ -33,6 +33,21 @@ extern "C" int64_t qinco_sample_workspace(int64_t n, int64_t V) {
   return 0;
 }
 
+template <typename T, int R>
+static void launch_sample_wave(const SampleArgs& a, hipStream_t st) {
+  long g = (a.n + kSampleRowWaves - 1) / kSampleRowWaves;
+  if (g > 1 << 20) g = 1 << 20;
+  hipLaunchKernelGGL((sample_wave_kernel<T, R>), dim3((unsigned)g), dim3(64 * kSampleRowWaves), 0, st, a);
+}
+
+template <typename T>
+static void launch_sample(const SampleArgs& a, hipStream_t st) {
+  if (a.V <= 64) launch_sample_wave<T, 1>(a, st);
+  else if (a.V <= 256) launch_sample_wave<T, 4>(a, st);
+  else if (a.V <= 1024) launch_sample_wave<T, 16>(a, st);
+  else hipLaunchKernelGGL(sample_row_kernel<T>, dim3((unsigned)(a.n < 65536 ? a.n : 65536)), dim3(kSampleThreads), 0, st, a);
+}
+
 extern "C" int qinco_sample_codes(const void* logits, int dtype, int64_t row_stride, int64_t n, int64_t V, const void* u, int u_is_f64,
                                   const qinco_sample_params* params, void* codes_out, int code_dtype, float* logp_out, void* workspace,
                                   int64_t workspace_bytes, void* stream) {
@@ -54,10 +69,9 @@ extern "C" int qinco_sample_codes(const void* logits, int dtype, int64_t row_str
                params->top_k, params->top_p_rows, params->top_p, params->min_p_rows, params->min_p, codes_out,
                code_dtype == QINCO_CODE_I64, logp_out, 62 - lv < 51 ? 62 - lv : 51};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  const dim3 grid((unsigned)(n < 65536 ? n : 65536)), block(kSampleThreads);
-  if (dtype == QINCO_T_F32) hipLaunchKernelGGL(sample_row_kernel<float>, grid, block, 0, st, a);
-  else if (dtype == QINCO_T_F16) hipLaunchKernelGGL(sample_row_kernel<_Float16>, grid, block, 0, st, a);
-  else hipLaunchKernelGGL(sample_row_kernel<__bf16>, grid, block, 0, st, a);
+  if (dtype == QINCO_T_F32) launch_sample<float>(a, st);
+  else if (dtype == QINCO_T_F16) launch_sample<_Float16>(a, st);
+  else launch_sample<__bf16>(a, st);
   HIP_TRY(hipGetLastError());
   return QINCO_OK;
 }

@@ -86,10 +86,14 @@ __device__ __forceinline__ double sample_arg(unsigned key, unsigned max_key, dou
   if (key == max_key) return 0.0;
   return fmax(((double)sample_unkey(key) - zmax) * invT, -100.0);
 }
-// mass as a whole number of 2^-F; zero for what min-p cuts
+// e = exp(x) as a whole number of 2^-F (scale = 2^F <= 2^51: the sum with 2^52 rounds it to one, ties to even)
+__device__ __forceinline__ unsigned long long sample_whole(double e, double scale) {
+  return (unsigned long long)__double_as_longlong(fma(e, scale, 0x1p52)) & ((1ull << 52) - 1);
+}
+// ... zero for what min-p cuts
 __device__ __forceinline__ unsigned long long sample_mass(double x, double scale, double m) {
   const double e = exp(x);
-  return e >= m ? (unsigned long long)(e * scale + 0.5) : 0ull;
+  return e >= m ? sample_whole(e, scale) : 0ull;
 }
 
 // smallest whole number that is at least p * total: "mass before < p * total" is "mass before < this"
@@ -99,19 +103,70 @@ __device__ __forceinline__ unsigned long long sample_bound(double p, unsigned lo
   return v < 1 ? 1 : (v > total ? total : v);
 }
 
-template <typename T>
-__device__ __forceinline__ T sample_wave_sum(T v) {
-  for (int m = 32; m > 0; m >>= 1) v += __shfl_xor(v, m, 64);
-  return v;
+// Wave-wide sums and scans by DPP (rows of 16 lanes shifted, then broadcast over the rows behind): every lane has to be active.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned sample_dpp(unsigned v) {   // 0 where the step has no source lane
+  return (unsigned)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, false);
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ unsigned long long sample_dpp(unsigned long long v) {
+  return (unsigned long long)sample_dpp<CTRL, ROWS>((unsigned)(v >> 32)) << 32 | sample_dpp<CTRL, ROWS>((unsigned)v);
 }
 template <typename T>
 __device__ __forceinline__ T sample_wave_scan(T v) {   // inclusive
-  const int lane = threadIdx.x & 63;
-  for (int d = 1; d < 64; d <<= 1) {
-    const T o = __shfl_up(v, d, 64);
-    if (lane >= d) v += o;
-  }
+  v += sample_dpp<0x111, 0xf>(v);
+  v += sample_dpp<0x112, 0xf>(v);
+  v += sample_dpp<0x114, 0xf>(v);
+  v += sample_dpp<0x118, 0xf>(v);
+  v += sample_dpp<0x142, 0xa>(v);
+  v += sample_dpp<0x143, 0xc>(v);
   return v;
+}
+__device__ __forceinline__ unsigned sample_lane(unsigned v, int lane) { return (unsigned)__builtin_amdgcn_readlane((int)v, lane); }
+__device__ __forceinline__ unsigned long long sample_lane(unsigned long long v, int lane) {
+  return (unsigned long long)sample_lane((unsigned)(v >> 32), lane) << 32 | sample_lane((unsigned)v, lane);
+}
+template <typename T>
+__device__ __forceinline__ T sample_wave_sum(T v) { return sample_lane(sample_wave_scan(v), 63); }
+__device__ __forceinline__ unsigned sample_wave_max(unsigned v) {
+  v = max(v, sample_dpp<0x111, 0xf>(v));
+  v = max(v, sample_dpp<0x112, 0xf>(v));
+  v = max(v, sample_dpp<0x114, 0xf>(v));
+  v = max(v, sample_dpp<0x118, 0xf>(v));
+  v = max(v, sample_dpp<0x142, 0xa>(v));
+  v = max(v, sample_dpp<0x143, 0xc>(v));
+  return sample_lane(v, 63);
+}
+
+// what the wave's lanes wrote to LDS is there for its other lanes (the LDS executes a wave's accesses in order: nothing to wait for)
+__device__ __forceinline__ void sample_wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// smallest r with r q >= rem (q >= 1, r < 2^25)
+__device__ __forceinline__ unsigned sample_ceil_div(unsigned long long rem, unsigned long long q) {
+  unsigned r = (unsigned)((double)rem / (double)q);
+  while (r * q < rem) ++r;
+  while (r && (r - 1) * q >= rem) --r;
+  return r;
+}
+
+// Bins of the first look at a row: 0 holds the largest logit, the last whatever lies 37 or more below it in units of T (no mass) or
+// the smallest.  fp32 subtraction and product are monotone, so a bin never holds a logit above one of an earlier bin.
+struct SampleBins {
+  float zmax, c;
+  int last;
+};
+__device__ __forceinline__ SampleBins sample_bins(unsigned kmax, unsigned kmin, double invT, int bins) {
+  const float zmax = sample_unkey(kmax);
+  const double range = fmin(((double)zmax - (double)sample_unkey(kmin)) * invT, 37.0);
+  return SampleBins{zmax, range > 0.0 ? (float)(bins * invT / range) : 0.f, bins - 1};
+}
+__device__ __forceinline__ int sample_bin(const SampleBins& b, float z) {
+  const float x = (b.zmax - z) * b.c;
+  return z == b.zmax ? 0 : (int)fminf(x, (float)b.last);
 }
 
 // One workgroup per row, any V: the row is read again for every digit of the two selections (from L2 behind the first time).
@@ -218,9 +273,9 @@ __device__ void sample_one_row(const SampleArgs& a, long row) {
       __syncthreads();
     }
     const unsigned long long q = mass(prefix);   // > 0: the digit walk ends on a key that has mass
-    const unsigned long long need = (bound - before + q - 1) / q;
-    if (prefix == t) r = need < r ? (unsigned)need : r;
-    else r = need < (unsigned)V ? (unsigned)need : (unsigned)V, t = prefix;
+    const unsigned need = sample_ceil_div(bound - before, q);
+    r = prefix == t && r < need ? r : need;
+    t = prefix;
   }
   // mass of the kept codes, wave by wave: wave w owns a run of indexes, so that ties are counted and the draw walks in index order
   const int seg = ((V + kSampleWaves * 64 - 1) / (kSampleWaves * 64)) * 64;
@@ -274,7 +329,7 @@ __device__ void sample_one_row(const SampleArgs& a, long row) {
           sample_answer(a, row, i + lane, (float)(sample_arg(key, kmax, zmax, s.invT) - log((double)total / scale)));
         break;
       }
-      run = __shfl(incl, 63, 64);
+      run = sample_lane(incl, 63);
       tied += __builtin_popcountll(at);
     }
   }
@@ -285,6 +340,226 @@ __global__ void __launch_bounds__(kSampleThreads) sample_row_kernel(SampleArgs a
   for (long row = blockIdx.x; row < a.n; row += gridDim.x) {
     sample_one_row<T>(a, row);
     __syncthreads();
+  }
+}
+
+// One wave per row, V <= 64 R: the row stays in registers (lane l holds codes l R ... l R + R - 1), no barrier anywhere.
+// Both cuts look at 64 bins of the row first (counts and masses by LDS atomics, scanned by the wave), then at the few codes of the one
+// bin that the cut falls into, a lane each.  A bin of more than 64 codes (heavy ties) is searched bit by bit instead.
+constexpr int kSampleRowWaves = 4;
+struct SampleWaveLds {
+  unsigned long long mass[64];
+  unsigned count[64];
+  unsigned long long m_mass[64];   // members of the bin in question
+  unsigned m_key[64];
+};
+
+template <int R>
+struct SampleWaveRow {
+  unsigned key[R];
+  unsigned long long q[R];
+
+  // codes with bin(z) == b into the members' arrays; more than 64: -1
+  __device__ int members(SampleWaveLds& s, const SampleBins& bins, unsigned b) const {
+    const int lane = threadIdx.x & 63;
+    int n = 0;
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const bool in = key[j] > kSampleKeyMasked && (unsigned)sample_bin(bins, sample_unkey(key[j])) == b;
+      const unsigned long long at = __ballot(in);
+      const int to = n + (int)__builtin_popcountll(at & ((1ull << lane) - 1));
+      if (in && to < 64) {
+        s.m_key[to] = key[j];
+        s.m_mass[to] = q[j];
+      }
+      n += (int)__builtin_popcountll(at);
+    }
+    return n <= 64 ? n : -1;
+  }
+};
+
+template <typename T, int R>
+__global__ void __launch_bounds__(64 * kSampleRowWaves) sample_wave_kernel(SampleArgs a) {
+  __shared__ SampleWaveLds lds[kSampleRowWaves];
+  SampleWaveLds& s = lds[threadIdx.x >> 6];
+  const int lane = threadIdx.x & 63, V = a.V;
+  const double scale = ldexp(1.0, a.F);
+  for (long row = (long)blockIdx.x * kSampleRowWaves + (threadIdx.x >> 6); row < a.n; row += (long)gridDim.x * kSampleRowWaves) {
+    const T* z = reinterpret_cast<const T*>(a.logits) + row * a.stride;
+    const SampleRow set = sample_row(a, row);
+    SampleWaveRow<R> w;
+    unsigned hi = 0, lo = 0;   // lo: the smallest key that is not masked, complemented
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const int i = lane * R + j;
+      w.key[j] = i < V ? sample_key(GroupNum<T>::get(z[i])) : kSampleKeyMasked;
+      hi = max(hi, w.key[j]);
+      lo = max(lo, w.key[j] > kSampleKeyMasked ? ~w.key[j] : 0u);
+    }
+    const unsigned kmax = sample_wave_max(hi), kmin = ~sample_wave_max(lo);
+    if (kmax <= kSampleKeyMasked) {
+      if (lane == 0) sample_answer(a, row, -1, -INFINITY);
+      continue;
+    }
+    if (set.greedy) {
+      const int first = __builtin_ctzll(__ballot(hi == kmax));
+      int at = 0;
+#pragma unroll
+      for (int j = R - 1; j >= 0; --j) at = w.key[j] == kmax ? j : at;
+      if (lane == first) sample_answer(a, row, lane * R + at, 0.f);
+      continue;
+    }
+    const double zmax = (double)sample_unkey(kmax);
+    unsigned floored = 0;   // bit j: cut by min-p
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const double e = exp(sample_arg(w.key[j], kmax, zmax, set.invT));
+      w.q[j] = w.key[j] > kSampleKeyMasked ? sample_whole(e, scale) : 0ull;
+      floored |= (e >= set.m ? 0u : 1u) << j;
+    }
+    unsigned t = kSampleKeyMasked, r = 0;
+    const bool by_count = set.k < V, by_mass = set.p < 1.0;
+    if (by_count || by_mass) {
+      const SampleBins bins = sample_bins(kmax, kmin, set.invT, 64);
+      s.mass[lane] = 0;
+      s.count[lane] = 0;
+      sample_wave_sync();
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        if (w.key[j] > kSampleKeyMasked) {
+          const int b = sample_bin(bins, sample_unkey(w.key[j]));
+          atomicAdd(&s.count[b], 1u);
+          atomicAdd(&s.mass[b], w.q[j]);
+        }
+      }
+      sample_wave_sync();
+      const unsigned c_in = s.count[lane], c_run = sample_wave_scan(c_in);
+      const unsigned long long m_in = s.mass[lane], m_run = sample_wave_scan(m_in);
+      unsigned long long total = sample_lane(m_run, 63);   // mass of what top-k keeps
+      int kb = 64;                                         // the bin that top-k cuts, 64: none
+      int n_kb = 0;
+      if (by_count && set.k < (int)sample_lane(c_run, 63)) {
+        kb = __builtin_ctzll(__ballot(c_run >= (unsigned)set.k));
+        const unsigned want = (unsigned)set.k - (sample_lane(c_run, kb) - sample_lane(c_in, kb));
+        const unsigned long long above = sample_lane(m_run, kb) - sample_lane(m_in, kb);
+        n_kb = w.members(s, bins, kb);
+        sample_wave_sync();
+        if (n_kb >= 0) {
+          const unsigned mk = lane < n_kb ? s.m_key[lane] : 0u;
+          const unsigned long long mq = lane < n_kb ? s.m_mass[lane] : 0ull;
+          unsigned gt = 0, ge = 0;
+          for (int i = 0; i < n_kb; ++i) {
+            const unsigned o = sample_lane(mk, i);
+            gt += o > mk;
+            ge += o >= mk;
+          }
+          const int at = __builtin_ctzll(__ballot(lane < n_kb && gt < want && want <= ge));
+          t = sample_lane(mk, at);
+          r = want - sample_lane(gt, at);
+          total = above + sample_wave_sum(mk > t ? mq : 0ull) + r * sample_lane(mq, at);
+        } else {   // the largest t that at least k keys reach, a bit at a time
+          unsigned key = 0;
+          for (int b = 31; b >= 0; --b) {
+            const unsigned c = key | 1u << b;
+            unsigned n = 0;
+#pragma unroll
+            for (int j = 0; j < R; ++j) n += (unsigned)__builtin_popcountll(__ballot(w.key[j] >= c));
+            if (n >= (unsigned)set.k) key = c;
+          }
+          t = key;
+          unsigned n = 0;
+          unsigned long long m = 0;
+#pragma unroll
+          for (int j = 0; j < R; ++j) {
+            n += (unsigned)__builtin_popcountll(__ballot(w.key[j] > t));
+            m += w.key[j] > t ? w.q[j] : 0ull;
+          }
+          r = (unsigned)set.k - n;
+          total = sample_wave_sum(m) + r * sample_mass(sample_arg(t, kmax, zmax, set.invT), scale, 0.0);
+        }
+      }
+      if (by_mass) {
+        const unsigned long long bound = sample_bound(set.p, total);
+        // (a bin that top-k cuts counts as reached: what it keeps of it is in `total`)
+        const unsigned long long reach = __ballot(m_run >= bound);
+        const int pb = min(reach ? __builtin_ctzll(reach) : 63, kb);
+        const unsigned long long need = bound - (sample_lane(m_run, pb) - sample_lane(m_in, pb));
+        const int n = pb == kb ? n_kb : w.members(s, bins, pb);
+        sample_wave_sync();
+        if (n >= 0) {
+          const unsigned mk = lane < n ? s.m_key[lane] : 0u;
+          unsigned long long mq = lane < n ? s.m_mass[lane] : 0ull;
+          if (mk <= t) mq = 0;
+          unsigned long long gt = 0, ge = 0;
+          for (int i = 0; i < n; ++i) {
+            const unsigned o = sample_lane(mk, i);
+            const unsigned long long m = sample_lane(mq, i);
+            gt += o > mk ? m : 0ull;
+            ge += o >= mk ? m : 0ull;
+          }
+          const unsigned long long hit = __ballot(mk > t && gt < need && need <= ge);
+          if (hit) {   // (else it falls on the ties that top-k kept)
+            const int at = __builtin_ctzll(hit);
+            t = sample_lane(mk, at);
+            r = sample_ceil_div(need - sample_lane(gt, at), sample_lane(mq, at));
+          } else {
+            r = min(r, sample_ceil_div(need - sample_wave_sum(mq), sample_mass(sample_arg(t, kmax, zmax, set.invT), scale, 0.0)));
+          }
+        } else {
+          const unsigned long long at_t = r ? r * sample_mass(sample_arg(t, kmax, zmax, set.invT), scale, 0.0) : 0ull;
+          unsigned key = 0;
+          for (int b = 31; b >= 0; --b) {
+            const unsigned c = key | 1u << b;
+            unsigned long long m = 0;
+#pragma unroll
+            for (int j = 0; j < R; ++j) m += w.key[j] >= c && w.key[j] > t ? w.q[j] : 0ull;
+            if (sample_wave_sum(m) + (t >= c ? at_t : 0ull) >= bound) key = c;
+          }
+          unsigned long long m = 0;
+#pragma unroll
+          for (int j = 0; j < R; ++j) m += w.key[j] > key && w.key[j] > t ? w.q[j] : 0ull;
+          const unsigned rr = sample_ceil_div(bound - sample_wave_sum(m) - (t > key ? at_t : 0ull),
+                                              sample_mass(sample_arg(key, kmax, zmax, set.invT), scale, 0.0));
+          r = key == t ? min(r, rr) : rr;
+          t = key;
+        }
+      }
+    }
+    // the draw: kept masses summed in index order
+    unsigned ties = 0;
+#pragma unroll
+    for (int j = 0; j < R; ++j) ties += w.key[j] == t;
+    unsigned nth = 0;
+    if (r) nth = sample_wave_scan(ties) - ties;
+    unsigned long long sum = 0;
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const bool tie = w.key[j] == t;
+      const bool kept = (w.key[j] > t || (tie && nth < r)) && !(floored >> j & 1);
+      nth += tie;
+      w.q[j] = kept ? w.q[j] : 0ull;
+      sum += w.q[j];
+    }
+    const unsigned long long run = sample_wave_scan(sum), total = sample_lane(run, 63);
+    unsigned long long target = (unsigned long long)(set.u * (double)total);
+    if (target >= total) target = total - 1;
+    const int first = __builtin_ctzll(__ballot(run > target));
+    if (lane == first) {
+      unsigned long long upto = run - sum;
+      int at = 0;
+      unsigned key = 0;
+      bool found = false;
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        upto += w.q[j];
+        if (!found && upto > target) {
+          found = true;
+          at = j;
+          key = w.key[j];
+        }
+      }
+      sample_answer(a, row, lane * R + at, (float)(sample_arg(key, kmax, zmax, set.invT) - log((double)total / scale)));
+    }
   }
 }
 
