@@ -28,9 +28,88 @@ static int size_of(int dtype) { return dtype == QINCO_T_F32 ? 4 : 2; }
 // ---------------------------------------------------------------------------------------------
 // sampling
 // ---------------------------------------------------------------------------------------------
+// V above which a row is split over workgroups
+static constexpr int64_t kSampleLongV = 16384;
+
+namespace {
+struct SamplePlan {
+  int64_t rows, chunks;                                                          // rows of a batch
+  int64_t best, least, mass, count, row_mass, row_count, cuts, chunk_mass, n_members, m_mass, m_key, m_idx, bytes;   // byte offsets
+};
+}  // namespace
+
+// Rows go through in batches whose chunks' bins stay within 64 MiB (they are written by one kernel and read by the next: within the
+// 256 MiB cache), one row at least.
+static SamplePlan sample_plan(int64_t n, int64_t V) {
+  SamplePlan p{};
+  if (V <= kSampleLongV) return p;
+  p.chunks = (V + kSampleChunk - 1) / kSampleChunk;
+  p.rows = ((int64_t)64 << 20) / (p.chunks * kSampleBins * 12);
+  if (p.rows < 1) p.rows = 1;
+  if (p.rows > n) p.rows = n;
+  int64_t at = 0;
+  auto take = [&](int64_t& o, int64_t bytes) {
+    o = at;
+    at += (bytes + 255) / 256 * 256;
+  };
+  const int64_t R = p.rows, RC = R * p.chunks;
+  take(p.best, RC * 8);
+  take(p.least, RC * 4);
+  take(p.mass, RC * kSampleBins * 8);
+  take(p.count, RC * kSampleBins * 4);
+  take(p.row_mass, R * kSampleBins * 8);
+  take(p.row_count, R * kSampleBins * 4);
+  take(p.cuts, R * (int64_t)sizeof(SampleCuts));
+  take(p.chunk_mass, RC * 8);
+  take(p.n_members, R * 4);
+  take(p.m_mass, R * kSampleMembers * 8);
+  take(p.m_key, R * kSampleMembers * 4);
+  take(p.m_idx, R * kSampleMembers * 4);
+  p.bytes = at;
+  return p;
+}
+
 extern "C" int64_t qinco_sample_workspace(int64_t n, int64_t V) {
   if (n < 0 || V < 1 || V > kMaxLists) return 0;
-  return 0;
+  return sample_plan(n, V).bytes;
+}
+
+template <typename T>
+static int launch_sample_long(const SampleArgs& a, const SamplePlan& p, char* ws, hipStream_t st) {
+  SampleLong l{};
+  l.chunks = (int)p.chunks;
+  l.best = reinterpret_cast<unsigned long long*>(ws + p.best);
+  l.least = reinterpret_cast<unsigned*>(ws + p.least);
+  l.mass = reinterpret_cast<unsigned long long*>(ws + p.mass);
+  l.count = reinterpret_cast<unsigned*>(ws + p.count);
+  l.row_mass = reinterpret_cast<unsigned long long*>(ws + p.row_mass);
+  l.row_count = reinterpret_cast<unsigned*>(ws + p.row_count);
+  l.cuts = reinterpret_cast<SampleCuts*>(ws + p.cuts);
+  l.chunk_mass = reinterpret_cast<unsigned long long*>(ws + p.chunk_mass);
+  l.n_members = reinterpret_cast<int*>(ws + p.n_members);
+  l.m_mass = reinterpret_cast<unsigned long long*>(ws + p.m_mass);
+  l.m_key = reinterpret_cast<unsigned*>(ws + p.m_key);
+  l.m_idx = reinterpret_cast<unsigned*>(ws + p.m_idx);
+  // both cuts off for every row: no bins
+  const bool cuts = a.k_rows || (a.k > 0 && a.k < a.V) || a.p_rows || a.p < 1.0;
+  for (long r0 = 0; r0 < a.n; r0 += p.rows) {
+    const long rows = a.n - r0 < p.rows ? a.n - r0 : (long)p.rows;
+    l.row0 = r0;
+    const dim3 grid((unsigned)(rows * p.chunks)), block(kSampleChunkThreads);
+    hipLaunchKernelGGL(sample_range_kernel<T>, grid, block, 0, st, a, l);
+    HIP_TRY(hipGetLastError());
+    if (cuts) {
+      hipLaunchKernelGGL(sample_bins_kernel<T>, grid, block, 0, st, a, l);
+      HIP_TRY(hipGetLastError());
+      hipLaunchKernelGGL(sample_sum_bins_kernel, dim3((unsigned)(rows * (kSampleBins / 64))), dim3(1024), 0, st, l);
+      HIP_TRY(hipGetLastError());
+    }
+    hipLaunchKernelGGL(sample_members_kernel<T>, grid, block, 0, st, a, l);
+    HIP_TRY(hipGetLastError());
+    hipLaunchKernelGGL(sample_finish_kernel<T>, dim3((unsigned)rows), block, 0, st, a, l);
+    HIP_TRY(hipGetLastError());
+  }
+  return QINCO_OK;
 }
 
 template <typename T, int R>
@@ -40,12 +119,22 @@ static void launch_sample_wave(const SampleArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((sample_wave_kernel<T, R>), dim3((unsigned)g), dim3(64 * kSampleRowWaves), 0, st, a);
 }
 
+template <typename T, int NT>
+static void launch_sample_block(const SampleArgs& a, hipStream_t st) {
+  hipLaunchKernelGGL((sample_block_kernel<T, NT, 16>), dim3((unsigned)(a.n < 65536 ? a.n : 65536)), dim3(NT), 0, st, a);
+}
+
 template <typename T>
-static void launch_sample(const SampleArgs& a, hipStream_t st) {
+static int launch_sample(const SampleArgs& a, const SamplePlan& p, char* ws, hipStream_t st) {
+  if (a.V > kSampleLongV) return launch_sample_long<T>(a, p, ws, st);
   if (a.V <= 64) launch_sample_wave<T, 1>(a, st);
   else if (a.V <= 256) launch_sample_wave<T, 4>(a, st);
   else if (a.V <= 1024) launch_sample_wave<T, 16>(a, st);
-  else hipLaunchKernelGGL(sample_row_kernel<T>, dim3((unsigned)(a.n < 65536 ? a.n : 65536)), dim3(kSampleThreads), 0, st, a);
+  else if (a.V <= 4096) launch_sample_block<T, 256>(a, st);
+  else if (a.V <= 8192) launch_sample_block<T, 512>(a, st);
+  else launch_sample_block<T, 1024>(a, st);
+  HIP_TRY(hipGetLastError());
+  return QINCO_OK;
 }
 
 extern "C" int qinco_sample_codes(const void* logits, int dtype, int64_t row_stride, int64_t n, int64_t V, const void* u, int u_is_f64,
@@ -61,19 +150,18 @@ extern "C" int qinco_sample_codes(const void* logits, int dtype, int64_t row_str
   if (row_stride < 0) return fail(QINCO_ERR_INVALID, "qinco_sample_codes: negative row stride");
   if (n == 0) return QINCO_OK;
   if (!logits || !u || !codes_out) return fail(QINCO_ERR_INVALID, "qinco_sample_codes: null buffer");
-  const int64_t need = qinco_sample_workspace(n, V);
-  if (need > 0 && (!workspace || workspace_bytes < need))
-    return fail(QINCO_ERR_INVALID, "qinco_sample_codes: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)need);
+  const SamplePlan p = sample_plan(n, V);
+  if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
+    return fail(QINCO_ERR_INVALID, "qinco_sample_codes: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)p.bytes);
   const int lv = bits_of((uint64_t)V);
   SampleArgs a{logits, (long)row_stride, (long)n, (int)V, u, u_is_f64 != 0, params->temperature_rows, params->temperature, params->top_k_rows,
                params->top_k, params->top_p_rows, params->top_p, params->min_p_rows, params->min_p, codes_out,
                code_dtype == QINCO_CODE_I64, logp_out, 62 - lv < 51 ? 62 - lv : 51};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-  if (dtype == QINCO_T_F32) launch_sample<float>(a, st);
-  else if (dtype == QINCO_T_F16) launch_sample<_Float16>(a, st);
-  else launch_sample<__bf16>(a, st);
-  HIP_TRY(hipGetLastError());
-  return QINCO_OK;
+  char* ws = reinterpret_cast<char*>(workspace);
+  if (dtype == QINCO_T_F32) return launch_sample<float>(a, p, ws, st);
+  if (dtype == QINCO_T_F16) return launch_sample<_Float16>(a, p, ws, st);
+  return launch_sample<__bf16>(a, p, ws, st);
 }
 
 // ---------------------------------------------------------------------------------------------
