@@ -34,7 +34,7 @@ static constexpr int64_t kSampleLongV = 16384;
 namespace {
 struct SamplePlan {
   int64_t rows, chunks;                                                          // rows of a batch
-  int64_t best, least, mass, count, row_mass, row_count, cuts, chunk_mass, n_members, m_mass, m_key, m_idx, bytes;   // byte offsets
+  int64_t best, least, floor, mass, count, row_mass, row_count, state, chunk_mass, m_z, m_idx, bytes;   // byte offsets
 };
 }  // namespace
 
@@ -55,15 +55,14 @@ static SamplePlan sample_plan(int64_t n, int64_t V) {
   const int64_t R = p.rows, RC = R * p.chunks;
   take(p.best, RC * 8);
   take(p.least, RC * 4);
+  take(p.floor, RC * 4);
   take(p.mass, RC * kSampleBins * 8);
   take(p.count, RC * kSampleBins * 4);
   take(p.row_mass, R * kSampleBins * 8);
   take(p.row_count, R * kSampleBins * 4);
-  take(p.cuts, R * (int64_t)sizeof(SampleCuts));
+  take(p.state, R * (int64_t)sizeof(SampleState));
   take(p.chunk_mass, RC * 8);
-  take(p.n_members, R * 4);
-  take(p.m_mass, R * kSampleMembers * 8);
-  take(p.m_key, R * kSampleMembers * 4);
+  take(p.m_z, R * kSampleMembers * 4);
   take(p.m_idx, R * kSampleMembers * 4);
   p.bytes = at;
   return p;
@@ -80,30 +79,25 @@ static int launch_sample_long(const SampleArgs& a, const SamplePlan& p, char* ws
   l.chunks = (int)p.chunks;
   l.best = reinterpret_cast<unsigned long long*>(ws + p.best);
   l.least = reinterpret_cast<unsigned*>(ws + p.least);
+  l.floor = reinterpret_cast<int*>(ws + p.floor);
   l.mass = reinterpret_cast<unsigned long long*>(ws + p.mass);
   l.count = reinterpret_cast<unsigned*>(ws + p.count);
   l.row_mass = reinterpret_cast<unsigned long long*>(ws + p.row_mass);
   l.row_count = reinterpret_cast<unsigned*>(ws + p.row_count);
-  l.cuts = reinterpret_cast<SampleCuts*>(ws + p.cuts);
+  l.state = reinterpret_cast<SampleState*>(ws + p.state);
   l.chunk_mass = reinterpret_cast<unsigned long long*>(ws + p.chunk_mass);
-  l.n_members = reinterpret_cast<int*>(ws + p.n_members);
-  l.m_mass = reinterpret_cast<unsigned long long*>(ws + p.m_mass);
-  l.m_key = reinterpret_cast<unsigned*>(ws + p.m_key);
+  l.m_z = reinterpret_cast<float*>(ws + p.m_z);
   l.m_idx = reinterpret_cast<unsigned*>(ws + p.m_idx);
-  // both cuts off for every row: no bins
-  const bool cuts = a.k_rows || (a.k > 0 && a.k < a.V) || a.p_rows || a.p < 1.0;
   for (long r0 = 0; r0 < a.n; r0 += p.rows) {
     const long rows = a.n - r0 < p.rows ? a.n - r0 : (long)p.rows;
     l.row0 = r0;
     const dim3 grid((unsigned)(rows * p.chunks)), block(kSampleChunkThreads);
     hipLaunchKernelGGL(sample_range_kernel<T>, grid, block, 0, st, a, l);
     HIP_TRY(hipGetLastError());
-    if (cuts) {
-      hipLaunchKernelGGL(sample_bins_kernel<T>, grid, block, 0, st, a, l);
-      HIP_TRY(hipGetLastError());
-      hipLaunchKernelGGL(sample_sum_bins_kernel, dim3((unsigned)(rows * (kSampleBins / 64))), dim3(1024), 0, st, l);
-      HIP_TRY(hipGetLastError());
-    }
+    hipLaunchKernelGGL(sample_bins_kernel<T>, grid, block, 0, st, a, l);
+    HIP_TRY(hipGetLastError());
+    hipLaunchKernelGGL(sample_cuts_kernel, dim3((unsigned)(rows * (kSampleBins / 64))), dim3(1024), 0, st, a, l);
+    HIP_TRY(hipGetLastError());
     hipLaunchKernelGGL(sample_members_kernel<T>, grid, block, 0, st, a, l);
     HIP_TRY(hipGetLastError());
     hipLaunchKernelGGL(sample_finish_kernel<T>, dim3((unsigned)rows), block, 0, st, a, l);
@@ -119,9 +113,9 @@ static void launch_sample_wave(const SampleArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((sample_wave_kernel<T, R>), dim3((unsigned)g), dim3(64 * kSampleRowWaves), 0, st, a);
 }
 
-template <typename T, int NT>
+template <typename T, int NT, int KPT>
 static void launch_sample_block(const SampleArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((sample_block_kernel<T, NT, 16>), dim3((unsigned)(a.n < 65536 ? a.n : 65536)), dim3(NT), 0, st, a);
+  hipLaunchKernelGGL((sample_block_kernel<T, NT, KPT>), dim3((unsigned)(a.n < 65536 ? a.n : 65536)), dim3(NT), 0, st, a);
 }
 
 template <typename T>
@@ -130,9 +124,10 @@ static int launch_sample(const SampleArgs& a, const SamplePlan& p, char* ws, hip
   if (a.V <= 64) launch_sample_wave<T, 1>(a, st);
   else if (a.V <= 256) launch_sample_wave<T, 4>(a, st);
   else if (a.V <= 1024) launch_sample_wave<T, 16>(a, st);
-  else if (a.V <= 4096) launch_sample_block<T, 256>(a, st);
-  else if (a.V <= 8192) launch_sample_block<T, 512>(a, st);
-  else launch_sample_block<T, 1024>(a, st);
+  else if (a.V <= 2048) launch_sample_block<T, 256, 8>(a, st);
+  else if (a.V <= 4096) launch_sample_block<T, 512, 8>(a, st);
+  else if (a.V <= 8192) launch_sample_block<T, 1024, 8>(a, st);
+  else launch_sample_block<T, 1024, 16>(a, st);
   HIP_TRY(hipGetLastError());
   return QINCO_OK;
 }
