@@ -96,7 +96,9 @@ static int launch_sample_long(const SampleArgs& a, const SamplePlan& p, char* ws
     HIP_TRY(hipGetLastError());
     hipLaunchKernelGGL(sample_bins_kernel<T>, grid, block, 0, st, a, l);
     HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL(sample_cuts_kernel, dim3((unsigned)(rows * (kSampleBins / 64))), dim3(1024), 0, st, a, l);
+    hipLaunchKernelGGL(sample_sum_bins_kernel, dim3((unsigned)(rows * (kSampleBins / 64))), dim3(1024), 0, st, l);
+    HIP_TRY(hipGetLastError());
+    hipLaunchKernelGGL(sample_cuts_kernel, dim3((unsigned)rows), dim3(1024), 0, st, a, l);
     HIP_TRY(hipGetLastError());
     hipLaunchKernelGGL(sample_members_kernel<T>, grid, block, 0, st, a, l);
     HIP_TRY(hipGetLastError());
@@ -125,9 +127,9 @@ static int launch_sample(const SampleArgs& a, const SamplePlan& p, char* ws, hip
   else if (a.V <= 256) launch_sample_wave<T, 4>(a, st);
   else if (a.V <= 1024) launch_sample_wave<T, 16>(a, st);
   else if (a.V <= 2048) launch_sample_block<T, 256, 8>(a, st);
-  else if (a.V <= 4096) launch_sample_block<T, 512, 8>(a, st);
-  else if (a.V <= 8192) launch_sample_block<T, 1024, 8>(a, st);
-  else launch_sample_block<T, 1024, 16>(a, st);
+  else if (a.V <= 4096) launch_sample_block<T, 256, 16>(a, st);
+  else if (a.V <= 8192) launch_sample_block<T, 256, 32>(a, st);
+  else launch_sample_block<T, 512, 32>(a, st);
   HIP_TRY(hipGetLastError());
   return QINCO_OK;
 }

@@ -514,37 +514,61 @@ __device__ __forceinline__ unsigned sample_search(SampleBlock<NT>& blk, SampleFo
   }
 }
 
-// The draw among the codes [w0, w0 + 64 STEPS) of every wave (w0: the wave's own first code), `run0` of mass and `tied0` codes at t before
-// the first wave's: the wave that the target falls into walks them, 64 neighbouring codes per step.  `sum` and `at_t`: the wave's own
-// mass above t and codes at t, also in blk.
+// The draw among the codes that the workgroup's waves own, [w_first + w 64 STEPS, + 64 STEPS) each, with `run` of mass and `seen` codes at
+// t before the first wave's; blk holds every wave's mass above t and codes at t.  The wave that the target falls into has its steps of 64
+// codes taken by all waves side by side, and the one that it falls into draws.  Barriers inside: every thread.
 template <typename T, int NT, int STEPS>
-__device__ __forceinline__ void sample_draw(const SampleArgs& a, long row, const T* logits, int w0, const SampleMass& mass, double m, float t,
-                                            unsigned r, unsigned long long qt, const SampleBlock<NT>& blk, unsigned long long sum,
-                                            unsigned at_t, unsigned long long run0, unsigned tied0, unsigned long long target,
-                                            unsigned long long total) {
+__device__ __forceinline__ void sample_draw(const SampleArgs& a, long row, const T* logits, int w_first, const SampleMass& mass, double m,
+                                            float t, unsigned r, unsigned long long qt, SampleBlock<NT>& blk, unsigned long long run,
+                                            unsigned seen, unsigned long long target, unsigned long long total) {
+  constexpr int NW = NT / 64, PER = STEPS > NW ? STEPS / NW : 1;   // steps of one wave
+  static_assert(STEPS <= NW || STEPS % NW == 0, "steps are dealt out evenly");
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  unsigned long long run = run0;
-  unsigned seen = tied0;
+  int at_wave = 0;
+#pragma unroll 1
+  for (; at_wave < NW - 1; ++at_wave) {
+    const unsigned long long next = run + blk.m[at_wave] + min(blk.c[at_wave], r > seen ? r - seen : 0u) * qt;
+    if (target < next) break;
+    run = next;
+    seen += blk.c[at_wave];
+  }
+  const int i0 = w_first + at_wave * 64 * STEPS + w * PER * 64;
+  unsigned long long q[PER], sum = 0;
+  float z[PER];
+  unsigned ties = 0;
+#pragma unroll
+  for (int j = 0; j < PER; ++j) {
+    z[j] = w * PER < STEPS ? sample_logit(logits, i0 + j * 64 + lane, a.V) : -INFINITY;
+    q[j] = z[j] > t ? mass.q(z[j], m) : 0ull;
+    sum += q[j];
+    ties += z[j] == t && r > 0;
+  }
+  sum = sample_wave_sum(sum);
+  ties = sample_wave_sum(ties);
+  __syncthreads();
+  if (lane == 0) {
+    blk.m[w] = sum;
+    blk.c[w] = ties;
+  }
+  __syncthreads();
 #pragma unroll 1
   for (int v = 0; v < w; ++v) {
     run += blk.m[v] + min(blk.c[v], r > seen ? r - seen : 0u) * qt;
     seen += blk.c[v];
   }
-  const unsigned long long here = sum + min(at_t, r > seen ? r - seen : 0u) * qt;
+  const unsigned long long here = sum + min(ties, r > seen ? r - seen : 0u) * qt;
   if (run <= target && target < run + here) {
-#pragma unroll 1
-    for (int j = 0; j < STEPS; ++j) {
-      const int i = w0 + j * 64 + lane;
-      const float z = sample_logit(logits, i, a.V);
-      const bool tie = r > 0 && z == t;
+    bool done = false;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+      const bool tie = r > 0 && z[j] == t;
       const unsigned long long at = __ballot(tie);
       const unsigned nth = seen + __builtin_popcountll(at & ((1ull << lane) - 1));
-      const unsigned long long kept = z > t ? mass.q(z, m) : (tie && nth < r ? qt : 0ull);
-      const unsigned long long incl = run + sample_wave_scan(kept);
+      const unsigned long long incl = run + sample_wave_scan(tie && nth < r ? qt : q[j]);
       const unsigned long long hit = __ballot(incl > target);
-      if (hit) {
-        if (lane == (int)__builtin_ctzll(hit)) sample_answer(a, row, i, mass.logp(z, total));
-        break;
+      if (!done && hit) {
+        if (lane == (int)__builtin_ctzll(hit)) sample_answer(a, row, i0 + j * 64 + lane, mass.logp(z[j], total));
+        done = true;
       }
       run = sample_lane(incl, 63);
       seen += __builtin_popcountll(at);
@@ -552,20 +576,34 @@ __device__ __forceinline__ void sample_draw(const SampleArgs& a, long row, const
   }
 }
 
-// One workgroup per row, its logits in registers: wave w owns a run of 64 KPT codes, 64 neighbouring ones per step.
+// One workgroup per row, its logits in registers: wave w owns a run of 64 KPT codes, 64 neighbouring ones per step.  The codes of the bin
+// that a cut falls into are listed, and up to 64 of them compared by one wave, a lane each; more (heavy ties) are searched in bins.
+// The kernel is bound by its barriers: four waves (eight beyond 8192 codes) and several workgroups per CU, rather than sixteen waves.
 template <typename T, int NT, int KPT>
-__global__ void __launch_bounds__(NT) sample_block_kernel(SampleArgs a) {
+__global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
   constexpr int PB = kSampleBins / NT;
   __shared__ unsigned long long bin_mass[kSampleBins], part[kSampleBins];
   __shared__ unsigned bin_count[kSampleBins];
   __shared__ SampleBlock<NT> blk;
   __shared__ SampleFound found;
   __shared__ unsigned range[2][NT / 64], key_range[2];
+  __shared__ float m_z[64];
+  __shared__ int n_listed;
+  __shared__ struct {
+    float t;
+    unsigned r;
+    unsigned long long in;
+  } cut;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, V = a.V, w0 = w * 64 * KPT;
   for (long row = blockIdx.x; row < a.n; row += gridDim.x) {
     const T* logits = reinterpret_cast<const T*>(a.logits) + row * a.stride;
     const SampleRow set = sample_row(a, row);
     float z[KPT], hi = -INFINITY, lo = INFINITY;
+    // (a new look at the same registers: nothing computed from them is kept from one phase to the next)
+    auto again = [&] {
+#pragma unroll
+      for (int j = 0; j < KPT; ++j) asm volatile("" : "+v"(z[j]));
+    };
 #pragma unroll
     for (int j = 0; j < KPT; ++j) z[j] = sample_logit(logits, w0 + j * 64 + lane, V);
 #pragma unroll
@@ -610,6 +648,7 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(SampleArgs a) {
     const bool by_mass = set.p < 1.0;
     if (set.k < V || by_mass) {
       const SampleBins bins = sample_bins(zmax, sample_unkey(~klo), set.y, kSampleBins);
+      again();
 #pragma unroll
       for (int j = 0; j < KPT; ++j) {
         if (z[j] > -INFINITY) {
@@ -622,6 +661,7 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(SampleArgs a) {
         }
         if (j & 1) __builtin_amdgcn_sched_barrier(0);   // (two exponentials at a time: more side by side only take registers)
       }
+      if (tid == 0) n_listed = 0;
       __syncthreads();
       unsigned long long m = 0, m_before, total;
       unsigned c = 0, c_before, c_all;
@@ -631,6 +671,19 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(SampleArgs a) {
         c += bin_count[tid * PB + j];
       }
       sample_block_scan<NT>(blk, m, c, m_before, c_before, total, c_all);
+      // codes of bin b above t into m_z; their number
+      auto list = [&](int b) {
+        again();
+#pragma unroll
+        for (int j = 0; j < KPT; ++j) {
+          if (z[j] > t && bins.of(z[j]) == b) {
+            const int to = atomicAdd(&n_listed, 1);
+            if (to < 64) m_z[to] = z[j];
+          }
+        }
+        __syncthreads();
+        return n_listed;
+      };
       // the smallest and largest key of bin b above t
       auto keys_of = [&](int b, unsigned& first, unsigned& last) {
         if (tid == 0) {
@@ -639,6 +692,7 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(SampleArgs a) {
         }
         __syncthreads();
         unsigned l = ~0u, h = 0;
+        again();
 #pragma unroll
         for (int j = 0; j < KPT; ++j) {
           if (z[j] > t && bins.of(z[j]) == b) {
@@ -654,9 +708,8 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(SampleArgs a) {
         first = key_range[0];
         last = key_range[1];
       };
-      int kb = kSampleBins;            // the bin that top-k cuts
-      unsigned long long k_above = 0;  // mass before that bin, and in it above t
-      unsigned long long k_in = 0;
+      int kb = kSampleBins;                          // the bin that top-k cuts
+      unsigned long long k_above = 0, k_in = 0;      // mass before that bin, and in it above t
       if ((unsigned)set.k < c_all) {
         if (c_before < (unsigned)set.k && (unsigned)set.k <= c_before + c) {
           unsigned cr = c_before;
@@ -677,26 +730,53 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(SampleArgs a) {
         kb = found.bin;
         const unsigned want = found.count;
         k_above = found.mass;
-        unsigned first, last;
-        keys_of(kb, first, last);
-        unsigned long long before;
-        const unsigned key = sample_search<NT>(blk, found, part, first, last, want, before, [&](auto f) {
+        const int n = list(kb);
+        if (n <= 64) {
+          if (w == 0) {
+            const float mz = lane < n ? m_z[lane] : -INFINITY;
+            unsigned gt = 0, ge = 0;
+            for (int i = 0; i < n; ++i) {
+              const float o = __uint_as_float(sample_lane(__float_as_uint(mz), i));
+              gt += o > mz;
+              ge += o >= mz;
+            }
+            const int at = __builtin_ctzll(__ballot(lane < n && gt < want && want <= ge));
+            const float z_at = __uint_as_float(sample_lane(__float_as_uint(mz), at));
+            const unsigned long long in = by_mass ? sample_wave_sum(mz > z_at ? mass.q(mz) : 0ull) : 0ull;
+            if (lane == 0) {
+              cut.t = z_at;
+              cut.r = want - sample_lane(gt, at);
+              cut.in = in;
+              n_listed = 0;
+            }
+          }
+          __syncthreads();
+          t = cut.t;
+          r = cut.r;
+          k_in = cut.in;
+        } else {
+          unsigned first, last;
+          keys_of(kb, first, last);
+          unsigned long long before;
+          const unsigned key = sample_search<NT>(blk, found, part, first, last, want, before, [&](auto f) {
+            again();
 #pragma unroll
-          for (int j = 0; j < KPT; ++j)
-            if (z[j] > -INFINITY && bins.of(z[j]) == kb) f(sample_key(z[j]), [] { return 1ull; });
-        });
-        t = sample_unkey(key);
-        r = want - (unsigned)before;
-        qt = mass.q(t);
-        if (by_mass) {
+            for (int j = 0; j < KPT; ++j)
+              if (z[j] > -INFINITY && bins.of(z[j]) == kb) f(sample_key(z[j]), [] { return 1ull; });
+          });
+          t = sample_unkey(key);
+          r = want - (unsigned)before;
+          if (tid == 0) n_listed = 0;
           unsigned long long in = 0, none;
           unsigned none_c, none_all;
+          again();
 #pragma unroll
           for (int j = 0; j < KPT; ++j)
             if (z[j] > t && bins.of(z[j]) == kb) in += mass.q(z[j]);
           sample_block_scan<NT>(blk, in, 0u, none, none_c, k_in, none_all);
-          total = k_above + k_in + r * qt;
         }
+        qt = mass.q(t);
+        total = k_above + k_in + r * qt;
       }
       if (by_mass) {
         const unsigned long long bound = sample_bound(set.p, total);
@@ -717,19 +797,44 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(SampleArgs a) {
           __syncthreads();
           const int pb = found.bin;
           const unsigned long long need = bound - found.mass;
-          unsigned first, last;
-          keys_of(pb, first, last);
-          unsigned long long before;
-          const unsigned key = sample_search<NT>(blk, found, part, first, last, need, before, [&](auto f) {
+          const int n = list(pb);
+          if (n <= 64) {
+            if (w == 0) {
+              const float mz = lane < n ? m_z[lane] : -INFINITY;
+              const unsigned long long mq = lane < n ? mass.q(mz) : 0ull;
+              unsigned long long gt = 0, ge = 0;
+              for (int i = 0; i < n; ++i) {
+                const float o = __uint_as_float(sample_lane(__float_as_uint(mz), i));
+                const unsigned long long q = sample_lane(mq, i);
+                gt += o > mz ? q : 0ull;
+                ge += o >= mz ? q : 0ull;
+              }
+              const int at = __builtin_ctzll(__ballot(lane < n && gt < need && need <= ge));
+              if (lane == at) {
+                cut.t = mz;
+                cut.r = sample_ceil_div(need - gt, mq);
+              }
+            }
+            __syncthreads();
+            t = cut.t;
+            r = cut.r;
+          } else {
+            unsigned first, last;
+            keys_of(pb, first, last);
+            unsigned long long before;
+            const unsigned key = sample_search<NT>(blk, found, part, first, last, need, before, [&](auto f) {
+              again();
 #pragma unroll
-            for (int j = 0; j < KPT; ++j)
-              if (z[j] > t && bins.of(z[j]) == pb) f(sample_key(z[j]), [&] { return mass.q(z[j]); });
-          });
-          t = sample_unkey(key);
-          r = sample_ceil_div(need - before, mass.q(t));
+              for (int j = 0; j < KPT; ++j)
+                if (z[j] > t && bins.of(z[j]) == pb) f(sample_key(z[j]), [&] { return mass.q(z[j]); });
+            });
+            t = sample_unkey(key);
+            r = sample_ceil_div(need - before, mass.q(t));
+          }
         }
       }
-      qt = mass.q(t, set.m);
+      qt = r ? mass.q(t, set.m) : 0ull;
+      again();
     }
     // kept masses, wave by wave
     unsigned at_t = 0;
@@ -754,7 +859,7 @@ __global__ void __launch_bounds__(NT) sample_block_kernel(SampleArgs a) {
       total += blk.m[v] + min(blk.c[v], r > seen ? r - seen : 0u) * qt;
       seen += blk.c[v];
     }
-    sample_draw<T, NT, KPT>(a, row, logits, w0, mass, set.m, t, r, qt, blk, sum, at_t, 0ull, 0u, sample_target(set.u, total), total);
+    sample_draw<T, NT, KPT>(a, row, logits, 0, mass, set.m, t, r, qt, blk, 0ull, 0u, sample_target(set.u, total), total);
     __syncthreads();
   }
 }
@@ -780,7 +885,7 @@ struct SampleState {                   // of a row
   unsigned want;                       // codes kept of it
   int b0, b1;                          // bins that the last cut falls into; kSampleBins: no cut
   int fb;                              // the first bin with codes that min-p cuts; bins before min(b0, fb) are kept whole
-  int n_members, done;                 // counters: members, and workgroups of (3) that are through
+  int n_members;
   unsigned long long above, base;      // mass before kb, and before b0
   unsigned long long bound;            // the mass that top-p cuts at, where top-k cuts nothing
   __device__ __forceinline__ bool member(int b) const { return (b >= b0 && b <= b1) || b == kb || (b == fb && fb < b0); }
@@ -840,7 +945,6 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_range_kernel(Sampl
     if (lane == 0) {
       l.best[r * l.chunks + c] = (unsigned long long)all << 32 | i;
       l.least[r * l.chunks + c] = s;
-      if (c == 0) l.state[r].n_members = l.state[r].done = 0;
     }
   }
 }
@@ -915,62 +1019,57 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_bins_kernel(Sample
   if (tid == 0) l.floor[r * l.chunks + c] = floor;
 }
 
-// Bins summed over the chunks: a workgroup owns 64 bins of a row, its 16 waves every 16th chunk.  The last of a row's 16 workgroups to
-// finish (a ticket; nobody waits) finds the cuts' bins.
-__global__ void __launch_bounds__(1024) sample_cuts_kernel(SampleArgs a, SampleLong l) {
-  constexpr int NT = 1024, PARTS = kSampleBins / 64;
+// bins summed over the chunks: a workgroup owns 64 bins of a row, its 16 waves every 16th chunk
+__global__ void __launch_bounds__(1024) sample_sum_bins_kernel(SampleLong l) {
   __shared__ unsigned long long mass[16][64];
   __shared__ unsigned count[16][64];
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const long r = blockIdx.x / (kSampleBins / 64);
+  const int b = (int)(blockIdx.x % (kSampleBins / 64)) * 64 + lane;
+  unsigned long long m = 0;
+  unsigned n = 0;
+  for (int c = w; c < l.chunks; c += 16) {
+    const size_t o = ((size_t)r * l.chunks + c) * kSampleBins + b;
+    m += l.mass[o];
+    n += l.count[o];
+  }
+  mass[w][lane] = m;
+  count[w][lane] = n;
+  __syncthreads();
+  if (w == 0) {
+    for (int v = 1; v < 16; ++v) {
+      m += mass[v][lane];
+      n += count[v][lane];
+    }
+    l.row_mass[r * kSampleBins + b] = m;
+    l.row_count[r * kSampleBins + b] = n;
+  }
+}
+
+// the cuts' bins of a row, a thread per bin (a kernel of its own: finding them by the last workgroup of the one above needs a fence that
+// empties the L2, measured 30 us against 5 + 5)
+__global__ void __launch_bounds__(1024) sample_cuts_kernel(SampleArgs a, SampleLong l) {
+  constexpr int NT = 1024;
   __shared__ SampleBlock<NT> blk;
   __shared__ SampleState st;
   __shared__ unsigned sh[3];
-  __shared__ int ticket;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
-  const long r = blockIdx.x / PARTS;
+  const int tid = threadIdx.x;
+  const long r = blockIdx.x;
   const SampleRow set = sample_row(a, l.row0 + r);
   const SampleRange g = sample_range(l, r, sh);
-  const bool none = g.zmax == -INFINITY || set.greedy;
-  if (!none) {
-    const int b = (int)(blockIdx.x % PARTS) * 64 + lane;
-    unsigned long long m = 0;
-    unsigned n = 0;
-    for (int c = w; c < l.chunks; c += 16) {
-      const size_t o = ((size_t)r * l.chunks + c) * kSampleBins + b;
-      m += l.mass[o];
-      n += l.count[o];
-    }
-    mass[w][lane] = m;
-    count[w][lane] = n;
-    __syncthreads();
-    if (w == 0) {
-      for (int v = 1; v < 16; ++v) {
-        m += mass[v][lane];
-        n += count[v][lane];
-      }
-      l.row_mass[r * kSampleBins + b] = m;
-      l.row_count[r * kSampleBins + b] = n;
-      __threadfence();
-    }
-  }
-  __syncthreads();
-  if (tid == 0) ticket = atomicAdd(&l.state[r].done, 1);
-  __syncthreads();
-  if (ticket != PARTS - 1) return;
-  __threadfence();
   if (tid == 0) {
     st.zmax = g.zmax;
     st.zmin = g.zmin;
     st.first = g.first;
     st.kb = st.b0 = st.b1 = st.fb = kSampleBins;
     st.want = 0;
-    st.n_members = st.done = 0;
+    st.n_members = 0;
     st.above = st.base = st.bound = 0;
   }
   __syncthreads();
-  if (!none) {
-    // a thread per bin (written by other workgroups of this launch: read past this CU's cache)
-    const unsigned long long m = __hip_atomic_load(&l.row_mass[r * kSampleBins + tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const unsigned n = __hip_atomic_load(&l.row_count[r * kSampleBins + tid], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  if (g.zmax > -INFINITY && !set.greedy) {
+    const unsigned long long m = l.row_mass[r * kSampleBins + tid];
+    const unsigned n = l.row_count[r * kSampleBins + tid];
     int f = kSampleBins;
     for (int c = tid; c < l.chunks; c += NT) f = min(f, l.floor[r * l.chunks + c]);
     if (f < kSampleBins) atomicMin(&st.fb, f);
@@ -981,7 +1080,7 @@ __global__ void __launch_bounds__(1024) sample_cuts_kernel(SampleArgs a, SampleL
       st.kb = st.b0 = st.b1 = tid;
       st.want = (unsigned)set.k - c_before;
       st.above = st.base = m_before;
-      st.bound = m;                    // (of kb, until the line below has read it)
+      st.bound = m;                    // (of kb, until the lines below have read it)
     }
     __syncthreads();
     if (set.p < 1.0) {
@@ -994,9 +1093,9 @@ __global__ void __launch_bounds__(1024) sample_cuts_kernel(SampleArgs a, SampleL
       }
       if (m_before < hi && hi <= m_before + m) st.b1 = tid;
       if (tid == 0) st.bound = lo;
-      __syncthreads();
     }
   }
+  __syncthreads();
   if (tid == 0) l.state[r] = st;
 }
 
@@ -1059,6 +1158,7 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
   __shared__ unsigned m_idx[kSampleMembers];
   __shared__ unsigned long long chunk[kSampleMaxChunks];
   __shared__ unsigned chunk_ties[kSampleMaxChunks];
+  __shared__ unsigned key_range[2];
   __shared__ int sh_chunk;
   __shared__ unsigned sh_tied;
   __shared__ unsigned long long sh_before;
@@ -1103,7 +1203,29 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
   unsigned ties = 0;   // codes kept of those at t
   unsigned long long qt = 0, before, all;
   unsigned none, none_all;
-  const unsigned kmin = sample_key(st.zmin), kmax = sample_key(st.zmax);
+  // the members' keys: fewer bits to search
+  unsigned kmin = sample_key(st.zmin), kmax = sample_key(st.zmax);
+  if (listed) {
+    if (tid == 0) {
+      key_range[0] = ~0u;
+      key_range[1] = 0;
+    }
+    __syncthreads();
+    unsigned lo = 0, hi = 0;   // lo: complemented
+    for (int i = tid; i < n; i += NT) {
+      lo = max(lo, ~sample_key(m_z[i]));
+      hi = max(hi, sample_key(m_z[i]));
+    }
+    lo = sample_wave_max(lo);
+    hi = sample_wave_max(hi);
+    if (lane == 0 && hi) {
+      atomicMin(&key_range[0], ~lo);
+      atomicMax(&key_range[1], hi);
+    }
+    __syncthreads();
+    kmin = key_range[0];
+    kmax = key_range[1];
+  }
   unsigned long long total = 0;
   if (st.kb < kSampleBins) {
     const unsigned key = sample_search<NT>(blk, found, part, kmin, kmax, st.want, before, [&](auto f) {
@@ -1172,8 +1294,8 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
     sh_tied = tied;
   }
   __syncthreads();
-  // ... and in that chunk: wave w walks codes [i0 + 1024 w, + 1024)
-  const int w0 = sh_chunk * kSampleChunk + w * 64 * kSampleChunkIpt;
+  // ... and in that chunk: wave w owns codes [i0 + 1024 w, + 1024)
+  const int i0 = sh_chunk * kSampleChunk, w0 = i0 + w * 64 * kSampleChunkIpt;
   unsigned long long sum = 0;
   unsigned at_t = 0;
 #pragma unroll 4
@@ -1189,7 +1311,7 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
     blk.c[w] = at_t;
   }
   __syncthreads();
-  sample_draw<T, NT, kSampleChunkIpt>(a, row, logits, w0, mass, set.m, t, ties, qt, blk, sum, at_t, sh_before, sh_tied, target, total);
+  sample_draw<T, NT, kSampleChunkIpt>(a, row, logits, i0, mass, set.m, t, ties, qt, blk, sh_before, sh_tied, target, total);
 }
 
 }  // namespace qinco
