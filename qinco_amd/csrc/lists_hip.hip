@@ -29,7 +29,7 @@ static int size_of(int dtype) { return dtype == QINCO_T_F32 ? 4 : 2; }
 // sampling
 // ---------------------------------------------------------------------------------------------
 // V above which a row is split over workgroups
-static constexpr int64_t kSampleLongV = 16384;
+static constexpr int64_t kSampleLongV = kSampleBlockV;
 
 namespace {
 struct SamplePlan {
@@ -115,9 +115,9 @@ static void launch_sample_wave(const SampleArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((sample_wave_kernel<T, R>), dim3((unsigned)g), dim3(64 * kSampleRowWaves), 0, st, a);
 }
 
-template <typename T, int NT, int KPT>
+template <typename T, int NT>
 static void launch_sample_block(const SampleArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((sample_block_kernel<T, NT, KPT>), dim3((unsigned)(a.n < 65536 ? a.n : 65536)), dim3(NT), 0, st, a);
+  hipLaunchKernelGGL((sample_block_kernel<T, NT>), dim3((unsigned)(a.n < 65536 ? a.n : 65536)), dim3(NT), (size_t)a.V * sizeof(T), st, a);
 }
 
 template <typename T>
@@ -126,10 +126,7 @@ static int launch_sample(const SampleArgs& a, const SamplePlan& p, char* ws, hip
   if (a.V <= 64) launch_sample_wave<T, 1>(a, st);
   else if (a.V <= 256) launch_sample_wave<T, 4>(a, st);
   else if (a.V <= 1024) launch_sample_wave<T, 16>(a, st);
-  else if (a.V <= 2048) launch_sample_block<T, 256, 8>(a, st);
-  else if (a.V <= 4096) launch_sample_block<T, 256, 16>(a, st);
-  else if (a.V <= 8192) launch_sample_block<T, 256, 32>(a, st);
-  else launch_sample_block<T, 512, 32>(a, st);
+  else launch_sample_block<T, 256>(a, st);
   HIP_TRY(hipGetLastError());
   return QINCO_OK;
 }

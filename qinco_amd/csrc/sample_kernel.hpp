@@ -514,16 +514,15 @@ __device__ __forceinline__ unsigned sample_search(SampleBlock<NT>& blk, SampleFo
   }
 }
 
-// The draw among the codes that the workgroup's waves own, [w_first + w 64 STEPS, + 64 STEPS) each, with `run` of mass and `seen` codes at
+// The draw among the codes that the workgroup's waves own, [w_first + w 64 steps, + 64 steps) each, with `run` of mass and `seen` codes at
 // t before the first wave's; blk holds every wave's mass above t and codes at t.  The wave that the target falls into has its steps of 64
-// codes taken by all waves side by side, and the one that it falls into draws.  Barriers inside: every thread.
-template <typename T, int NT, int STEPS>
-__device__ __forceinline__ void sample_draw(const SampleArgs& a, long row, const T* logits, int w_first, const SampleMass& mass, double m,
+// codes taken by all waves side by side, and the one that it falls into draws.  `z`: the row.  Barriers inside: every thread.
+template <typename T, int NT>
+__device__ __forceinline__ void sample_draw(const SampleArgs& a, long row, const T* z, int w_first, int steps, const SampleMass& mass, double m,
                                             float t, unsigned r, unsigned long long qt, SampleBlock<NT>& blk, unsigned long long run,
                                             unsigned seen, unsigned long long target, unsigned long long total) {
-  constexpr int NW = NT / 64, PER = STEPS > NW ? STEPS / NW : 1;   // steps of one wave
-  static_assert(STEPS <= NW || STEPS % NW == 0, "steps are dealt out evenly");
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  constexpr int NW = NT / 64;
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, per = (steps + NW - 1) / NW;   // steps of one wave
   int at_wave = 0;
 #pragma unroll 1
   for (; at_wave < NW - 1; ++at_wave) {
@@ -532,16 +531,13 @@ __device__ __forceinline__ void sample_draw(const SampleArgs& a, long row, const
     run = next;
     seen += blk.c[at_wave];
   }
-  const int i0 = w_first + at_wave * 64 * STEPS + w * PER * 64;
-  unsigned long long q[PER], sum = 0;
-  float z[PER];
+  const int first = w_first + at_wave * 64 * steps, j0 = w * per, j1 = min(j0 + per, steps);
+  unsigned long long sum = 0;
   unsigned ties = 0;
-#pragma unroll
-  for (int j = 0; j < PER; ++j) {
-    z[j] = w * PER < STEPS ? sample_logit(logits, i0 + j * 64 + lane, a.V) : -INFINITY;
-    q[j] = z[j] > t ? mass.q(z[j], m) : 0ull;
-    sum += q[j];
-    ties += z[j] == t && r > 0;
+  for (int j = j0; j < j1; ++j) {
+    const float x = sample_logit(z, first + j * 64 + lane, a.V);
+    sum += x > t ? mass.q(x, m) : 0ull;
+    ties += x == t && r > 0;
   }
   sum = sample_wave_sum(sum);
   ties = sample_wave_sum(ties);
@@ -558,17 +554,18 @@ __device__ __forceinline__ void sample_draw(const SampleArgs& a, long row, const
   }
   const unsigned long long here = sum + min(ties, r > seen ? r - seen : 0u) * qt;
   if (run <= target && target < run + here) {
-    bool done = false;
-#pragma unroll
-    for (int j = 0; j < PER; ++j) {
-      const bool tie = r > 0 && z[j] == t;
+#pragma unroll 1
+    for (int j = j0; j < j1; ++j) {
+      const int i = first + j * 64 + lane;
+      const float x = sample_logit(z, i, a.V);
+      const bool tie = r > 0 && x == t;
       const unsigned long long at = __ballot(tie);
       const unsigned nth = seen + __builtin_popcountll(at & ((1ull << lane) - 1));
-      const unsigned long long incl = run + sample_wave_scan(tie && nth < r ? qt : q[j]);
+      const unsigned long long incl = run + sample_wave_scan(x > t ? mass.q(x, m) : (tie && nth < r ? qt : 0ull));
       const unsigned long long hit = __ballot(incl > target);
-      if (!done && hit) {
-        if (lane == (int)__builtin_ctzll(hit)) sample_answer(a, row, i0 + j * 64 + lane, mass.logp(z[j], total));
-        done = true;
+      if (hit) {
+        if (lane == (int)__builtin_ctzll(hit)) sample_answer(a, row, i, mass.logp(x, total));
+        break;
       }
       run = sample_lane(incl, 63);
       seen += __builtin_popcountll(at);
@@ -576,11 +573,14 @@ __device__ __forceinline__ void sample_draw(const SampleArgs& a, long row, const
   }
 }
 
-// One workgroup per row, its logits in registers: wave w owns a run of 64 KPT codes, 64 neighbouring ones per step.  The codes of the bin
-// that a cut falls into are listed, and up to 64 of them compared by one wave, a lane each; more (heavy ties) are searched in bins.
-// The kernel is bound by its barriers: four waves (eight beyond 8192 codes) and several workgroups per CU, rather than sixteen waves.
-template <typename T, int NT, int KPT>
+// One workgroup per row, its logits in LDS (V of them, as they come): wave w owns a run of `steps` x 64 codes.  The codes of the bin that a
+// cut falls into are listed, and up to 64 of them compared by one wave, a lane each; more (heavy ties) are searched in bins.  The kernel
+// is bound by its barriers and the latency between them: four waves per row and several rows per CU, rather than sixteen waves.
+constexpr int kSampleBlockV = 10240;   // row + 21 KB of bins and scratch within the 64 KB of LDS that a launch may ask for without more ado
+template <typename T, int NT>
 __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
+  extern __shared__ __align__(16) unsigned char sample_row_lds[];
+  T* row_z = reinterpret_cast<T*>(sample_row_lds);
   constexpr int PB = kSampleBins / NT;
   __shared__ unsigned long long bin_mass[kSampleBins], part[kSampleBins];
   __shared__ unsigned bin_count[kSampleBins];
@@ -594,23 +594,28 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
     unsigned r;
     unsigned long long in;
   } cut;
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, V = a.V, w0 = w * 64 * KPT;
+  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, V = a.V;
+  const int steps = (V + NT - 1) / NT, w0 = w * steps * 64;
   for (long row = blockIdx.x; row < a.n; row += gridDim.x) {
     const T* logits = reinterpret_cast<const T*>(a.logits) + row * a.stride;
     const SampleRow set = sample_row(a, row);
-    float z[KPT], hi = -INFINITY, lo = INFINITY;
-    // (a new look at the same registers: nothing computed from them is kept from one phase to the next)
-    auto again = [&] {
-#pragma unroll
-      for (int j = 0; j < KPT; ++j) asm volatile("" : "+v"(z[j]));
-    };
-#pragma unroll
-    for (int j = 0; j < KPT; ++j) z[j] = sample_logit(logits, w0 + j * 64 + lane, V);
-#pragma unroll
-    for (int j = 0; j < KPT; ++j) {
-      hi = fmaxf(hi, z[j]);
-      lo = fminf(lo, z[j] > -INFINITY ? z[j] : INFINITY);
+    float hi = -INFINITY, lo = INFINITY;
+#pragma unroll 4
+    for (int j = 0; j < steps; ++j) {
+      const int i = w0 + j * 64 + lane;
+      const float z = sample_logit(logits, i, V);
+      if (i < V) row_z[i] = logits[i];
+      hi = fmaxf(hi, z);
+      lo = fminf(lo, z > -INFINITY ? z : INFINITY);
     }
+    // f(z) for every code of this thread that can be drawn (a thread reads what it wrote)
+    auto each = [&](auto f) {
+#pragma unroll 2
+      for (int j = 0; j < steps; ++j) {
+        const float z = sample_logit(row_z, w0 + j * 64 + lane, V);
+        if (z > -INFINITY) f(z);
+      }
+    };
     unsigned khi = sample_wave_max(sample_key(hi)), klo = sample_wave_max(~sample_key(lo));
     if (lane == 0) {
       range[0][w] = khi;
@@ -626,9 +631,8 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
     const float zmax = sample_unkey(khi);
     if (zmax == -INFINITY || set.greedy) {
       unsigned first = 0;   // complement of the lowest index of the largest logit
-#pragma unroll
-      for (int j = KPT - 1; j >= 0; --j)
-        if (z[j] == zmax) first = ~(unsigned)(w0 + j * 64 + lane);
+      for (int j = steps - 1; j >= 0; --j)
+        if (sample_logit(row_z, w0 + j * 64 + lane, V) == zmax) first = max(first, ~(unsigned)(w0 + j * 64 + lane));
       first = sample_wave_max(first);
       __syncthreads();
       if (lane == 0) range[0][w] = first;
@@ -648,19 +652,14 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
     const bool by_mass = set.p < 1.0;
     if (set.k < V || by_mass) {
       const SampleBins bins = sample_bins(zmax, sample_unkey(~klo), set.y, kSampleBins);
-      again();
-#pragma unroll
-      for (int j = 0; j < KPT; ++j) {
-        if (z[j] > -INFINITY) {
-          const int b = bins.of(z[j]);
-          atomicAdd(&bin_count[b], 1u);
-          if (by_mass) {
-            const unsigned long long q = mass.q(z[j]);
-            if (q) atomicAdd(&bin_mass[b], q);
-          }
+      each([&](float z) {
+        const int b = bins.of(z);
+        atomicAdd(&bin_count[b], 1u);
+        if (by_mass) {
+          const unsigned long long q = mass.q(z);
+          if (q) atomicAdd(&bin_mass[b], q);
         }
-        if (j & 1) __builtin_amdgcn_sched_barrier(0);   // (two exponentials at a time: more side by side only take registers)
-      }
+      });
       if (tid == 0) n_listed = 0;
       __syncthreads();
       unsigned long long m = 0, m_before, total;
@@ -673,14 +672,12 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
       sample_block_scan<NT>(blk, m, c, m_before, c_before, total, c_all);
       // codes of bin b above t into m_z; their number
       auto list = [&](int b) {
-        again();
-#pragma unroll
-        for (int j = 0; j < KPT; ++j) {
-          if (z[j] > t && bins.of(z[j]) == b) {
+        each([&](float z) {
+          if (z > t && bins.of(z) == b) {
             const int to = atomicAdd(&n_listed, 1);
-            if (to < 64) m_z[to] = z[j];
+            if (to < 64) m_z[to] = z;
           }
-        }
+        });
         __syncthreads();
         return n_listed;
       };
@@ -692,14 +689,12 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
         }
         __syncthreads();
         unsigned l = ~0u, h = 0;
-        again();
-#pragma unroll
-        for (int j = 0; j < KPT; ++j) {
-          if (z[j] > t && bins.of(z[j]) == b) {
-            l = min(l, sample_key(z[j]));
-            h = max(h, sample_key(z[j]));
+        each([&](float z) {
+          if (z > t && bins.of(z) == b) {
+            l = min(l, sample_key(z));
+            h = max(h, sample_key(z));
           }
-        }
+        });
         if (h) {
           atomicMin(&key_range[0], l);
           atomicMax(&key_range[1], h);
@@ -759,20 +754,18 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
           keys_of(kb, first, last);
           unsigned long long before;
           const unsigned key = sample_search<NT>(blk, found, part, first, last, want, before, [&](auto f) {
-            again();
-#pragma unroll
-            for (int j = 0; j < KPT; ++j)
-              if (z[j] > -INFINITY && bins.of(z[j]) == kb) f(sample_key(z[j]), [] { return 1ull; });
+            each([&](float z) {
+              if (bins.of(z) == kb) f(sample_key(z), [] { return 1ull; });
+            });
           });
           t = sample_unkey(key);
           r = want - (unsigned)before;
           if (tid == 0) n_listed = 0;
           unsigned long long in = 0, none;
           unsigned none_c, none_all;
-          again();
-#pragma unroll
-          for (int j = 0; j < KPT; ++j)
-            if (z[j] > t && bins.of(z[j]) == kb) in += mass.q(z[j]);
+          each([&](float z) {
+            if (z > t && bins.of(z) == kb) in += mass.q(z);
+          });
           sample_block_scan<NT>(blk, in, 0u, none, none_c, k_in, none_all);
         }
         qt = mass.q(t);
@@ -823,10 +816,9 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
             keys_of(pb, first, last);
             unsigned long long before;
             const unsigned key = sample_search<NT>(blk, found, part, first, last, need, before, [&](auto f) {
-              again();
-#pragma unroll
-              for (int j = 0; j < KPT; ++j)
-                if (z[j] > t && bins.of(z[j]) == pb) f(sample_key(z[j]), [&] { return mass.q(z[j]); });
+              each([&](float z) {
+                if (z > t && bins.of(z) == pb) f(sample_key(z), [&] { return mass.q(z); });
+              });
             });
             t = sample_unkey(key);
             r = sample_ceil_div(need - before, mass.q(t));
@@ -834,17 +826,14 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
         }
       }
       qt = r ? mass.q(t, set.m) : 0ull;
-      again();
     }
     // kept masses, wave by wave
     unsigned at_t = 0;
     unsigned long long sum = 0;
-#pragma unroll
-    for (int j = 0; j < KPT; ++j) {
-      at_t += z[j] == t && r > 0;
-      if (z[j] > t) sum += mass.q(z[j], set.m);
-      if (j & 1) __builtin_amdgcn_sched_barrier(0);
-    }
+    each([&](float z) {
+      at_t += z == t && r > 0;
+      if (z > t) sum += mass.q(z, set.m);
+    });
     at_t = sample_wave_sum(at_t);
     sum = sample_wave_sum(sum);
     if (lane == 0) {
@@ -859,7 +848,7 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
       total += blk.m[v] + min(blk.c[v], r > seen ? r - seen : 0u) * qt;
       seen += blk.c[v];
     }
-    sample_draw<T, NT, KPT>(a, row, logits, 0, mass, set.m, t, r, qt, blk, 0ull, 0u, sample_target(set.u, total), total);
+    sample_draw<T, NT>(a, row, row_z, 0, steps, mass, set.m, t, r, qt, blk, 0ull, 0u, sample_target(set.u, total), total);
     __syncthreads();
   }
 }
@@ -1311,7 +1300,7 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
     blk.c[w] = at_t;
   }
   __syncthreads();
-  sample_draw<T, NT, kSampleChunkIpt>(a, row, logits, i0, mass, set.m, t, ties, qt, blk, sh_before, sh_tied, target, total);
+  sample_draw<T, NT>(a, row, logits, i0, kSampleChunkIpt, mass, set.m, t, ties, qt, blk, sh_before, sh_tied, target, total);
 }
 
 }  // namespace qinco
