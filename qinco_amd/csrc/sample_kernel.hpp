@@ -46,11 +46,20 @@ struct SampleRow {
   bool greedy;
 };
 
+// 1 / x for x > 0: the hardware's estimate and two Newton steps, good to the last bit or two (a tiny or infinite x: the estimate alone)
+__device__ __forceinline__ double sample_reciprocal(double x) {
+  const double e = __builtin_amdgcn_rcp(x);
+  double r = fma(fma(-x, e, 1.0), e, e);
+  r = fma(fma(-x, r, 1.0), r, r);
+  return r == r ? r : e;
+}
+
 __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, long r) {
   SampleRow s;
   const double T = a.T_rows ? (double)a.T_rows[r] : a.T;
   s.greedy = !(T > 0.0);
-  s.y = s.greedy ? 0.0 : 1.4426950408889634074 / T;
+  s.y = s.greedy ? 1.0 : 1.4426950408889634074 * sample_reciprocal(T);
+  s.y = fmax(s.y, 1e-290);   // (T = inf: every finite logit has the same mass, and inf - inf stays out of the arithmetic)
   s.k = a.k_rows ? a.k_rows[r] : a.k;
   if (s.k <= 0 || s.k > a.V) s.k = a.V;
   s.p = a.p_rows ? (double)a.p_rows[r] : a.p;
@@ -86,19 +95,20 @@ constexpr unsigned kSampleKeyMasked = 0x007FFFFFu;   // sample_key(-inf)
 
 // the row's own constants
 struct SampleMass {
-  float top;         // max z
   double zmax, y, scale;
-  // log2 of e = exp((z - max z) / T); at or below -150 the mass is zero
-  __device__ __forceinline__ double arg(float z) const { return z == top ? 0.0 : fmax(((double)z - zmax) * y, -150.0); }
-  // e = 2^x: x = k + f with |f| <= 1/2, the series of exp(f ln 2) to the 12th power (what is left out is below (ln 2 / 2)^13 / 13! =
-  // 2e-16), times 2^k.  No range checks: arg() keeps x inside.
+  // top: max z.  An infinite one stands as a number above all others: what equals it has an argument above 0, everything else one far below
+  __device__ __forceinline__ SampleMass(float top, double log2e_T, int F)
+      : zmax(top < INFINITY ? (double)top : 1.7e308), y(log2e_T), scale(__hiloint2double((1023 + F) << 20, 0)) {}
+  // log2 of e = exp((z - max z) / T); at -150 the mass is zero
+  __device__ __forceinline__ double arg(float z) const { return fmin(fmax(((double)z - zmax) * y, -150.0), 0.0); }
+  // 2^x for -150 <= x <= 0: x = k + f with |f| <= 1/2 (the sum with 1.5 2^52 rounds x to k and leaves it in the low word), the series of
+  // exp(f ln 2) to the 11th power (what is left out is below (ln 2 / 2)^12 / 12! = 7e-15), and k added to the exponent.
   static __device__ __forceinline__ double exp2(double x) {
     constexpr double l = 0.69314718055994530942;
     constexpr double c2 = l * l / 2, c3 = c2 * l / 3, c4 = c3 * l / 4, c5 = c4 * l / 5, c6 = c5 * l / 6, c7 = c6 * l / 7, c8 = c7 * l / 8,
-                     c9 = c8 * l / 9, c10 = c9 * l / 10, c11 = c10 * l / 11, c12 = c11 * l / 12;
-    const double k = rint(x), f = x - k;
-    double e = fma(c12, f, c11);
-    e = fma(e, f, c10);
+                     c9 = c8 * l / 9, c10 = c9 * l / 10, c11 = c10 * l / 11;
+    const double k = x + 0x1.8p52, f = x - (k - 0x1.8p52);
+    double e = fma(c11, f, c10);
     e = fma(e, f, c9);
     e = fma(e, f, c8);
     e = fma(e, f, c7);
@@ -109,7 +119,7 @@ struct SampleMass {
     e = fma(e, f, c2);
     e = fma(e, f, l);
     e = fma(e, f, 1.0);
-    return ldexp(e, (int)k);
+    return __hiloint2double(__double2hiint(e) + (__double2loint(k) << 20), __double2loint(e));
   }
   __device__ __forceinline__ double e(float z) const { return exp2(arg(z)); }
   // as a whole number of 2^-F (scale = 2^F <= 2^51: the sum with 2^52 rounds it to one, ties to even)
@@ -121,9 +131,29 @@ struct SampleMass {
     const double v = e(z);
     return v >= m ? whole(v) : 0ull;
   }
-  // natural logarithm of a code's share of `total`
+  // natural logarithm of a code's share of `total` (1 <= total / scale < 2^25): total / scale = 2^k b with 2/3 < b <= 4/3, and
+  // log b = 2 (s + s^3 / 3 + s^5 / 5 + ...), s = (b - 1) / (b + 1), |s| <= 1/5, to s^19 (what is left out is below 1e-15)
   __device__ __forceinline__ float logp(float z, unsigned long long total) const {
-    return (float)(arg(z) * 0.69314718055994530942 - log((double)total / scale));
+    const double v = (double)total;
+    int k = (__double2hiint(v) >> 20) - 1023;
+    double b = __hiloint2double((__double2hiint(v) & 0xFFFFF) | 1023 << 20, __double2loint(v));
+    if (b > 4.0 / 3.0) {
+      b *= 0.5;
+      ++k;
+    }
+    k -= (__double2hiint(scale) >> 20) - 1023;
+    const double s = (b - 1.0) * sample_reciprocal(b + 1.0), s2 = s * s;
+    double p = 1.0 / 19.0;
+    p = fma(p, s2, 1.0 / 17.0);
+    p = fma(p, s2, 1.0 / 15.0);
+    p = fma(p, s2, 1.0 / 13.0);
+    p = fma(p, s2, 1.0 / 11.0);
+    p = fma(p, s2, 1.0 / 9.0);
+    p = fma(p, s2, 1.0 / 7.0);
+    p = fma(p, s2, 1.0 / 5.0);
+    p = fma(p, s2, 1.0 / 3.0);
+    p = fma(p * s2, s, s);
+    return (float)fma(0.69314718055994530942, arg(z) - (double)k, -2.0 * p);
   }
 };
 
@@ -139,6 +169,7 @@ __device__ __forceinline__ unsigned long long sample_target(double u, unsigned l
 }
 // smallest r with r q >= rem (q >= 1, r < 2^25)
 __device__ __forceinline__ unsigned sample_ceil_div(unsigned long long rem, unsigned long long q) {
+  if (rem <= q) return rem ? 1 : 0;
   unsigned r = (unsigned)((double)rem / (double)q);
   while (r * q < rem) ++r;
   while (r && (r - 1) * q >= rem) --r;
@@ -194,8 +225,8 @@ struct SampleBins {
   __device__ __forceinline__ int of(float z) const { return (int)fminf((zmax - z) * c, last); }
 };
 __device__ __forceinline__ SampleBins sample_bins(float zmax, float zmin, double y, int bins) {
-  const double range = fmin(((double)zmax - (double)zmin) * y, 54.0);
-  const float c = range > 0.0 ? (float)fmin(bins * y / range, 3e38) : 0.f;
+  const float range = fminf((zmax - zmin) * (float)y, 54.f);   // (any c > 0 will do: its rounding moves bins, not codes)
+  const float c = range > 0.f ? fminf((float)bins * (float)y * __builtin_amdgcn_rcpf(range), 3e38f) : 0.f;
   return SampleBins{zmax, zmax < INFINITY ? c : 0.f, (float)(bins - 1)};
 }
 
@@ -239,9 +270,10 @@ struct SampleWaveRow {
 template <typename T, int R>
 __global__ void __launch_bounds__(64 * kSampleRowWaves) sample_wave_kernel(SampleArgs a) {
   __shared__ SampleWaveLds lds[kSampleRowWaves];
-  SampleWaveLds& s = lds[threadIdx.x >> 6];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // (known to be the same in every lane: the row's settings are scalars)
+  SampleWaveLds& s = lds[wave];
   const int lane = threadIdx.x & 63, V = a.V;
-  for (long row = (long)blockIdx.x * kSampleRowWaves + (threadIdx.x >> 6); row < a.n; row += (long)gridDim.x * kSampleRowWaves) {
+  for (long row = (long)blockIdx.x * kSampleRowWaves + wave; row < a.n; row += (long)gridDim.x * kSampleRowWaves) {
     const T* logits = reinterpret_cast<const T*>(a.logits) + row * a.stride;
     const SampleRow set = sample_row(a, row);
     SampleWaveRow<R> w;
@@ -265,7 +297,7 @@ __global__ void __launch_bounds__(64 * kSampleRowWaves) sample_wave_kernel(Sampl
       if (lane == first) sample_answer(a, row, lane * R + at, 0.f);
       continue;
     }
-    const SampleMass mass{zmax, (double)zmax, set.y, ldexp(1.0, a.F)};
+    const SampleMass mass(zmax, set.y, a.F);
     unsigned floored = 0;   // bit j: cut by min-p
 #pragma unroll
     for (int j = 0; j < R; ++j) {
@@ -645,7 +677,7 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
       __syncthreads();
       continue;
     }
-    const SampleMass mass{zmax, (double)zmax, set.y, ldexp(1.0, a.F)};
+    const SampleMass mass(zmax, set.y, a.F);
     float t = -INFINITY;
     unsigned r = 0;
     unsigned long long qt = 0;   // mass of a code at t
@@ -898,8 +930,17 @@ struct SampleLong {
 
 template <typename T>
 __device__ __forceinline__ void sample_load_chunk(const SampleArgs& a, const T* logits, int i0, float (&z)[kSampleChunkIpt]) {
+  if (i0 + kSampleChunk <= a.V) {
+    const T* p = logits + i0 + threadIdx.x;
 #pragma unroll
-  for (int j = 0; j < kSampleChunkIpt; ++j) z[j] = sample_logit(logits, i0 + j * kSampleChunkThreads + (int)threadIdx.x, a.V);
+    for (int j = 0; j < kSampleChunkIpt; ++j) {
+      const float x = GroupNum<T>::get(p[j * kSampleChunkThreads]);
+      z[j] = x == x ? x : -INFINITY;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < kSampleChunkIpt; ++j) z[j] = sample_logit(logits, i0 + j * kSampleChunkThreads + (int)threadIdx.x, a.V);
+  }
 }
 
 template <typename T>
@@ -984,7 +1025,7 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_bins_kernel(Sample
   if (tid == 0) floor = kSampleBins;
   const SampleRange g = sample_range(l, r, sh);   // (its barrier: the bins are cleared)
   if (g.zmax == -INFINITY || set.greedy) return;
-  const SampleMass mass{g.zmax, (double)g.zmax, set.y, ldexp(1.0, a.F)};
+  const SampleMass mass(g.zmax, set.y, a.F);
   const SampleBins bins = sample_bins(g.zmax, g.zmin, set.y, kSampleBins);
   const bool by_count = set.k < a.V;
   int first = kSampleBins;
@@ -1126,7 +1167,7 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_members_kernel(Sam
   if (n == 0) return;
   if (tid == 0) first_here = atomicAdd(&l.state[r].n_members, n);
   __syncthreads();
-  const SampleMass mass{st.zmax, (double)st.zmax, set.y, ldexp(1.0, a.F)};
+  const SampleMass mass(st.zmax, set.y, a.F);
   for (int i = tid; i < min(n, kSampleMembers); i += NT) {
     const int to = first_here + i;
     if (to < kSampleMembers) {
@@ -1162,7 +1203,7 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
     }
     return;
   }
-  const SampleMass mass{st.zmax, (double)st.zmax, set.y, ldexp(1.0, a.F)};
+  const SampleMass mass(st.zmax, set.y, a.F);
   const SampleBins bins = sample_bins(st.zmax, st.zmin, set.y, kSampleBins);
   const T* logits = reinterpret_cast<const T*>(a.logits) + row * a.stride;
   const int n = st.n_members;
