@@ -96,29 +96,28 @@ constexpr unsigned kSampleKeyMasked = 0x007FFFFFu;   // sample_key(-inf)
 // the row's own constants
 struct SampleMass {
   double zmax, y, scale;
+  double c[12];   // of 2^f: (ln 2)^n / n!
   // top: max z.  An infinite one stands as a number above all others: what equals it has an argument above 0, everything else one far below
   __device__ __forceinline__ SampleMass(float top, double log2e_T, int F)
-      : zmax(top < INFINITY ? (double)top : 1.7e308), y(log2e_T), scale(__hiloint2double((1023 + F) << 20, 0)) {}
+      : zmax(top < INFINITY ? (double)top : 1.7e308), y(log2e_T), scale(__hiloint2double((1023 + F) << 20, 0)) {
+    constexpr double l = 0.69314718055994530942;
+    c[0] = 1.0;
+    c[1] = l;
+#pragma unroll
+    for (int n = 2; n < 12; ++n) c[n] = c[n - 1] * l / n;
+    // (kept in scalar registers: as literals the compiler moves each into a vector register pair again before every product)
+#pragma unroll
+    for (int n = 1; n < 12; ++n) asm("" : "+s"(c[n]));
+  }
   // log2 of e = exp((z - max z) / T); at -150 the mass is zero
   __device__ __forceinline__ double arg(float z) const { return fmin(fmax(((double)z - zmax) * y, -150.0), 0.0); }
   // 2^x for -150 <= x <= 0: x = k + f with |f| <= 1/2 (the sum with 1.5 2^52 rounds x to k and leaves it in the low word), the series of
   // exp(f ln 2) to the 11th power (what is left out is below (ln 2 / 2)^12 / 12! = 7e-15), and k added to the exponent.
-  static __device__ __forceinline__ double exp2(double x) {
-    constexpr double l = 0.69314718055994530942;
-    constexpr double c2 = l * l / 2, c3 = c2 * l / 3, c4 = c3 * l / 4, c5 = c4 * l / 5, c6 = c5 * l / 6, c7 = c6 * l / 7, c8 = c7 * l / 8,
-                     c9 = c8 * l / 9, c10 = c9 * l / 10, c11 = c10 * l / 11;
+  __device__ __forceinline__ double exp2(double x) const {
     const double k = x + 0x1.8p52, f = x - (k - 0x1.8p52);
-    double e = fma(c11, f, c10);
-    e = fma(e, f, c9);
-    e = fma(e, f, c8);
-    e = fma(e, f, c7);
-    e = fma(e, f, c6);
-    e = fma(e, f, c5);
-    e = fma(e, f, c4);
-    e = fma(e, f, c3);
-    e = fma(e, f, c2);
-    e = fma(e, f, l);
-    e = fma(e, f, 1.0);
+    double e = c[11];
+#pragma unroll
+    for (int n = 10; n >= 0; --n) e = fma(e, f, c[n]);
     return __hiloint2double(__double2hiint(e) + (__double2loint(k) << 20), __double2loint(e));
   }
   __device__ __forceinline__ double e(float z) const { return exp2(arg(z)); }
@@ -1027,18 +1026,16 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_bins_kernel(Sample
   if (g.zmax == -INFINITY || set.greedy) return;
   const SampleMass mass(g.zmax, set.y, a.F);
   const SampleBins bins = sample_bins(g.zmax, g.zmin, set.y, kSampleBins);
-  const bool by_count = set.k < a.V;
+  const bool by_count = set.k < a.V, by_floor = set.m > 0.0;
   int first = kSampleBins;
 #pragma unroll
   for (int j = 0; j < kSampleChunkIpt; ++j) {
-    if (z[j] > -INFINITY) {
-      const int b = bins.of(z[j]);
-      const double e = mass.e(z[j]);
-      const unsigned long long q = mass.whole(e);
-      if (by_count) atomicAdd(&bin_count[b], 1u);
-      if (q) atomicAdd(&bin_mass[b], q);
-      first = e >= set.m ? first : min(first, b);
-    }
+    const int b = bins.of(z[j]);
+    const double e = mass.e(z[j]);
+    const unsigned long long q = mass.whole(e);
+    if (by_count && z[j] > -INFINITY) atomicAdd(&bin_count[b], 1u);
+    if (q) atomicAdd(&bin_mass[b], q);
+    if (by_floor) first = min(first, e >= set.m || z[j] == -INFINITY ? kSampleBins : b);
     if (j & 1) __builtin_amdgcn_sched_barrier(0);
   }
   if (first < kSampleBins) atomicMin(&floor, first);
