@@ -4,8 +4,11 @@
 //
 // SORT.  key_i = list of entry i; order = stable sort of the entries by key, a radix sort by digits of at most 11 bits, lowest digit
 // first.  Every pass is stable and free of atomics whose order shows: a tile of entries counts its digits (histogram), the counts are
-// summed down the tiles (scan), and every tile ranks its entries again and writes them to base[digit] + rank (scatter).  The rank of an
-// entry = the entries of the same digit before it: inside a wave by ballots over the digit's bits, across waves by a table in LDS.
+// summed down the tiles (scan), and every tile ranks its entries again, orders them by digit in LDS and writes them out in runs (scatter).
+// The rank of an entry = the entries of the same digit before it: inside a wave by ballots over the digit's bits, across waves by a table
+// in LDS.  `place` is the passes' permutations one after the other: each pass notes where it put every entry next to where it found it
+// (neighbouring stores), and the last kernel follows the notes (reads that the cache serves) -- a 4-byte store to a random place costs
+// a whole sector.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -13,8 +16,8 @@
 namespace qinco {
 
 constexpr int kGroupThreads = 512, kGroupWaves = kGroupThreads / 64;
-constexpr int kGroupIpt = 8;                              // entries per thread
-constexpr int kGroupTile = kGroupThreads * kGroupIpt;     // 4096 entries per workgroup
+constexpr int kGroupIpt = 8;                              // entries per thread of the one-workgroup sort
+constexpr int kGroupTile = kGroupThreads * kGroupIpt;     // ... its most entries
 constexpr int kGroupMaxBits = 11, kGroupMaxBins = 1 << kGroupMaxBits;
 constexpr unsigned kGroupNone = 0xFFFFFFFFu;              // key of an entry without a list
 constexpr int kGroupSmallOffsets = 4096;                  // lists up to which the one-workgroup kernel writes the offsets itself
@@ -38,17 +41,19 @@ __device__ __forceinline__ unsigned group_key(const GroupKeys& g, unsigned i, bo
 }
 
 struct GroupPass {
-  GroupKeys in;             // first pass: the lists
-  const unsigned* key_in;   // later passes: keys and entries as the pass before left them, `*total` of them
-  const int* idx_in;
-  unsigned* key_out;        // sorted keys (null: nobody needs them)
-  int* idx_out;             // entries in this pass's order; the last pass: `order`
-  int* place;               // last pass: place[entry] = slot; first pass: -1 for entries without a list
-  int* offsets;             // written by a sort of one pass (E + 1), else null
-  unsigned* counts;         // [tile][bin], after the scan: entries of that bin in earlier tiles
-  unsigned* totals;         // [bin]
-  unsigned* total;          // entries that have a list
-  int* bad;                 // nullable: set to 1 if an id is >= E
+  GroupKeys in;                          // first pass: the lists
+  const unsigned long long* pair_in;     // later passes: key << 32 | entry as the pass before left them, `*total` of them
+  unsigned long long* pair_out;          // ... and for the pass behind this one
+  int* order;                            // last pass: entries in slot order
+  unsigned* key_out;                     // last of several passes: keys in slot order
+  int* place;                            // first pass: where each entry went, -1 without a list
+  int* went;                             // later passes: where each pair went
+  int* offsets;                          // written by a sort of one pass (E + 1), else null
+  unsigned* counts;                      // [tile][bin], after the scan: entries of that bin in earlier tiles
+  unsigned* totals;                      // [bin]
+  unsigned* start;                       // last of several passes: first slot of each bin, and behind the last one (bins + 1)
+  unsigned* total;                       // entries that have a list
+  int* bad;                              // nullable: set to 1 if an id is >= E
   int shift, bits, first, last;
 };
 
@@ -67,49 +72,66 @@ __device__ __forceinline__ unsigned long long group_match(unsigned d, bool valid
   return m;
 }
 
+template <int IPT>
 __global__ void __launch_bounds__(kGroupThreads) group_hist_kernel(GroupPass a) {
   __shared__ unsigned hist[kGroupMaxBins];
   const int bins = 1 << a.bits;
   for (int b = threadIdx.x; b < bins; b += kGroupThreads) hist[b] = 0;
-  __syncthreads();
   const unsigned N = a.first ? a.in.N : *a.total;
   const unsigned mask = bins - 1;
+  unsigned key[IPT];
   bool any_bad = false;
 #pragma unroll
-  for (int r = 0; r < kGroupIpt; ++r) {
-    const unsigned i = blockIdx.x * (unsigned)kGroupTile + r * kGroupThreads + threadIdx.x;
+  for (int r = 0; r < IPT; ++r) {
+    const unsigned i = blockIdx.x * (unsigned)(kGroupThreads * IPT) + r * kGroupThreads + threadIdx.x;
+    key[r] = kGroupNone;
     if (i < N) {
       bool bad = false;
-      const unsigned key = a.first ? group_key(a.in, i, bad) : a.key_in[i];
+      key[r] = a.first ? group_key(a.in, i, bad) : (unsigned)(a.pair_in[i] >> 32);
       any_bad |= bad;
-      if (key != kGroupNone) atomicAdd(&hist[(key >> a.shift) & mask], 1u);
     }
   }
+  __syncthreads();
+#pragma unroll
+  for (int r = 0; r < IPT; ++r)
+    if (key[r] != kGroupNone) atomicAdd(&hist[(key[r] >> a.shift) & mask], 1u);
   if (any_bad && a.bad) *a.bad = 1;
   __syncthreads();
   for (int b = threadIdx.x; b < bins; b += kGroupThreads) a.counts[(size_t)blockIdx.x * bins + b] = hist[b];
 }
 
-// counts[tile][bin] -> entries of the bin in earlier tiles; totals[bin].  A workgroup owns 64 bins, its 16 waves a run of tiles each.
+// counts[tile][bin] -> entries of the bin in earlier tiles; totals[bin].  A workgroup owns 64 bins, its 16 waves a run of tiles each,
+// held in registers up to 16 of them.
 __global__ void __launch_bounds__(1024) group_scan_kernel(unsigned* counts, unsigned* totals, int tiles, int bins) {
   __shared__ unsigned part[16][64];
+  constexpr int HELD = 16;
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int bin = blockIdx.x * 64 + lane;
   const int per = (tiles + 15) / 16;
   const int t0 = w * per, t1 = t0 + per < tiles ? t0 + per : tiles;
-  unsigned sum = 0;
+  unsigned held[HELD], sum = 0;
+#pragma unroll
+  for (int j = 0; j < HELD; ++j) held[j] = bin < bins && t0 + j < t1 ? counts[(size_t)(t0 + j) * bins + bin] : 0;
+#pragma unroll
+  for (int j = 0; j < HELD; ++j) sum += held[j];
   if (bin < bins)
-    for (int t = t0; t < t1; ++t) sum += counts[(size_t)t * bins + bin];
+    for (int t = t0 + HELD; t < t1; ++t) sum += counts[(size_t)t * bins + bin];
   part[w][lane] = sum;
   __syncthreads();
   unsigned run = 0, all = 0;
+#pragma unroll
   for (int v = 0; v < 16; ++v) {
     const unsigned p = part[v][lane];
     run += v < w ? p : 0;
     all += p;
   }
   if (bin < bins) {
-    for (int t = t0; t < t1; ++t) {
+#pragma unroll
+    for (int j = 0; j < HELD; ++j) {
+      if (t0 + j < t1) counts[(size_t)(t0 + j) * bins + bin] = run;
+      run += held[j];
+    }
+    for (int t = t0 + HELD; t < t1; ++t) {
       const size_t o = (size_t)t * bins + bin;
       const unsigned c = counts[o];
       counts[o] = run;
@@ -140,65 +162,56 @@ __device__ __forceinline__ unsigned group_block_scan(unsigned v, unsigned* tmp, 
   return before + s - v;
 }
 
+template <int IPT>
 __global__ void __launch_bounds__(kGroupThreads) group_scatter_kernel(GroupPass a) {
-  __shared__ unsigned short whist[kGroupWaves][kGroupMaxBins];   // entries of a digit in the wave so far, then in earlier waves
-  __shared__ unsigned base[kGroupMaxBins];
+  constexpr int TILE = kGroupThreads * IPT, BPT = kGroupMaxBins / kGroupThreads;
+  __shared__ unsigned long long tile[TILE];                      // the tile's pairs by digit
+  __shared__ unsigned short whist[kGroupWaves][kGroupMaxBins];   // entries of a digit in the wave so far, then in the tile before the wave's
+  __shared__ unsigned base[kGroupMaxBins];                       // first slot of the tile's entries of a digit, less their place in the tile
   __shared__ unsigned tmp[kGroupWaves];
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const int bins = 1 << a.bits;
   const unsigned mask = bins - 1;
-  for (int b = tid; b < bins; b += kGroupThreads)
-    for (int v = 0; v < kGroupWaves; ++v) whist[v][b] = 0;
   const unsigned N = a.first ? a.in.N : *a.total;
-  const unsigned tile0 = blockIdx.x * (unsigned)kGroupTile;
-  unsigned key[kGroupIpt], rank[kGroupIpt];
-  int idx[kGroupIpt];
+  const unsigned tile0 = blockIdx.x * (unsigned)TILE;
+  unsigned long long pair[IPT];
+  unsigned rank[IPT];
 #pragma unroll
-  for (int r = 0; r < kGroupIpt; ++r) {
-    const unsigned i = tile0 + w * (64 * kGroupIpt) + r * 64 + lane;
-    key[r] = kGroupNone;
-    idx[r] = (int)i;
+  for (int r = 0; r < IPT; ++r) {
+    const unsigned i = tile0 + w * (64 * IPT) + r * 64 + lane;
+    pair[r] = ~0ull;
     if (i < N) {
-      bool bad;
       if (a.first) {
-        key[r] = group_key(a.in, i, bad);
-        if (key[r] == kGroupNone) a.place[i] = -1;
+        bool bad;
+        pair[r] = (unsigned long long)group_key(a.in, i, bad) << 32 | i;
       } else {
-        key[r] = a.key_in[i];
-        idx[r] = a.idx_in[i];
+        pair[r] = a.pair_in[i];
       }
     }
   }
-  // the first slot of every digit: totals summed over the digits, plus the digit's entries in earlier tiles
-  const int bpt = (bins + kGroupThreads - 1) / kGroupThreads;   // 1 .. 4 neighbouring bins per thread
-  unsigned mine[kGroupMaxBins / kGroupThreads], s = 0;
+  // thread -> neighbouring bins (1 .. 4)
+  const int bpt = (bins + kGroupThreads - 1) / kGroupThreads;
+  unsigned mine[BPT], earlier[BPT], s = 0;
 #pragma unroll
-  for (int j = 0; j < kGroupMaxBins / kGroupThreads; ++j) {
+  for (int j = 0; j < BPT; ++j) {
     const int b = tid * bpt + j;
-    mine[j] = (j < bpt && b < bins) ? a.totals[b] : 0;
+    const bool in = j < bpt && b < bins;
+    mine[j] = in ? a.totals[b] : 0;
+    earlier[j] = in ? a.counts[(size_t)blockIdx.x * bins + b] : 0;
     s += mine[j];
   }
+  for (int b = tid * 2; b < bins; b += kGroupThreads * 2)   // (two 16-bit counters per store; of one bin there are two all the same)
+    for (int v = 0; v < kGroupWaves; ++v) *reinterpret_cast<unsigned*>(&whist[v][b]) = 0;
   unsigned all;
   unsigned start = group_block_scan(s, tmp, &all);   // (its barriers also stand between the clearing of whist and its use)
 #pragma unroll
-  for (int j = 0; j < kGroupMaxBins / kGroupThreads; ++j) {
-    const int b = tid * bpt + j;
-    if (j < bpt && b < bins) {
-      if (blockIdx.x == 0 && a.offsets && (unsigned)b < a.in.E) a.offsets[b] = (int)start;
-      base[b] = start + a.counts[(size_t)blockIdx.x * bins + b];
-      start += mine[j];
-    }
-  }
-  if (blockIdx.x == 0 && tid == 0) {
-    if (a.offsets) a.offsets[a.in.E] = (int)all;
-    if (a.first) *a.total = all;
-  }
-#pragma unroll
-  for (int r = 0; r < kGroupIpt; ++r) {
-    const bool valid = key[r] != kGroupNone;
-    const unsigned d = (key[r] >> a.shift) & mask;
+  for (int r = 0; r < IPT; ++r) {
+    const unsigned key = (unsigned)(pair[r] >> 32);
+    const bool valid = key != kGroupNone;
+    const unsigned d = (key >> a.shift) & mask;
     const unsigned long long m = group_match(d, valid, a.bits);
     const unsigned below = __builtin_popcountll(m & ((1ull << lane) - 1));
+    rank[r] = 0;
     if (valid) {
       const unsigned seen = group_seen(whist[w][d]);
       rank[r] = seen + below;
@@ -206,38 +219,102 @@ __global__ void __launch_bounds__(kGroupThreads) group_scatter_kernel(GroupPass 
     }
   }
   __syncthreads();
-  for (int b = tid; b < bins; b += kGroupThreads) {
-    unsigned run = 0;
-    for (int v = 0; v < kGroupWaves; ++v) {
-      const unsigned c = whist[v][b];
-      whist[v][b] = (unsigned short)run;
-      run += c;
+  // counts per wave -> places in the tile
+  unsigned here[BPT], h = 0;
+#pragma unroll
+  for (int j = 0; j < BPT; ++j) {
+    const int b = tid * bpt + j;
+    here[j] = 0;
+    if (j < bpt && b < bins)
+      for (int v = 0; v < kGroupWaves; ++v) here[j] += whist[v][b];
+    h += here[j];
+  }
+  unsigned in_tile;
+  unsigned at = group_block_scan(h, tmp, &in_tile);
+#pragma unroll
+  for (int j = 0; j < BPT; ++j) {
+    const int b = tid * bpt + j;
+    if (j < bpt && b < bins) {
+      if (blockIdx.x == 0) {
+        if (a.offsets && (unsigned)b < a.in.E) a.offsets[b] = (int)start;
+        if (a.last && a.start) a.start[b] = start;
+      }
+      base[b] = start + earlier[j] - at;
+      unsigned run = at;
+      for (int v = 0; v < kGroupWaves; ++v) {
+        const unsigned c = whist[v][b];
+        whist[v][b] = (unsigned short)run;
+        run += c;
+      }
+      start += mine[j];
+      at += here[j];
     }
+  }
+  if (blockIdx.x == 0 && tid == 0) {
+    if (a.offsets) a.offsets[a.in.E] = (int)all;
+    if (a.last && a.start) a.start[bins] = all;
+    if (a.first) *a.total = all;
+  }
+  __syncthreads();
+  int* const went = a.first ? a.place : a.went;
+#pragma unroll
+  for (int r = 0; r < IPT; ++r) {
+    const unsigned i = tile0 + w * (64 * IPT) + r * 64 + lane, key = (unsigned)(pair[r] >> 32);
+    int to = -1;
+    if (key != kGroupNone) {
+      const unsigned d = (key >> a.shift) & mask, p = whist[w][d] + rank[r];
+      tile[p] = pair[r];
+      to = (int)(base[d] + p);
+    }
+    if (i < N) went[i] = to;
   }
   __syncthreads();
 #pragma unroll
-  for (int r = 0; r < kGroupIpt; ++r) {
-    if (key[r] != kGroupNone) {
-      const unsigned d = (key[r] >> a.shift) & mask;
-      const unsigned dst = base[d] + whist[w][d] + rank[r];
-      a.idx_out[dst] = idx[r];
-      if (a.key_out) a.key_out[dst] = key[r];
-      if (a.last) a.place[idx[r]] = (int)dst;
+  for (int r = 0; r < IPT; ++r) {
+    const unsigned p = r * kGroupThreads + tid;
+    if (p < in_tile) {
+      const unsigned long long v = tile[p];
+      const unsigned key = (unsigned)(v >> 32), to = base[(key >> a.shift) & mask] + p;
+      if (a.last) {
+        a.order[to] = (int)(unsigned)v;
+        if (a.key_out) a.key_out[to] = key;
+      } else {
+        a.pair_out[to] = v;
+      }
     }
-  }
-  if (a.last) {
-    for (int r = 0; r < kGroupIpt; ++r) {
-      const unsigned p = tile0 + r * kGroupThreads + tid;
-      if (p >= all && p < a.in.N) a.idx_out[p] = -1;
-    }
+    if (a.last && tile0 + p >= all && tile0 + p < a.in.N) a.order[tile0 + p] = -1;
   }
 }
 
-// offsets[e] = entries whose key is below e: a binary search in the sorted keys per list
-__global__ void __launch_bounds__(256) group_offsets_kernel(const unsigned* keys, const unsigned* total, int* offsets, unsigned E) {
-  const unsigned n = *total;
-  for (unsigned long e = blockIdx.x * 256ul + threadIdx.x; e <= E; e += gridDim.x * 256ul) {
-    unsigned lo = 0, hi = n;
+// The end of a sort of several passes, two jobs side by side: workgroups below `follow` follow the passes behind the first one, place[i] =
+// went2[went1[place[i]]], four entries per thread; the others search the sorted keys for offsets[e] = entries whose key is below e, inside
+// e's bin of the last pass where there is one (start: bins of keys >> shift; null: everything is searched).
+__global__ void __launch_bounds__(256) group_end_kernel(unsigned follow, int* place, const int* went1, const int* went2, unsigned N,
+                                                        const unsigned* keys, const unsigned* total, const unsigned* start, int shift,
+                                                        int* offsets, unsigned E) {
+  if (blockIdx.x < follow) {
+    const unsigned i0 = blockIdx.x * 1024u + threadIdx.x;
+    int p[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) p[r] = i0 + r * 256 < N ? place[i0 + r * 256] : -1;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) p[r] = p[r] >= 0 ? went1[p[r]] : -1;
+    if (went2) {
+#pragma unroll
+      for (int r = 0; r < 4; ++r) p[r] = p[r] >= 0 ? went2[p[r]] : -1;
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (i0 + r * 256 < N) place[i0 + r * 256] = p[r];
+    return;
+  }
+  for (unsigned long e = (blockIdx.x - follow) * 256ul + threadIdx.x; e <= E; e += (gridDim.x - follow) * 256ul) {
+    unsigned lo = 0, hi = *total;
+    if (e == E) lo = hi;
+    else if (start) {
+      lo = start[e >> shift];
+      hi = start[(e >> shift) + 1];
+    }
     while (lo < hi) {
       const unsigned mid = lo + (hi - lo) / 2;
       if (keys[mid] < e) lo = mid + 1;
@@ -343,11 +420,11 @@ __global__ void __launch_bounds__(kGroupThreads) group_small_kernel(GroupPass a,
   for (unsigned p = tid; p < a.in.N; p += kGroupThreads) {
     if (p < n) {
       const int i = sidx[p];
-      a.idx_out[p] = i;
+      a.order[p] = i;
       a.place[i] = (int)p;
       if (a.key_out) a.key_out[p] = skey[p];
     } else {
-      a.idx_out[p] = -1;
+      a.order[p] = -1;
     }
   }
   if (tid == 0 && a.total) *a.total = n;

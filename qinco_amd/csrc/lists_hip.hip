@@ -163,34 +163,62 @@ extern "C" int qinco_sample_codes(const void* logits, int dtype, int64_t row_str
 // ---------------------------------------------------------------------------------------------
 namespace {
 struct GroupPlan {
-  int bits, passes;     // bits of one digit (the same for every pass)
+  int bits, passes;                                       // bits of one digit (the same for every pass)
+  int ipt;
   int64_t tiles;
-  // workspace, in 32-bit words: total | totals | counts | key and entry buffers of the passes
-  int64_t totals, counts, buf, words;
-  int buffers;          // arrays of N words behind `buf`
+  int64_t totals, start, counts, pairs, keys, went, words;   // workspace in 32-bit words (the total of entries is its first)
 };
 }  // namespace
 
+// Entries per thread.  A tile has a cost of its own (tables of its digits), few tiles leave the chip empty.  Measured, a sort by 1024 lists
+// with 2 / 4 / 8 per thread: 2^17 entries 12.6 / 14.4 / 18.9 us, 2^18 14.4 / 15.4 / 19.5, 2^19 23.3 / 17.9 / 20.7, 2^20 43.4 / 28.4 / 24.5,
+// 2^22 151 / 104 / 67; by 2^20 lists 2^17 34.9 / 38.2 / 45.9, 2^18 41.8 / 43.7 / 50.5, 2^19 63.8 / 53.3 / 58.2, 2^20 112 / 79.6 / 70.3.
 static GroupPlan group_plan(int64_t N, int64_t E) {
   GroupPlan p{};
   const int all = bits_of((uint64_t)E);
   p.passes = all <= kGroupMaxBits ? 1 : (all + kGroupMaxBits - 1) / kGroupMaxBits;
   p.bits = (all + p.passes - 1) / p.passes;
-  p.tiles = (N + kGroupTile - 1) / kGroupTile;
+  p.ipt = N <= (1 << 18) ? 2 : N <= (1 << 19) ? 4 : 8;
+  p.tiles = (N + kGroupThreads * p.ipt - 1) / (kGroupThreads * p.ipt);
   const int64_t bins = (int64_t)1 << p.bits;
-  const bool small = p.tiles <= 1;
-  // two passes: key + entry of the first, sorted keys of the second; three: the same, and the second's entries
-  p.buffers = small ? (E > kGroupSmallOffsets ? 1 : 0) : (p.passes == 1 ? 0 : p.passes == 2 ? 3 : 4);
-  p.totals = 16;
-  p.counts = p.totals + (small ? 0 : bins);
-  p.buf = p.counts + (small ? 0 : p.tiles * bins);
-  p.words = p.buf + p.buffers * N;
+  const bool small = N <= kGroupTile;
+  int64_t at = 16;
+  auto take = [&](int64_t& o, int64_t words) {
+    o = at;
+    at += (words + 15) / 16 * 16;
+  };
+  take(p.totals, small ? 0 : bins);
+  take(p.start, small ? 0 : bins + 1);
+  take(p.counts, small ? 0 : p.tiles * bins);
+  take(p.pairs, small || p.passes == 1 ? 0 : 2 * N * (p.passes == 2 ? 1 : 2));
+  take(p.keys, (small ? E > kGroupSmallOffsets : p.passes > 1) ? N : 0);
+  take(p.went, small ? 0 : N * (p.passes - 1));
+  p.words = at;
   return p;
 }
 
 extern "C" int64_t qinco_group_workspace(int64_t entries, int64_t n_lists) {
   if (entries < 0 || entries > INT32_MAX || n_lists < 1 || n_lists > kMaxLists) return 0;
   return group_plan(entries, n_lists).words * 4;
+}
+
+template <typename F>
+static void with_ipt(int ipt, F f) {
+  if (ipt == 2) f(std::integral_constant<int, 2>{});
+  else if (ipt == 4) f(std::integral_constant<int, 4>{});
+  else f(std::integral_constant<int, 8>{});
+}
+
+// N entries to follow (0: none), E + 1 offsets to find
+static int launch_end(int* place, const int* went1, const int* went2, int64_t N, const unsigned* keys, const unsigned* total,
+                      const unsigned* start, int shift, int* offsets, unsigned E, hipStream_t st) {
+  const unsigned follow = (unsigned)((N + 1023) / 1024);
+  long g = ((long)E + 256) / 256;
+  if (g > 4096) g = 4096;
+  hipLaunchKernelGGL(group_end_kernel, dim3(follow + (unsigned)g), dim3(256), 0, st, follow, place, went1, went2, (unsigned)N, keys, total,
+                     start, shift, offsets, E);
+  HIP_TRY(hipGetLastError());
+  return QINCO_OK;
 }
 
 extern "C" int qinco_group_rows(const void* lists, int code_dtype, int64_t row_stride, int64_t n, int32_t k, int64_t n_lists, int32_t* order,
@@ -212,50 +240,44 @@ extern "C" int qinco_group_rows(const void* lists, int code_dtype, int64_t row_s
   GroupPass a{};
   a.in = GroupKeys{lists, code_dtype, (long)row_stride, (unsigned)k, (unsigned)N, E};
   a.place = place;
+  a.order = order;
   a.total = ws;
   a.totals = ws + p.totals;
   a.counts = ws + p.counts;
   a.bad = bad;
   a.bits = p.bits;
   a.first = a.last = 1;
-  a.idx_out = order;
-  unsigned* sorted = nullptr;   // keys in slot order, where the offsets are searched in them
-  if (p.tiles <= 1) {
-    if (p.buffers) sorted = ws + p.buf;
-    a.key_out = sorted;
-    a.offsets = sorted ? nullptr : offsets;
+  if (N <= kGroupTile) {
+    const bool search = E > (unsigned)kGroupSmallOffsets;
+    a.key_out = search ? ws + p.keys : nullptr;
+    a.offsets = search ? nullptr : offsets;
     hipLaunchKernelGGL(group_small_kernel, dim3(1), dim3(kGroupThreads), 0, st, a, p.passes);
     HIP_TRY(hipGetLastError());
-  } else {
-    unsigned* buf = ws + p.buf;
-    unsigned* keys[2] = {buf, buf + N};
-    int* idx[2] = {reinterpret_cast<int*>(buf + 2 * N), reinterpret_cast<int*>(buf + 3 * N)};
-    const int bins = 1 << p.bits;
-    for (int pass = 0; pass < p.passes; ++pass) {
-      a.shift = pass * p.bits;
-      a.first = pass == 0;
-      a.last = pass == p.passes - 1;
-      a.key_in = pass ? keys[(pass - 1) & 1] : nullptr;
-      a.idx_in = pass ? idx[(pass - 1) & 1] : nullptr;
-      a.key_out = p.passes > 1 ? keys[pass & 1] : nullptr;
-      a.idx_out = a.last ? order : idx[pass & 1];
-      a.offsets = p.passes == 1 ? offsets : nullptr;
-      if (a.last && p.passes > 1) sorted = a.key_out;
-      hipLaunchKernelGGL(group_hist_kernel, dim3((unsigned)p.tiles), dim3(kGroupThreads), 0, st, a);
-      HIP_TRY(hipGetLastError());
-      hipLaunchKernelGGL(group_scan_kernel, dim3((unsigned)((bins + 63) / 64)), dim3(1024), 0, st, a.counts, a.totals, (int)p.tiles, bins);
-      HIP_TRY(hipGetLastError());
-      hipLaunchKernelGGL(group_scatter_kernel, dim3((unsigned)p.tiles), dim3(kGroupThreads), 0, st, a);
-      HIP_TRY(hipGetLastError());
-    }
+    return search ? launch_end(nullptr, nullptr, nullptr, 0, a.key_out, ws, nullptr, 0, offsets, E, st) : QINCO_OK;
   }
-  if (sorted) {
-    long g = ((long)n_lists + 256) / 256;
-    if (g > 4096) g = 4096;
-    hipLaunchKernelGGL(group_offsets_kernel, dim3((unsigned)g), dim3(256), 0, st, sorted, a.total, offsets, E);
+  unsigned long long* pairs = reinterpret_cast<unsigned long long*>(ws + p.pairs);
+  int* went = reinterpret_cast<int*>(ws + p.went);
+  const int bins = 1 << p.bits;
+  const dim3 grid((unsigned)p.tiles), block(kGroupThreads);
+  for (int pass = 0; pass < p.passes; ++pass) {
+    a.shift = pass * p.bits;
+    a.first = pass == 0;
+    a.last = pass == p.passes - 1;
+    a.pair_in = pass ? pairs + (int64_t)((pass - 1) & 1) * N : nullptr;
+    a.pair_out = a.last ? nullptr : pairs + (int64_t)(pass & 1) * N;
+    a.key_out = a.last && pass ? ws + p.keys : nullptr;
+    a.start = a.last && pass ? ws + p.start : nullptr;
+    a.went = pass ? went + (int64_t)(pass - 1) * N : nullptr;
+    a.offsets = p.passes == 1 ? offsets : nullptr;
+    with_ipt(p.ipt, [&](auto ipt) { hipLaunchKernelGGL((group_hist_kernel<decltype(ipt)::value>), grid, block, 0, st, a); });
+    HIP_TRY(hipGetLastError());
+    hipLaunchKernelGGL(group_scan_kernel, dim3((unsigned)((bins + 63) / 64)), dim3(1024), 0, st, a.counts, a.totals, (int)p.tiles, bins);
+    HIP_TRY(hipGetLastError());
+    with_ipt(p.ipt, [&](auto ipt) { hipLaunchKernelGGL((group_scatter_kernel<decltype(ipt)::value>), grid, block, 0, st, a); });
     HIP_TRY(hipGetLastError());
   }
-  return QINCO_OK;
+  if (p.passes == 1) return QINCO_OK;
+  return launch_end(place, went, p.passes > 2 ? went + N : nullptr, N, a.key_out, ws, a.start, a.shift, offsets, E, st);
 }
 
 // rows of `bytes` bytes at these addresses and strides: the widest unit they all are multiples of

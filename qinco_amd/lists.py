@@ -6,37 +6,34 @@ carries rows into that order, `RowGroups.combine` brings them back with weights;
 """
 from __future__ import annotations
 
+import torch
+from torch.autograd.function import once_differentiable
+
 from . import _lib
 from .sample import on_device, on_its_device, row_type, unit_rows
 
 MAX_LISTS = 1 << 24
-
-
-def _stream(dev):
-    import torch
-    return torch.cuda.current_stream(dev).cuda_stream
+_IDS = {torch.int64: _lib.CODE_I64, torch.int32: _lib.CODE_I32, torch.uint8: _lib.CODE_U8}
 
 
 def group_rows(lists, n_lists: int, check: bool = True) -> "RowGroups":
     """lists: torch CUDA tensor (n,) or (n, k) of int64 / int32 / uint8 ids in [0, n_lists), any row stride (`codes[:, 0]` is taken as it
     is); an id < 0 has no list.  Returns the entries (row * k + slot) in list order, stable: RowGroups.  Asynchronous on the current
     stream, except for check: wait and raise IndexError if an id is >= n_lists; check=False leaves such an entry without a list."""
-    import torch
     lib = _lib.load()
     on_device(lists, "lists")
     if lists.dim() not in (1, 2):
         raise ValueError(f"lists must be (n,) or (n, k), got {tuple(lists.shape)}")
     if not 1 <= int(n_lists) <= MAX_LISTS:
         raise ValueError(f"n_lists must be in [1, 2^24], got {n_lists}")
-    code = {torch.int64: _lib.CODE_I64, torch.int32: _lib.CODE_I32, torch.uint8: _lib.CODE_U8}.get(lists.dtype)
+    code = _IDS.get(lists.dtype)
     if code is None:
         raise ValueError(f"lists must be int64, int32 or uint8, got {lists.dtype}")
-    if lists.dim() == 1:
-        lists = lists.unsqueeze(1)
-    n, k = lists.shape
+    n, k = lists.shape if lists.dim() == 2 else (lists.shape[0], 1)
     if k < 1 or n * k >= 1 << 31:
         raise ValueError(f"need k >= 1 and n k < 2^31, got {tuple(lists.shape)}")
-    lists = unit_rows(lists)
+    if k > 1:
+        lists = unit_rows(lists)
     dev = lists.device
     order = torch.empty(n * k, dtype=torch.int32, device=dev)
     place = torch.empty((n, k), dtype=torch.int32, device=dev)
@@ -45,10 +42,12 @@ def group_rows(lists, n_lists: int, check: bool = True) -> "RowGroups":
     need = lib.qinco_group_workspace(n * k, int(n_lists))
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
     on_its_device(dev, lib.qinco_group_rows, lists.data_ptr(), code, lists.stride(0), n, k, int(n_lists), order.data_ptr(), place.data_ptr(),
-                  offsets.data_ptr(), bad.data_ptr() if check else None, ws.data_ptr(), need, _stream(dev))
+                  offsets.data_ptr(), bad.data_ptr() if check else None, ws.data_ptr(), need)
     if check and int(bad):
         raise IndexError(f"a list id is >= n_lists = {n_lists}")
-    return RowGroups(order, place, offsets)
+    groups = RowGroups.__new__(RowGroups)
+    groups._set(order, place, offsets)
+    return groups
 
 
 class RowGroups:
@@ -58,12 +57,14 @@ class RowGroups:
       offsets (n_lists + 1,) first place of each list; the last value = places in use"""
 
     def __init__(self, order, place, offsets):
-        import torch
         for t, what, dim in ((order, "order", 1), (place, "place", 2), (offsets, "offsets", 1)):
             if on_device(t, what).dtype != torch.int32 or t.dim() != dim or not t.is_contiguous() or t.device != place.device:
                 raise ValueError(f"{what} must be a contiguous int32 tensor of {dim} dimension(s) on one device with the others")
         if order.numel() != place.numel() or place.shape[1] < 1 or offsets.numel() < 2:
             raise ValueError(f"order {tuple(order.shape)}, place {tuple(place.shape)}, offsets {tuple(offsets.shape)} do not belong together")
+        self._set(order, place, offsets)
+
+    def _set(self, order, place, offsets):
         self.order, self.place, self.offsets = order, place, offsets
         self.n, self.k = place.shape
         self.n_lists = offsets.numel() - 1
@@ -80,18 +81,16 @@ class RowGroups:
     def gather(self, x):
         """x (n, D) of any type, also code rows -> (n k, D): row order[s] // k at place s, zeros behind the last place in use.
         The gradient is the sum over a row's places, in 32 bits, rounded once (float32, float16, bfloat16)."""
-        import torch
         x = self._rows(x, self.n, "x")
         if x.requires_grad and torch.is_grad_enabled():
             row_type(x, "x that requires a gradient")
-            return _functions()[0].apply(x, self)
+            return _Gather.apply(x, self)
         return self._gather(x)
 
     def combine(self, y, weights=None):
         """y (n k, D) float32 / float16 / bfloat16 in list order -> (n, D): sum_j weights[r, j] y[place[r, j]] over the entries that have
         a list (zeros for a row without one), in 32 bits in the order of j, rounded once.  weights (n, k) float32 or y's type; None: ones.
         Rows of y behind the last place in use and weights of entries without a list are not read; their gradients are zeros."""
-        import torch
         y = self._rows(y, self.n * self.k, "y")
         row_type(y, "y")
         if weights is not None:
@@ -99,7 +98,7 @@ class RowGroups:
                 raise ValueError(f"weights must be ({self.n}, {self.k}) float32 or {y.dtype} on {y.device}, got {tuple(weights.shape)} {weights.dtype}")
             weights = weights.contiguous()
         if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
-            return _functions()[1].apply(y, weights, self)
+            return _Combine.apply(y, weights, self)
         return self._combine(y, weights)
 
     # -- the library calls; arguments are checked already
@@ -107,70 +106,55 @@ class RowGroups:
         return self.offsets.data_ptr() + 4 * self.n_lists
 
     def _gather(self, x):
-        import torch
         out = torch.empty((self.n * self.k, x.shape[1]), dtype=x.dtype, device=x.device)
         size = x.element_size()
         on_its_device(x.device, _lib.load().qinco_group_gather, x.data_ptr(), x.stride(0) * size, x.shape[1] * size, self.place.data_ptr(),
-                      self._end(), self.n, self.k, out.data_ptr(), _stream(x.device))
+                      self._end(), self.n, self.k, out.data_ptr())
         return out
 
     def _combine(self, y, weights):
-        import torch
         out = torch.empty((self.n, y.shape[1]), dtype=y.dtype, device=y.device)
         on_its_device(y.device, _lib.load().qinco_group_combine, y.data_ptr(), row_type(y, "y"), y.stride(0), y.shape[1],
                       weights.data_ptr() if weights is not None else None, row_type(weights, "weights") if weights is not None else 0,
-                      self.place.data_ptr(), self.n, self.k, out.data_ptr(), _stream(y.device))
+                      self.place.data_ptr(), self.n, self.k, out.data_ptr())
         return out
 
     def _combine_grad(self, dout, y, weights, need_dy, need_dw):
-        import torch
         dy = torch.empty(y.shape, dtype=y.dtype, device=y.device) if need_dy else None
         dw = torch.empty(weights.shape, dtype=weights.dtype, device=y.device) if need_dw else None
         on_its_device(y.device, _lib.load().qinco_group_combine_grad, dout.data_ptr(), dout.stride(0), y.data_ptr(), y.stride(0),
                       row_type(y, "y"), y.shape[1], weights.data_ptr(), row_type(weights, "weights"), self.place.data_ptr(), self._end(),
-                      self.n, self.k, dy.data_ptr() if need_dy else None, dw.data_ptr() if need_dw else None, _stream(y.device))
+                      self.n, self.k, dy.data_ptr() if need_dy else None, dw.data_ptr() if need_dw else None)
         return dy, dw
 
 
-_FUNCTIONS = None
+class _Gather(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, groups):
+        ctx.groups = groups
+        ctx.save_for_backward(groups.place, groups.offsets)   # (an in-place change between the passes is an error)
+        return groups._gather(x)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        ctx.saved_tensors
+        return ctx.groups._combine(unit_rows(dout), None), None
 
 
-def _functions():
-    """(gather, combine) as torch.autograd functions; made at the first call that needs a gradient (torch is imported late here)."""
-    global _FUNCTIONS
-    if _FUNCTIONS is None:
-        import torch
-        from torch.autograd.function import once_differentiable
+class _Combine(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y, weights, groups):
+        ctx.groups, ctx.weighted = groups, weights is not None
+        ctx.save_for_backward(groups.place, groups.offsets, *((y, weights) if ctx.weighted else ()))
+        return groups._combine(y, weights)
 
-        class Gather(torch.autograd.Function):
-            @staticmethod
-            def forward(ctx, x, groups):
-                ctx.groups = groups
-                ctx.save_for_backward(groups.place, groups.offsets)   # (an in-place change between the passes is an error)
-                return groups._gather(x)
-
-            @staticmethod
-            @once_differentiable
-            def backward(ctx, dout):
-                ctx.saved_tensors
-                return ctx.groups._combine(unit_rows(dout), None), None
-
-        class Combine(torch.autograd.Function):
-            @staticmethod
-            def forward(ctx, y, weights, groups):
-                ctx.groups, ctx.weighted = groups, weights is not None
-                ctx.save_for_backward(groups.place, groups.offsets, *((y, weights) if ctx.weighted else ()))
-                return groups._combine(y, weights)
-
-            @staticmethod
-            @once_differentiable
-            def backward(ctx, dout):
-                saved = ctx.saved_tensors
-                dout = unit_rows(dout)
-                if not ctx.weighted:
-                    return ctx.groups._gather(dout), None, None
-                dy, dw = ctx.groups._combine_grad(dout, saved[2], saved[3], *ctx.needs_input_grad[:2])
-                return dy, dw, None
-
-        _FUNCTIONS = (Gather, Combine)
-    return _FUNCTIONS
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        saved = ctx.saved_tensors
+        dout = unit_rows(dout)
+        if not ctx.weighted:
+            return ctx.groups._gather(dout), None, None
+        dy, dw = ctx.groups._combine_grad(dout, saved[2], saved[3], *ctx.needs_input_grad[:2])
+        return dy, dw, None

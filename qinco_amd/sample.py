@@ -9,24 +9,26 @@ import ctypes as C
 import math
 
 import numpy as np
+import torch
 
 from . import _lib
-from .engine import _is_torch
 
 _CODES = {np.dtype(np.int64): _lib.CODE_I64, np.dtype(np.int32): _lib.CODE_I32}
 
 
+_TYPES = {torch.float32: _lib.T_F32, torch.float16: _lib.T_F16, torch.bfloat16: _lib.T_BF16}
+
+
 def on_device(t, what: str):
     """A torch CUDA tensor, or an error that names the argument."""
-    if not (_is_torch(t) and t.is_cuda):
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
         raise ValueError(f"{what} must be a torch CUDA tensor")
     return t
 
 
 def row_type(t, what: str) -> int:
     """QINCO_T_* of a tensor of rows."""
-    import torch
-    code = {torch.float32: _lib.T_F32, torch.float16: _lib.T_F16, torch.bfloat16: _lib.T_BF16}.get(t.dtype)
+    code = _TYPES.get(t.dtype)
     if code is None:
         raise ValueError(f"{what} must be float32, float16 or bfloat16, got {t.dtype}")
     return code
@@ -38,13 +40,15 @@ def unit_rows(t):
 
 
 def on_its_device(dev, call, *args) -> None:
-    """One library call with `dev` current (kernels are launched on a stream of the current device)."""
-    import torch
+    """One library call on the current stream of `dev` (its last argument), with `dev` current: kernels are launched on a stream of the
+    current device."""
     if torch.cuda.current_device() == dev.index:
-        _lib.check(call(*args))
+        rc = call(*args, torch.cuda.current_stream().cuda_stream)
     else:
         with torch.cuda.device(dev):
-            _lib.check(call(*args))
+            rc = call(*args, torch.cuda.current_stream().cuda_stream)
+    if rc:
+        _lib.check(rc)
 
 
 def sample_codes(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, code_dtype=np.int64, return_logp: bool = False):
@@ -60,7 +64,6 @@ def sample_codes(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, c
     the same inputs give the same codes, whatever else is in the batch.
 
     temperature, top_p, min_p (float32) and top_k (int32) may be tensors (n,) with a value per row; there a temperature <= 0 is 0."""
-    import torch
     lib = _lib.load()
     on_device(logits, "logits")
     if logits.dim() != 2 or logits.shape[1] < 1:
@@ -76,7 +79,7 @@ def sample_codes(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, c
     params = _lib.QincoSampleParams(struct_bytes=C.sizeof(_lib.QincoSampleParams))
     for name, value, want in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
                               ("min_p", min_p, torch.float32)):
-        if _is_torch(value):
+        if isinstance(value, torch.Tensor):
             if on_device(value, name).shape != (n,) or value.dtype != want:
                 raise ValueError(f"{name} must be a number or ({n},) {want}, got {tuple(value.shape)} {value.dtype}")
             keep.append(value.contiguous())
@@ -87,7 +90,7 @@ def sample_codes(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, c
             setattr(params, name, float(value))
     if any(t.device != dev for t in keep):
         raise ValueError("logits, u and the settings must be on one device")
-    if not _is_torch(temperature) and not 0.0 <= params.temperature < math.inf:
+    if not isinstance(temperature, torch.Tensor) and not 0.0 <= params.temperature < math.inf:
         raise ValueError(f"temperature must be finite and >= 0, got {temperature}")
     if params.top_p != params.top_p or params.min_p != params.min_p or params.min_p > 1.0:
         raise ValueError(f"top_p must be a number and min_p at most 1, got {top_p} and {min_p}")
@@ -100,5 +103,5 @@ def sample_codes(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, c
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     on_its_device(dev, lib.qinco_sample_codes, logits.data_ptr(), dtype, logits.stride(0), n, V, u.data_ptr(), u.dtype == torch.float64,
                   C.byref(params), codes.data_ptr(), code, logp.data_ptr() if return_logp else None,
-                  ws.data_ptr() if need else None, need, torch.cuda.current_stream(dev).cuda_stream)
+                  ws.data_ptr() if need else None, need)
     return (codes, logp) if return_logp else codes
