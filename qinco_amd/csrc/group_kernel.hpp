@@ -441,37 +441,59 @@ __global__ void __launch_bounds__(kGroupThreads) group_small_kernel(GroupPass a,
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Rows.  All of these are bound by HBM: a row is read or written once, in the widest units that its width, strides and base allow
-// (16 bytes down to 1); `lanes` (a power of two up to 64) lanes share a row and step through its units, so no index is divided.
+// Rows.  All of these are bound by HBM: a row is read or written once, in units of 16 bytes whatever its alignment (the hardware takes
+// 16-byte accesses at any element); the last unit ends with the row and overlaps the one before it.  Rows shorter than that go element by
+// element (E = 1).  `lanes` (a power of two up to 64) lanes share a row and step through its units, so no index is divided.
 // ---------------------------------------------------------------------------------------------------------------------
 struct GroupRows {
   const int* place;    // (n, k)
   const int* end;      // = offsets + E: slots in use
   long n, N;           // rows, entries = n k
   int k;
-  int units;           // units per row
+  int D, units;        // elements and units per row
   int lanes_log2;
 };
 
-template <typename U>
-__global__ void __launch_bounds__(256) group_gather_kernel(GroupRows g, const char* x, long x_stride, char* out, long row_bytes) {
+template <typename T, int E>
+struct GroupUnit {
+  struct alignas(sizeof(T)) Raw { T v[E]; };
+  T v[E];
+  __device__ __forceinline__ void load(const T* at) {
+    const Raw r = *reinterpret_cast<const Raw*>(at);
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] = r.v[e];
+  }
+  __device__ __forceinline__ void store(T* at) const {
+    Raw r;
+#pragma unroll
+    for (int e = 0; e < E; ++e) r.v[e] = v[e];
+    *reinterpret_cast<Raw*>(at) = r;
+  }
+};
+
+// T: an unsigned type, the widest (up to 8 bytes) that rows, strides and bases are multiples of
+template <typename T, int E>
+__global__ void __launch_bounds__(256) group_gather_kernel(GroupRows g, const T* x, long x_stride, T* out) {
   const int lanes = 1 << g.lanes_log2;
   const int u0 = threadIdx.x & (lanes - 1);
   const long per = 256 >> g.lanes_log2;
   const long first = (long)blockIdx.x * per + (threadIdx.x >> g.lanes_log2), step = (long)gridDim.x * per;
+  GroupUnit<T, E> v;
   for (long r = first; r < g.n; r += step) {
     const int* pl = g.place + r * g.k;
-    const U* src = reinterpret_cast<const U*>(x + r * x_stride);
     for (int u = u0; u < g.units; u += lanes) {
-      const U v = src[u];
+      const int at = min(u * E, g.D - E);
+      v.load(x + r * x_stride + at);
       for (int j = 0; j < g.k; ++j) {
         const int p = pl[j];
-        if (p >= 0) reinterpret_cast<U*>(out + (long)p * row_bytes)[u] = v;
+        if (p >= 0) v.store(out + (long)p * g.D + at);
       }
     }
   }
+#pragma unroll
+  for (int e = 0; e < E; ++e) v.v[e] = T{};
   for (long s = *g.end + first; s < g.N; s += step)
-    for (int u = u0; u < g.units; u += lanes) reinterpret_cast<U*>(out + s * row_bytes)[u] = U{};
+    for (int u = u0; u < g.units; u += lanes) v.store(out + s * g.D + min(u * E, g.D - E));
 }
 
 template <typename T> struct GroupNum;
@@ -488,8 +510,6 @@ template <> struct GroupNum<__bf16> {
   static __device__ __forceinline__ __bf16 put(float v) { return (__bf16)v; }
 };
 
-template <typename T, int E> struct alignas(sizeof(T) * E) GroupVec { T v[E]; };
-
 // weight of entry i in 32 bits (w_dtype: QINCO_T_*; no weights: 1)
 __device__ __forceinline__ float group_weight(const void* w, int w_dtype, long i) {
   if (!w) return 1.f;
@@ -499,85 +519,138 @@ __device__ __forceinline__ float group_weight(const void* w, int w_dtype, long i
 }
 
 // out[r] = sum_j w[r, j] y[place[r, j]]: sums in 32 bits in the order of j, rounded once.  The gradient of the gather is this with
-// weights of one.
-template <typename T, int E>
+// weights of one.  J entries of a row are loaded before the first one is used.
+template <typename T, int E, int J>
 __global__ void __launch_bounds__(256) group_combine_kernel(GroupRows g, const T* y, long y_stride, const void* wt, int w_dtype, T* out) {
-  using V = GroupVec<T, E>;
   const int lanes = 1 << g.lanes_log2;
   const int u0 = threadIdx.x & (lanes - 1);
   const long per = 256 >> g.lanes_log2;
   const long first = (long)blockIdx.x * per + (threadIdx.x >> g.lanes_log2), step = (long)gridDim.x * per;
   for (long r = first; r < g.n; r += step) {
     for (int u = u0; u < g.units; u += lanes) {
+      const int at = min(u * E, g.D - E);
       float acc[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) acc[e] = 0.f;
-      for (int j = 0; j < g.k; ++j) {
-        const int p = g.place[r * g.k + j];
-        if (p >= 0) {
-          const float w = group_weight(wt, w_dtype, r * g.k + j);
-          const V v = reinterpret_cast<const V*>(y + (long)p * y_stride)[u];
+      for (int j0 = 0; j0 < g.k; j0 += J) {
+        int p[J];
+        float w[J];
+        GroupUnit<T, E> v[J];
 #pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] = fmaf(w, GroupNum<T>::get(v.v[e]), acc[e]);
+        for (int j = 0; j < J; ++j) p[j] = j0 + j < g.k ? g.place[r * g.k + j0 + j] : -1;
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          if (p[j] >= 0) {
+            w[j] = group_weight(wt, w_dtype, r * g.k + j0 + j);
+            v[j].load(y + (long)p[j] * y_stride + at);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+          if (p[j] >= 0) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[e] = fmaf(w[j], GroupNum<T>::get(v[j].v[e]), acc[e]);
+          }
         }
       }
-      V o;
+      GroupUnit<T, E> o;
 #pragma unroll
       for (int e = 0; e < E; ++e) o.v[e] = GroupNum<T>::put(acc[e]);
-      reinterpret_cast<V*>(out + r * (long)g.units * E)[u] = o;
+      o.store(out + r * g.D + at);
     }
   }
 }
 
-// dy[place[r, j]] = w[r, j] dout[r], dw[r, j] = <dout[r], y[place[r, j]]> in one pass over y and dout; rows of dy no entry owns: zeros
+// sum over the 2^lanes_log2 neighbouring lanes of a row: inside 16 lanes by DPP (swap neighbours, swap pairs, mirror halves, mirror)
+template <int CTRL>
+__device__ __forceinline__ float group_dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float group_lanes_sum(float v, int lanes_log2) {
+  if (lanes_log2 > 0) v += group_dpp<0xB1>(v);
+  if (lanes_log2 > 1) v += group_dpp<0x4E>(v);
+  if (lanes_log2 > 2) v += group_dpp<0x141>(v);
+  if (lanes_log2 > 3) v += group_dpp<0x140>(v);
+  if (lanes_log2 > 4) v += __shfl_xor(v, 16, 64);
+  if (lanes_log2 > 5) v += __shfl_xor(v, 32, 64);
+  return v;
+}
+
+// dy[place[r, j]] = w[r, j] dout[r], dw[r, j] = <dout[r], y[place[r, j]]> in one pass over y and dout; rows of dy no entry owns: zeros.
+// Two entries at a time (1 / 2 / 4 / 8: 65536 rows of 8 x 128 bf16 68 / 76 / 72 / 77 us, fp32 155 / 127 / 128 / 129, 2 x 768 bf16
+// 104 / 113 / 131 / 191, 4096 rows of 4 x 384 fp32 13.3 / 12.3 / 12.3 / 13.6): more take registers and with them waves.
 template <typename T, int E, typename W>
 __global__ void __launch_bounds__(256) group_combine_grad_kernel(GroupRows g, const T* dout, long dout_stride, const T* y, long y_stride,
                                                                  const W* wt, T* dy, W* dw) {
-  using V = GroupVec<T, E>;
-  constexpr int J = 8;   // entries of a row taken together: their dot products are summed over the row's lanes at the end
+  constexpr int J = 2;
   const int lanes = 1 << g.lanes_log2;
   const int u0 = threadIdx.x & (lanes - 1);
   const long per = 256 >> g.lanes_log2;
   const long first = (long)blockIdx.x * per + (threadIdx.x >> g.lanes_log2), step = (long)gridDim.x * per;
-  const long row_elems = (long)g.units * E;
-  for (long r = first; r < g.n; r += step) {
-    const V* d = reinterpret_cast<const V*>(dout + r * dout_stride);
+  // (the loop over rows is taken by whole waves: the sums over a row's lanes want all of them active)
+  const long rounds = (g.n + step - 1) / step;
+  for (long i = 0; i < rounds; ++i) {
+    const long r = first + i * step;
     for (int j0 = 0; j0 < g.k; j0 += J) {
       int p[J];
       float w[J], dot[J];
 #pragma unroll
+      for (int j = 0; j < J; ++j) p[j] = r < g.n && j0 + j < g.k ? g.place[r * g.k + j0 + j] : -1;
+#pragma unroll
       for (int j = 0; j < J; ++j) {
-        p[j] = j0 + j < g.k ? g.place[r * g.k + j0 + j] : -1;
-        w[j] = p[j] >= 0 ? GroupNum<W>::get(wt[r * g.k + j0 + j]) : 0.f;
+        w[j] = dy && p[j] >= 0 ? GroupNum<W>::get(wt[r * g.k + j0 + j]) : 0.f;
         dot[j] = 0.f;
       }
-      for (int u = u0; u < g.units; u += lanes) {
-        const V dv = d[u];
+      if (r < g.n) {
+        for (int u = u0; u < g.units; u += lanes) {
+          const int at = min(u * E, g.D - E);
+          GroupUnit<T, E> d, v[J];
+          d.load(dout + r * dout_stride + at);
+          if (dw) {
 #pragma unroll
-        for (int j = 0; j < J; ++j) {
-          if (p[j] >= 0) {
-            const V v = reinterpret_cast<const V*>(y + (long)p[j] * y_stride)[u];
-            V o;
+            for (int j = 0; j < J; ++j)
+              if (p[j] >= 0) v[j].load(y + (long)p[j] * y_stride + at);
+          }
+          if (dy) {
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-              const float x = GroupNum<T>::get(dv.v[e]);
-              dot[j] = fmaf(x, GroupNum<T>::get(v.v[e]), dot[j]);
-              o.v[e] = GroupNum<T>::put(w[j] * x);
+            for (int j = 0; j < J; ++j) {
+              if (p[j] >= 0) {
+                GroupUnit<T, E> o;
+#pragma unroll
+                for (int e = 0; e < E; ++e) o.v[e] = GroupNum<T>::put(w[j] * GroupNum<T>::get(d.v[e]));
+                o.store(dy + (long)p[j] * g.D + at);
+              }
             }
-            if (dy) reinterpret_cast<V*>(dy + (long)p[j] * row_elems)[u] = o;
+          }
+          if (dw) {
+            float x[E];
+#pragma unroll
+            for (int e = 0; e < E; ++e) x[e] = at + e >= u * E ? GroupNum<T>::get(d.v[e]) : 0.f;   // (the overlap counts once)
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+              if (p[j] >= 0) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) dot[j] = fmaf(x[e], GroupNum<T>::get(v[j].v[e]), dot[j]);
+              }
+            }
           }
         }
       }
+      if (dw) {
 #pragma unroll
-      for (int j = 0; j < J; ++j) {
-        for (int m = lanes >> 1; m > 0; m >>= 1) dot[j] += __shfl_xor(dot[j], m, 64);
-        if (dw && u0 == 0 && j0 + j < g.k) dw[r * g.k + j0 + j] = GroupNum<W>::put(dot[j]);
+        for (int j = 0; j < J; ++j) {
+          const float s = group_lanes_sum(dot[j], g.lanes_log2);
+          if (u0 == 0 && r < g.n && j0 + j < g.k) dw[r * g.k + j0 + j] = GroupNum<W>::put(s);
+        }
       }
     }
   }
   if (!dy) return;
+  GroupUnit<T, E> zero;
+#pragma unroll
+  for (int e = 0; e < E; ++e) zero.v[e] = T{};
   for (long s = *g.end + first; s < g.N; s += step)
-    for (int u = u0; u < g.units; u += lanes) reinterpret_cast<V*>(dy + s * row_elems)[u] = V{};
+    for (int u = u0; u < g.units; u += lanes) zero.store(dy + s * g.D + min(u * E, g.D - E));
 }
 
 }  // namespace qinco

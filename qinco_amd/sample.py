@@ -43,10 +43,10 @@ def on_its_device(dev, call, *args) -> None:
     """One library call on the current stream of `dev` (its last argument), with `dev` current: kernels are launched on a stream of the
     current device."""
     if torch.cuda.current_device() == dev.index:
-        rc = call(*args, torch.cuda.current_stream().cuda_stream)
+        rc = call(*args, torch.cuda.current_stream(dev).cuda_stream)
     else:
         with torch.cuda.device(dev):
-            rc = call(*args, torch.cuda.current_stream().cuda_stream)
+            rc = call(*args, torch.cuda.current_stream(dev).cuda_stream)
     if rc:
         _lib.check(rc)
 
