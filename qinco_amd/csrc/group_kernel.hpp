@@ -454,6 +454,12 @@ struct GroupRows {
   int lanes_log2;
 };
 
+// slot of an entry, -1 without one (and for what cannot be a slot: nothing is read or written out of bounds whatever `place` holds)
+__device__ __forceinline__ int group_place(const GroupRows& g, long r, int j) {
+  const int p = g.place[r * g.k + j];
+  return (unsigned)p < (unsigned)g.N ? p : -1;
+}
+
 template <typename T, int E>
 struct GroupUnit {
   struct alignas(sizeof(T)) Raw { T v[E]; };
@@ -486,13 +492,13 @@ __global__ void __launch_bounds__(256) group_gather_kernel(GroupRows g, const T*
       v.load(x + r * x_stride + at);
       for (int j = 0; j < g.k; ++j) {
         const int p = pl[j];
-        if (p >= 0) v.store(out + (long)p * g.D + at);
+        if ((unsigned)p < (unsigned)g.N) v.store(out + (long)p * g.D + at);
       }
     }
   }
 #pragma unroll
   for (int e = 0; e < E; ++e) v.v[e] = T{};
-  for (long s = *g.end + first; s < g.N; s += step)
+  for (long s = max(*g.end, 0) + first; s < g.N; s += step)
     for (int u = u0; u < g.units; u += lanes) v.store(out + s * g.D + min(u * E, g.D - E));
 }
 
@@ -537,7 +543,7 @@ __global__ void __launch_bounds__(256) group_combine_kernel(GroupRows g, const T
         float w[J];
         GroupUnit<T, E> v[J];
 #pragma unroll
-        for (int j = 0; j < J; ++j) p[j] = j0 + j < g.k ? g.place[r * g.k + j0 + j] : -1;
+        for (int j = 0; j < J; ++j) p[j] = j0 + j < g.k ? group_place(g, r, j0 + j) : -1;
 #pragma unroll
         for (int j = 0; j < J; ++j) {
           if (p[j] >= 0) {
@@ -595,7 +601,7 @@ __global__ void __launch_bounds__(256) group_combine_grad_kernel(GroupRows g, co
       int p[J];
       float w[J], dot[J];
 #pragma unroll
-      for (int j = 0; j < J; ++j) p[j] = r < g.n && j0 + j < g.k ? g.place[r * g.k + j0 + j] : -1;
+      for (int j = 0; j < J; ++j) p[j] = r < g.n && j0 + j < g.k ? group_place(g, r, j0 + j) : -1;
 #pragma unroll
       for (int j = 0; j < J; ++j) {
         w[j] = dy && p[j] >= 0 ? GroupNum<W>::get(wt[r * g.k + j0 + j]) : 0.f;
@@ -649,7 +655,7 @@ __global__ void __launch_bounds__(256) group_combine_grad_kernel(GroupRows g, co
   GroupUnit<T, E> zero;
 #pragma unroll
   for (int e = 0; e < E; ++e) zero.v[e] = T{};
-  for (long s = *g.end + first; s < g.N; s += step)
+  for (long s = max(*g.end, 0) + first; s < g.N; s += step)
     for (int u = u0; u < g.units; u += lanes) zero.store(dy + s * g.D + min(u * E, g.D - E));
 }
 

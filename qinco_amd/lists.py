@@ -10,7 +10,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .sample import on_device, on_its_device, row_type, unit_rows
+from .sample import _TYPES, on_device, on_its_device, row_type, unit_rows
 
 MAX_LISTS = 1 << 24
 _IDS = {torch.int64: _lib.CODE_I64, torch.int32: _lib.CODE_I32, torch.uint8: _lib.CODE_U8}
@@ -54,7 +54,8 @@ class RowGroups:
     """Entries in list order (int32 CUDA tensors):
       order   (n k,)         entry row * k + slot in each place; -1 behind the last place in use
       place   (n, k)         place of each entry; -1 without a list
-      offsets (n_lists + 1,) first place of each list; the last value = places in use"""
+      offsets (n_lists + 1,) first place of each list; the last value = places in use
+    They are not to change while a backward pass may still use them."""
 
     def __init__(self, order, place, offsets):
         for t, what, dim in ((order, "order", 1), (place, "place", 2), (offsets, "offsets", 1)):
@@ -68,13 +69,15 @@ class RowGroups:
         self.order, self.place, self.offsets = order, place, offsets
         self.n, self.k = place.shape
         self.n_lists = offsets.numel() - 1
+        self._end = offsets.data_ptr() + 4 * self.n_lists   # address of the places in use
 
     def counts(self):
         """Entries of every list (n_lists,)."""
         return self.offsets.diff()
 
     def _rows(self, t, rows: int, what: str):
-        if on_device(t, what).dim() != 2 or t.shape[0] != rows or t.shape[1] < 1 or t.device != self.place.device:
+        shape = on_device(t, what).shape
+        if len(shape) != 2 or shape[0] != rows or shape[1] < 1 or t.device != self.place.device:
             raise ValueError(f"{what} must be ({rows}, D) with D >= 1 on {self.place.device}, got {tuple(t.shape)} on {t.device}")
         return unit_rows(t)
 
@@ -102,59 +105,67 @@ class RowGroups:
         return self._combine(y, weights)
 
     # -- the library calls; arguments are checked already
-    def _end(self):
-        return self.offsets.data_ptr() + 4 * self.n_lists
-
     def _gather(self, x):
-        out = torch.empty((self.n * self.k, x.shape[1]), dtype=x.dtype, device=x.device)
-        size = x.element_size()
-        on_its_device(x.device, _lib.load().qinco_group_gather, x.data_ptr(), x.stride(0) * size, x.shape[1] * size, self.place.data_ptr(),
-                      self._end(), self.n, self.k, out.data_ptr())
+        D, size, dev = x.shape[1], x.element_size(), x.device
+        out = torch.empty((self.n * self.k, D), dtype=x.dtype, device=dev)
+        on_its_device(dev, _lib.load().qinco_group_gather, x.data_ptr(), x.stride(0) * size, D * size, self.place.data_ptr(), self._end,
+                      self.n, self.k, out.data_ptr())
         return out
 
     def _combine(self, y, weights):
-        out = torch.empty((self.n, y.shape[1]), dtype=y.dtype, device=y.device)
-        on_its_device(y.device, _lib.load().qinco_group_combine, y.data_ptr(), row_type(y, "y"), y.stride(0), y.shape[1],
-                      weights.data_ptr() if weights is not None else None, row_type(weights, "weights") if weights is not None else 0,
-                      self.place.data_ptr(), self.n, self.k, out.data_ptr())
+        D, dev = y.shape[1], y.device
+        out = torch.empty((self.n, D), dtype=y.dtype, device=dev)
+        wt, w_type = (weights.data_ptr(), _TYPES[weights.dtype]) if weights is not None else (None, 0)
+        on_its_device(dev, _lib.load().qinco_group_combine, y.data_ptr(), _TYPES[y.dtype], y.stride(0), D, wt, w_type, self.place.data_ptr(),
+                      self.n, self.k, out.data_ptr())
         return out
 
     def _combine_grad(self, dout, y, weights, need_dy, need_dw):
-        dy = torch.empty(y.shape, dtype=y.dtype, device=y.device) if need_dy else None
-        dw = torch.empty(weights.shape, dtype=weights.dtype, device=y.device) if need_dw else None
-        on_its_device(y.device, _lib.load().qinco_group_combine_grad, dout.data_ptr(), dout.stride(0), y.data_ptr(), y.stride(0),
-                      row_type(y, "y"), y.shape[1], weights.data_ptr(), row_type(weights, "weights"), self.place.data_ptr(), self._end(),
-                      self.n, self.k, dy.data_ptr() if need_dy else None, dw.data_ptr() if need_dw else None)
+        D, dev = y.shape[1], y.device
+        dy = torch.empty((self.n * self.k, D), dtype=y.dtype, device=dev) if need_dy else None
+        dw = torch.empty((self.n, self.k), dtype=weights.dtype, device=dev) if need_dw else None
+        on_its_device(dev, _lib.load().qinco_group_combine_grad, dout.data_ptr(), dout.stride(0), y.data_ptr(), y.stride(0), _TYPES[y.dtype], D,
+                      weights.data_ptr(), _TYPES[weights.dtype], self.place.data_ptr(), self._end, self.n, self.k,
+                      dy.data_ptr() if need_dy else None, dw.data_ptr() if need_dw else None)
         return dy, dw
+
+
+def _gather_grad(ctx, dout):
+    return ctx.groups._combine(unit_rows(dout), None), None
+
+
+def _combine_grad(ctx, dout):
+    dout = unit_rows(dout)
+    if not ctx.weighted:
+        return ctx.groups._gather(dout), None, None
+    y, weights = ctx.saved_tensors
+    return (*ctx.groups._combine_grad(dout, y, weights, ctx.needs_input_grad[0], ctx.needs_input_grad[1]), None)
+
+
+# Second derivatives are refused.  once_differentiable() costs as much as the rest of a small backward call, and without create_graph (the
+# gradient mode is off then) there is nothing to refuse.
+_gather_grad_once, _combine_grad_once = once_differentiable(_gather_grad), once_differentiable(_combine_grad)
 
 
 class _Gather(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, groups):
         ctx.groups = groups
-        ctx.save_for_backward(groups.place, groups.offsets)   # (an in-place change between the passes is an error)
         return groups._gather(x)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
-        ctx.saved_tensors
-        return ctx.groups._combine(unit_rows(dout), None), None
+        return _gather_grad_once(ctx, dout) if torch.is_grad_enabled() else _gather_grad(ctx, dout)
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y, weights, groups):
         ctx.groups, ctx.weighted = groups, weights is not None
-        ctx.save_for_backward(groups.place, groups.offsets, *((y, weights) if ctx.weighted else ()))
+        if weights is not None:
+            ctx.save_for_backward(y, weights)
         return groups._combine(y, weights)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dout):
-        saved = ctx.saved_tensors
-        dout = unit_rows(dout)
-        if not ctx.weighted:
-            return ctx.groups._gather(dout), None, None
-        dy, dw = ctx.groups._combine_grad(dout, saved[2], saved[3], *ctx.needs_input_grad[:2])
-        return dy, dw, None
+        return _combine_grad_once(ctx, dout) if torch.is_grad_enabled() else _combine_grad(ctx, dout)

@@ -16,6 +16,8 @@ from . import _lib
 _CODES = {np.dtype(np.int64): _lib.CODE_I64, np.dtype(np.int32): _lib.CODE_I32}
 
 
+_RANDOM, _FLOAT, _INT = (torch.float32, torch.float64), (torch.float32,), (torch.int32,)
+_PARAMS_BYTES = C.sizeof(_lib.QincoSampleParams)
 _TYPES = {torch.float32: _lib.T_F32, torch.float16: _lib.T_F16, torch.bfloat16: _lib.T_BF16}
 
 
@@ -39,14 +41,20 @@ def unit_rows(t):
     return t if t.shape[1] == 1 or t.stride(1) == 1 else t.contiguous()
 
 
+_current_device = torch.cuda.current_device
+# the handle of a device's current stream without a Stream object around it (2 us of a call of 12), where this torch has it
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
 def on_its_device(dev, call, *args) -> None:
     """One library call on the current stream of `dev` (its last argument), with `dev` current: kernels are launched on a stream of the
     current device."""
-    if torch.cuda.current_device() == dev.index:
-        rc = call(*args, torch.cuda.current_stream(dev).cuda_stream)
+    index = dev.index
+    if _current_device() == index:
+        rc = call(*args, _raw_stream(index))
     else:
         with torch.cuda.device(dev):
-            rc = call(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = call(*args, _raw_stream(index))
     if rc:
         _lib.check(rc)
 
@@ -72,36 +80,47 @@ def sample_codes(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, c
     logits = unit_rows(logits)
     n, V = logits.shape
     dev = logits.device
-    if on_device(u, "u").shape != (n,) or u.dtype not in (torch.float32, torch.float64):
-        raise ValueError(f"u must be ({n},) float32 or float64, got {tuple(u.shape)} {u.dtype}")
-    u = u.contiguous()
-    keep = [u]
-    params = _lib.QincoSampleParams(struct_bytes=C.sizeof(_lib.QincoSampleParams))
-    for name, value, want in (("temperature", temperature, torch.float32), ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
-                              ("min_p", min_p, torch.float32)):
-        if isinstance(value, torch.Tensor):
-            if on_device(value, name).shape != (n,) or value.dtype != want:
-                raise ValueError(f"{name} must be a number or ({n},) {want}, got {tuple(value.shape)} {value.dtype}")
-            keep.append(value.contiguous())
-            setattr(params, name + "_rows", keep[-1].data_ptr())
-        elif want is torch.int32:
-            params.top_k = min(max(int(value), 0), V)
-        else:
-            setattr(params, name, float(value))
-    if any(t.device != dev for t in keep):
-        raise ValueError("logits, u and the settings must be on one device")
-    if not isinstance(temperature, torch.Tensor) and not 0.0 <= params.temperature < math.inf:
-        raise ValueError(f"temperature must be finite and >= 0, got {temperature}")
-    if params.top_p != params.top_p or params.min_p != params.min_p or params.min_p > 1.0:
-        raise ValueError(f"top_p must be a number and min_p at most 1, got {top_p} and {min_p}")
-    if np.dtype(code_dtype) not in _CODES:
+
+    def rows(t, what, types):
+        if on_device(t, what).shape != (n,) or t.dtype not in types or t.device != dev:
+            raise ValueError(f"{what} must be ({n},) of {' or '.join(map(str, types))} on {dev}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+        return t.contiguous()
+    u = rows(u, "u", _RANDOM)
+    params = _lib.QincoSampleParams(_PARAMS_BYTES)
+    keep = []                                          # (arrays made contiguous live until the call is enqueued)
+    if isinstance(temperature, torch.Tensor):
+        keep.append(rows(temperature, "temperature", _FLOAT))
+        params.temperature_rows = keep[-1].data_ptr()
+    else:
+        params.temperature = temperature = float(temperature)
+        if not 0.0 <= temperature < math.inf:
+            raise ValueError(f"temperature must be finite and >= 0, got {temperature}")
+    if isinstance(top_k, torch.Tensor):
+        keep.append(rows(top_k, "top_k", _INT))
+        params.top_k_rows = keep[-1].data_ptr()
+    else:
+        params.top_k = min(max(int(top_k), 0), V)
+    if isinstance(top_p, torch.Tensor):
+        keep.append(rows(top_p, "top_p", _FLOAT))
+        params.top_p_rows = keep[-1].data_ptr()
+    else:
+        params.top_p = top_p = float(top_p)
+        if top_p != top_p:
+            raise ValueError("top_p must be a number")
+    if isinstance(min_p, torch.Tensor):
+        keep.append(rows(min_p, "min_p", _FLOAT))
+        params.min_p_rows = keep[-1].data_ptr()
+    else:
+        params.min_p = min_p = float(min_p)
+        if not min_p <= 1.0:
+            raise ValueError(f"min_p must be at most 1, got {min_p}")
+    code = _CODES.get(np.dtype(code_dtype))
+    if code is None:
         raise ValueError("code_dtype must be int64 or int32 (a row with nothing to draw answers -1)")
-    code = _CODES[np.dtype(code_dtype)]
     codes = torch.empty(n, dtype=torch.int64 if code == _lib.CODE_I64 else torch.int32, device=dev)
     logp = torch.empty(n, dtype=torch.float32, device=dev) if return_logp else None
     need = lib.qinco_sample_workspace(n, V)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     on_its_device(dev, lib.qinco_sample_codes, logits.data_ptr(), dtype, logits.stride(0), n, V, u.data_ptr(), u.dtype == torch.float64,
-                  C.byref(params), codes.data_ptr(), code, logp.data_ptr() if return_logp else None,
-                  ws.data_ptr() if need else None, need)
+                  params, codes.data_ptr(), code, logp.data_ptr() if return_logp else None, ws.data_ptr() if need else None, need)
     return (codes, logp) if return_logp else codes
