@@ -32,17 +32,19 @@ static constexpr int64_t kSampleLongV = kSampleBlockV;
 namespace {
 struct SamplePlan {
   int64_t rows, chunks;                                                          // rows of a batch
-  int64_t best, least, floor, mass, count, row_mass, row_count, state, chunk_mass, m_z, m_idx, bytes;   // byte offsets
+  int64_t most;                                                                  // members that a row's list holds
+  int64_t best, least, floor, mass, count, row_mass, row_count, state, chunk_mass, m_z, m_where, bytes;   // byte offsets
 };
 }  // namespace
 
-// Rows go through in batches whose chunks' bins stay within 64 MiB (they are written by one kernel and read by the next: within the
-// 256 MiB cache), one row at least.
+// Rows go through in batches whose workspace stays within 128 MiB (what one kernel writes the next finds in the 256 MiB cache), one row at
+// least.  A row's list holds an eighth of it: bins that the cuts fall into hold more only where that many logits are next to each other.
 static SamplePlan sample_plan(int64_t n, int64_t V) {
   SamplePlan p{};
   if (V <= kSampleLongV) return p;
   p.chunks = (V + kSampleChunk - 1) / kSampleChunk;
-  p.rows = ((int64_t)64 << 20) / (p.chunks * kSampleBins * 12);
+  p.most = V / 8 > 2 * kSampleMembers ? V / 8 : 2 * kSampleMembers;
+  p.rows = ((int64_t)128 << 20) / (p.chunks * kSampleBins * 12 + kSampleBins * 12 + p.most * 8);
   if (p.rows < 1) p.rows = 1;
   if (p.rows > n) p.rows = n;
   int64_t at = 0;
@@ -60,8 +62,8 @@ static SamplePlan sample_plan(int64_t n, int64_t V) {
   take(p.row_count, R * kSampleBins * 4);
   take(p.state, R * (int64_t)sizeof(SampleState));
   take(p.chunk_mass, RC * 8);
-  take(p.m_z, R * kSampleMembers * 4);
-  take(p.m_idx, R * kSampleMembers * 4);
+  take(p.m_z, R * p.most * 4);
+  take(p.m_where, R * p.most * 4);
   p.bytes = at;
   return p;
 }
@@ -85,7 +87,8 @@ static int launch_sample_long(const SampleArgs& a, const SamplePlan& p, char* ws
   l.state = reinterpret_cast<SampleState*>(ws + p.state);
   l.chunk_mass = reinterpret_cast<unsigned long long*>(ws + p.chunk_mass);
   l.m_z = reinterpret_cast<float*>(ws + p.m_z);
-  l.m_idx = reinterpret_cast<unsigned*>(ws + p.m_idx);
+  l.m_where = reinterpret_cast<unsigned*>(ws + p.m_where);
+  l.most = (int)p.most;
   for (long r0 = 0; r0 < a.n; r0 += p.rows) {
     const long rows = a.n - r0 < p.rows ? a.n - r0 : (long)p.rows;
     l.row0 = r0;

@@ -886,17 +886,33 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
 
 // ---------------------------------------------------------------------------------------------------------------------
 // The longest rows, a workgroup per chunk of 16384 codes: (1) largest and smallest logit of every chunk, (2) its bins, (3) the bins summed
-// over the chunks and the cuts' bins found, (4) the codes of those bins ("members") listed, and the mass of what every chunk keeps whole,
-// (5) one workgroup per row: the cuts among the members, the chunk that the draw falls into, and the code in it.  Three passes over the
-// logits, of which the cache serves the later two; nobody waits for another workgroup inside a kernel.
+// over the chunks, (4) the cuts' bins found, (5) the codes of those bins ("members") listed, equal ones of a chunk as one where they are
+// many, and the mass of what every chunk keeps whole, (6) one workgroup per row: the cuts among the members, the chunk that the draw falls
+// into, and the code in it.  Three passes over the logits, of which the cache serves the later two; nobody waits for another workgroup
+// inside a kernel.
 //
 // Where both cuts are on, what top-k keeps of its bin is not known before its members are looked at; the mass that top-p cuts at is then
 // known only to within that bin's mass, and the members of all bins it can fall into are taken.
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kSampleChunkThreads = 1024, kSampleChunkIpt = 16, kSampleChunk = kSampleChunkThreads * kSampleChunkIpt;
 constexpr int kSampleMaxChunks = 1024;          // V <= 2^24
-constexpr int kSampleMembers = 2048;            // of a row; with more (heavy ties) the last kernel searches the whole row
-constexpr unsigned kSampleFloored = 1u << 31;   // flag beside a member's index (< 2^24): cut by min-p
+constexpr int kSampleHere = 2048;               // members of a chunk listed one by one; with more, equal ones as one
+constexpr int kSampleMembers = 4096;            // members of a row that the last kernel holds in LDS
+
+// Bins of such a row: 128 to a power of two of 1 + s (max z - z), eight powers down to where nothing has mass (54 / y) or the smallest
+// logit.  Next to the largest logit they are 30 times as fine as linear ones (logits that hardly differ, beside masks of the type's lowest
+// value, would all lie in one of those), where a cut of ordinary logits falls twice as coarse.  Sum, product and the bits of a positive fp32 are monotone; a NaN goes to the last bin.
+struct SampleLogBins {
+  float zmax, s;
+  __device__ __forceinline__ int of(float z) const {
+    const unsigned bits = __float_as_uint(fmaf(zmax - z, s, 1.f)) - 0x3F800000u;
+    return (int)min(bits >> 16, (unsigned)kSampleBins - 1);
+  }
+};
+__device__ __forceinline__ SampleLogBins sample_log_bins(float zmax, float zmin, double y) {
+  const float d = fminf(zmax - zmin, (float)fmin(54.0 / y, 3e38));
+  return SampleLogBins{zmax, d > 0.f && zmax < INFINITY ? fminf(255.f / d, 3e38f) : 0.f};
+}
 
 struct SampleState {                   // of a row
   float zmax, zmin;
@@ -914,6 +930,7 @@ struct SampleState {                   // of a row
 struct SampleLong {
   long row0;                           // first row of the batch
   int chunks;
+  int most;                            // members that a row's list holds (with more the last kernel searches the row itself)
   unsigned long long* best;            // [row][chunk] key of the largest logit << 32 | ~lowest index that holds it
   unsigned* least;                     // [row][chunk] ~key of the smallest logit that is not -inf
   int* floor;                          // [row][chunk] first bin with a code that min-p cuts
@@ -923,8 +940,8 @@ struct SampleLong {
   unsigned* row_count;
   SampleState* state;                  // [row]
   unsigned long long* chunk_mass;      // [row][chunk] of codes kept whole
-  float* m_z;                          // [row][kSampleMembers]
-  unsigned* m_idx;                     // index, kSampleFloored
+  float* m_z;                          // [row][most] logit
+  unsigned* m_where;                   // its chunk << 15 | how many (1 .. 16384)
 };
 
 template <typename T>
@@ -1025,7 +1042,7 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_bins_kernel(Sample
   const SampleRange g = sample_range(l, r, sh);   // (its barrier: the bins are cleared)
   if (g.zmax == -INFINITY || set.greedy) return;
   const SampleMass mass(g.zmax, set.y, a.F);
-  const SampleBins bins = sample_bins(g.zmax, g.zmin, set.y, kSampleBins);
+  const SampleLogBins bins = sample_log_bins(g.zmax, g.zmin, set.y);
   const bool by_count = set.k < a.V, by_floor = set.m > 0.0;
   int first = kSampleBins;
 #pragma unroll
@@ -1128,16 +1145,19 @@ __global__ void __launch_bounds__(1024) sample_cuts_kernel(SampleArgs a, SampleL
 
 template <typename T>
 __global__ void __launch_bounds__(kSampleChunkThreads) sample_members_kernel(SampleArgs a, SampleLong l) {
-  constexpr int NT = kSampleChunkThreads;
+  constexpr int NT = kSampleChunkThreads, LOOKS = 16;
+  constexpr unsigned EMPTY = kSampleKeyMasked;                // (-inf is no member)
   __shared__ SampleBlock<NT> blk;
-  __shared__ float m_z[kSampleMembers];
-  __shared__ unsigned m_idx[kSampleMembers];
+  __shared__ unsigned m_key[kSampleHere], m_count[kSampleHere];
   __shared__ int n_here, first_here;
   const long r = blockIdx.x / l.chunks;
-  const int c = blockIdx.x - (int)(r * l.chunks), i0 = c * kSampleChunk, tid = threadIdx.x;
+  const int c = blockIdx.x - (int)(r * l.chunks), i0 = c * kSampleChunk, tid = threadIdx.x, lane = tid & 63;
   const SampleRow set = sample_row(a, l.row0 + r);
   const SampleState st = l.state[r];
   if (st.zmax == -INFINITY || set.greedy) return;
+  const bool any = st.b0 < kSampleBins || st.fb < kSampleBins;
+  float z[kSampleChunkIpt];
+  if (any) sample_load_chunk(a, reinterpret_cast<const T*>(a.logits) + (l.row0 + r) * a.stride, i0, z);
   if (tid == 0) n_here = 0;
   // what the chunk keeps whole: its bins before the cuts
   const unsigned long long m = tid < min(st.b0, st.fb) ? l.mass[((size_t)r * l.chunks + c) * kSampleBins + tid] : 0ull;
@@ -1145,33 +1165,91 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_members_kernel(Sam
   unsigned none, none_all;
   sample_block_scan<NT>(blk, m, 0u, before, none, all, none_all);
   if (tid == 0) l.chunk_mass[r * l.chunks + c] = all;
-  if (st.b0 == kSampleBins && st.fb == kSampleBins) return;
-  float z[kSampleChunkIpt];
-  sample_load_chunk(a, reinterpret_cast<const T*>(a.logits) + (l.row0 + r) * a.stride, i0, z);
-  const SampleBins bins = sample_bins(st.zmax, st.zmin, set.y, kSampleBins);
+  if (!any) return;
+  const SampleLogBins bins = sample_log_bins(st.zmax, st.zmin, set.y);
+  unsigned is = 0;   // bit j: z[j] is a member
 #pragma unroll
-  for (int j = 0; j < kSampleChunkIpt; ++j) {
-    if (z[j] > -INFINITY && st.member(bins.of(z[j]))) {
-      const int to = atomicAdd(&n_here, 1);
-      if (to < kSampleMembers) {
-        m_z[to] = z[j];
-        m_idx[to] = (unsigned)(i0 + j * NT + tid);
-      }
-    }
-  }
+  for (int j = 0; j < kSampleChunkIpt; ++j) is |= (unsigned)(z[j] > -INFINITY && st.member(bins.of(z[j]))) << j;
+  if (is) atomicAdd(&n_here, __builtin_popcount(is));
   __syncthreads();
   const int n = n_here;
   if (n == 0) return;
-  if (tid == 0) first_here = atomicAdd(&l.state[r].n_members, n);
+  float* const out_z = l.m_z + r * l.most;
+  unsigned* const out_where = l.m_where + r * l.most;
+  const unsigned chunk = (unsigned)c << 15;
+  auto put = [&](int to, float x, unsigned count) {
+    if (to < l.most) {
+      out_z[to] = x;
+      out_where[to] = chunk | count;
+    }
+  };
   __syncthreads();
-  const SampleMass mass(st.zmax, set.y, a.F);
-  for (int i = tid; i < min(n, kSampleMembers); i += NT) {
-    const int to = first_here + i;
-    if (to < kSampleMembers) {
-      l.m_z[r * kSampleMembers + to] = m_z[i];
-      l.m_idx[r * kSampleMembers + to] = m_idx[i] | (mass.e(m_z[i]) >= set.m ? 0u : kSampleFloored);
+  if (n <= kSampleHere) {
+    if (tid == 0) {
+      first_here = atomicAdd(&l.state[r].n_members, n);
+      n_here = 0;
+    }
+    __syncthreads();
+    if (is) {
+      int to = first_here + atomicAdd(&n_here, __builtin_popcount(is));
+#pragma unroll
+      for (int j = 0; j < kSampleChunkIpt; ++j)
+        if (is >> j & 1) put(to++, z[j], 1);
+    }
+    return;
+  }
+  // many: counted by key in a table of the workgroup; what finds no room there goes into the list as it is
+  for (int i = tid; i < kSampleHere; i += NT) {
+    m_key[i] = EMPTY;
+    m_count[i] = 0;
+  }
+  if (tid == 0) n_here = 0;
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < kSampleChunkIpt; ++j) {
+    unsigned long long todo = __ballot(is >> j & 1);
+    const unsigned key = sample_key(z[j]);
+    for (int look = 0; todo && look < 2; ++look) {   // (keys that several lanes hold go in as one)
+      const int lead = __builtin_ctzll(todo);
+      const unsigned long long same = todo & __ballot((is >> j & 1) && key == sample_lane(key, lead));
+      if (__builtin_popcountll(same) == 1 && look) break;
+      bool in = false;
+      if (lane == lead) {
+        const unsigned h = (key * 2654435761u) >> 21;
+        for (int i = 0; i < LOOKS && !in; ++i) {
+          const unsigned at = (h + i) & (kSampleHere - 1), old = atomicCAS(&m_key[at], EMPTY, key);
+          if (old == EMPTY || old == key) {
+            atomicAdd(&m_count[at], (unsigned)__builtin_popcountll(same));
+            in = true;
+          }
+        }
+        if (!in) put(atomicAdd(&l.state[r].n_members, 1), z[j], (unsigned)__builtin_popcountll(same));
+      }
+      todo &= ~same;
+    }
+    if (todo >> lane & 1) {
+      bool in = false;
+      const unsigned h = (key * 2654435761u) >> 21;
+      for (int i = 0; i < LOOKS && !in; ++i) {
+        const unsigned at = (h + i) & (kSampleHere - 1), old = atomicCAS(&m_key[at], EMPTY, key);
+        if (old == EMPTY || old == key) {
+          atomicAdd(&m_count[at], 1u);
+          in = true;
+        }
+      }
+      if (!in) put(atomicAdd(&l.state[r].n_members, 1), z[j], 1);
     }
   }
+  __syncthreads();
+  int mine = 0;
+  for (int i = tid; i < kSampleHere; i += NT) mine += m_count[i] > 0;
+  int to = mine ? atomicAdd(&n_here, mine) : 0;
+  __syncthreads();
+  if (tid == 0 && n_here) first_here = atomicAdd(&l.state[r].n_members, n_here);
+  __syncthreads();
+  to += first_here;
+  for (int i = tid; i < kSampleHere; i += NT)
+    if (m_count[i] > 0) put(to++, sample_unkey(m_key[i]), m_count[i]);
 }
 
 template <typename T>
@@ -1180,9 +1258,8 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
   __shared__ SampleBlock<NT> blk;
   __shared__ SampleFound found;
   __shared__ unsigned long long part[kSampleBins];
-  __shared__ unsigned long long m_mass[kSampleMembers];
   __shared__ float m_z[kSampleMembers];
-  __shared__ unsigned m_idx[kSampleMembers];
+  __shared__ unsigned m_where[kSampleMembers];
   __shared__ unsigned long long chunk[kSampleMaxChunks];
   __shared__ unsigned chunk_ties[kSampleMaxChunks];
   __shared__ unsigned key_range[2];
@@ -1201,71 +1278,67 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
     return;
   }
   const SampleMass mass(st.zmax, set.y, a.F);
-  const SampleBins bins = sample_bins(st.zmax, st.zmin, set.y, kSampleBins);
+  const SampleLogBins bins = sample_log_bins(st.zmax, st.zmin, set.y);
   const T* logits = reinterpret_cast<const T*>(a.logits) + row * a.stride;
-  const int n = st.n_members;
-  const bool listed = n <= kSampleMembers;
+  const bool listed = st.n_members <= l.most, held = st.n_members <= kSampleMembers;   // (else the row itself is the list)
+  const int n = listed ? st.n_members : a.V;
   chunk[tid] = listed && tid < l.chunks ? l.chunk_mass[r * l.chunks + tid] : 0ull;
   chunk_ties[tid] = 0;
-  if (listed)
-    for (int i = tid; i < n; i += NT) {
-      m_z[i] = l.m_z[r * kSampleMembers + i];
-      m_idx[i] = l.m_idx[r * kSampleMembers + i];
-      m_mass[i] = mass.q(m_z[i]);
-    }
+  if (tid == 0) {
+    key_range[0] = ~0u;
+    key_range[1] = 0;
+  }
   __syncthreads();
-  // every member, or with too many of them every code: f(z, its mass when asked for)
+  // f(logit, how many, chunk) for every member
   auto each = [&](auto f) {
-    if (listed) {
-      for (int i = tid; i < n; i += NT) f(m_z[i], [&] { return m_mass[i]; });
+    if (held) {
+      for (int i = tid; i < n; i += NT) f(m_z[i], m_where[i] & 0x7FFFu, m_where[i] >> 15);
     } else {
 #pragma unroll 1
-      for (int i = tid; i < a.V; i += NT) {
-        const float z = sample_logit(logits, i, a.V);
-        if (z > -INFINITY) f(z, [&] { return mass.q(z); });
+      for (int i = tid; i < n; i += NT) {
+        const float z = listed ? l.m_z[r * l.most + i] : sample_logit(logits, i, a.V);
+        const unsigned at = listed ? l.m_where[r * l.most + i] : (unsigned)(i / kSampleChunk) << 15 | 1u;
+        if (z > -INFINITY) f(z, at & 0x7FFFu, at >> 15);
       }
     }
   };
+  // the members' keys: fewer bits to search
+  unsigned lo = 0, hi = 0;   // lo: complemented
+  if (held) {
+    for (int i = tid; i < n; i += NT) {
+      m_z[i] = l.m_z[r * l.most + i];
+      m_where[i] = l.m_where[r * l.most + i];
+    }
+  }
+  each([&](float z, unsigned, unsigned) {   // (a thread reads what it wrote)
+    lo = max(lo, ~sample_key(z));
+    hi = max(hi, sample_key(z));
+  });
+  lo = sample_wave_max(lo);
+  hi = sample_wave_max(hi);
+  if (lane == 0 && hi) {
+    atomicMin(&key_range[0], ~lo);
+    atomicMax(&key_range[1], hi);
+  }
+  __syncthreads();
+  const unsigned kmin = key_range[0], kmax = key_range[1];
   float t = -INFINITY;
   unsigned ties = 0;   // codes kept of those at t
-  unsigned long long qt = 0, before, all;
+  unsigned long long qt = 0, before, all = 0;
   unsigned none, none_all;
-  // the members' keys: fewer bits to search
-  unsigned kmin = sample_key(st.zmin), kmax = sample_key(st.zmax);
-  if (listed) {
-    if (tid == 0) {
-      key_range[0] = ~0u;
-      key_range[1] = 0;
-    }
-    __syncthreads();
-    unsigned lo = 0, hi = 0;   // lo: complemented
-    for (int i = tid; i < n; i += NT) {
-      lo = max(lo, ~sample_key(m_z[i]));
-      hi = max(hi, sample_key(m_z[i]));
-    }
-    lo = sample_wave_max(lo);
-    hi = sample_wave_max(hi);
-    if (lane == 0 && hi) {
-      atomicMin(&key_range[0], ~lo);
-      atomicMax(&key_range[1], hi);
-    }
-    __syncthreads();
-    kmin = key_range[0];
-    kmax = key_range[1];
-  }
   unsigned long long total = 0;
   if (st.kb < kSampleBins) {
     const unsigned key = sample_search<NT>(blk, found, part, kmin, kmax, st.want, before, [&](auto f) {
-      each([&](float z, auto) {
-        if (bins.of(z) == st.kb) f(sample_key(z), [] { return 1ull; });
+      each([&](float z, unsigned c, unsigned) {
+        if (bins.of(z) == st.kb) f(sample_key(z), [&] { return (unsigned long long)c; });
       });
     });
     t = sample_unkey(key);
     ties = st.want - (unsigned)before;
     qt = mass.q(t);
     unsigned long long in = 0;
-    each([&](float z, auto q) {
-      if (z > t && bins.of(z) == st.kb) in += q();
+    each([&](float z, unsigned c, unsigned) {
+      if (z > t && bins.of(z) == st.kb) in += c * mass.q(z);
     });
     sample_block_scan<NT>(blk, in, 0u, before, none, all, none_all);
     total = st.above + all + ties * qt;
@@ -1277,8 +1350,8 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
       ties = min(ties, sample_ceil_div(bound - st.above - all, qt));
     } else {
       const unsigned key = sample_search<NT>(blk, found, part, kmin, kmax, bound - st.base, before, [&](auto f) {
-        each([&](float z, auto q) {
-          if (z > t && bins.of(z) >= st.b0) f(sample_key(z), q);
+        each([&](float z, unsigned c, unsigned) {
+          if (z > t && bins.of(z) >= st.b0) f(sample_key(z), [&] { return c * mass.q(z); });
         });
       });
       t = sample_unkey(key);
@@ -1287,27 +1360,13 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
   }
   qt = ties ? mass.q(t, set.m) : 0ull;
   // kept members into their chunks, and the ties at t
-  if (listed) {
-    for (int i = tid; i < n; i += NT) {
-      const unsigned c = (m_idx[i] & ~kSampleFloored) / kSampleChunk;
-      if (m_z[i] > t && !(m_idx[i] & kSampleFloored)) atomicAdd(&chunk[c], m_mass[i]);
-      if (m_z[i] == t && ties) atomicAdd(&chunk_ties[c], 1u);
+  each([&](float z, unsigned c, unsigned at) {
+    if (z > t) {
+      const unsigned long long q = mass.q(z, set.m);
+      if (q) atomicAdd(&chunk[at], c * q);
     }
-  } else {
-#pragma unroll 1
-    for (int c = 0; c < l.chunks; ++c) {
-      unsigned long long sum = 0;
-      unsigned at = 0;
-#pragma unroll 1
-      for (int j = 0; j < kSampleChunkIpt; ++j) {
-        const float z = sample_logit(logits, c * kSampleChunk + j * NT + tid, a.V);
-        sum += z > t ? mass.q(z, set.m) : 0ull;
-        at += z == t && ties > 0;
-      }
-      if (sum) atomicAdd(&chunk[c], sum);
-      if (at) atomicAdd(&chunk_ties[c], at);
-    }
-  }
+    if (z == t && ties) atomicAdd(&chunk_ties[at], c);
+  });
   __syncthreads();
   unsigned tied, tied_all;
   const unsigned at_chunk = chunk_ties[tid];
