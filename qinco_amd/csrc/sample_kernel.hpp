@@ -924,7 +924,7 @@ struct SampleState {                   // of a row
   int n_members;
   unsigned long long above, base;      // mass before kb, and before b0
   unsigned long long bound;            // the mass that top-p cuts at, where top-k cuts nothing
-  __device__ __forceinline__ bool member(int b) const { return (b >= b0 && b <= b1) || b == kb || (b == fb && fb < b0); }
+  float lo[3], hi[3];                  // logits of bins b0 .. b1, of kb, and of fb if it is before b0 (lo > hi: none)
 };
 
 struct SampleLong {
@@ -1140,6 +1140,22 @@ __global__ void __launch_bounds__(1024) sample_cuts_kernel(SampleArgs a, SampleL
     }
   }
   __syncthreads();
+  if (tid < 6) {   // the ends of the members' logits: the bins are monotone, so each is found bit by bit over the keys
+    const SampleLogBins bins = sample_log_bins(g.zmax, g.zmin, set.y);
+    const int which = tid >> 1;
+    const int x = which == 0 ? st.b0 : which == 1 ? st.kb : st.fb, y = which == 0 ? st.b1 : x;
+    unsigned key = 0;   // tid even: the largest key whose bin is behind y (lo is the one above it); odd: the largest whose bin is x or behind it
+    for (int b = 31; b >= 0; --b) {
+      const unsigned c = key | 1u << b;
+      const float z = sample_unkey(c);
+      const bool behind = c <= kSampleKeyMasked || (z <= g.zmax && bins.of(z) >= (tid & 1 ? x : y + 1));
+      if (behind) key = c;
+    }
+    const bool none = x >= kSampleBins || (which == 2 && st.fb >= st.b0);
+    if (tid & 1) st.hi[which] = none ? -INFINITY : sample_unkey(key);
+    else st.lo[which] = none ? INFINITY : sample_unkey(max(key, kSampleKeyMasked) + 1);
+  }
+  __syncthreads();
   if (tid == 0) l.state[r] = st;
 }
 
@@ -1157,22 +1173,30 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_members_kernel(Sam
   if (st.zmax == -INFINITY || set.greedy) return;
   const bool any = st.b0 < kSampleBins || st.fb < kSampleBins;
   float z[kSampleChunkIpt];
-  if (any) sample_load_chunk(a, reinterpret_cast<const T*>(a.logits) + (l.row0 + r) * a.stride, i0, z);
-  if (tid == 0) n_here = 0;
+  unsigned is = 0;   // bit j: z[j] is a member
+  if (any) {
+    sample_load_chunk(a, reinterpret_cast<const T*>(a.logits) + (l.row0 + r) * a.stride, i0, z);
+#pragma unroll
+    for (int j = 0; j < kSampleChunkIpt; ++j) is |= (unsigned)(z[j] >= st.lo[0] && z[j] <= st.hi[0]) << j;
+    if ((st.kb < st.b0 || st.kb > st.b1) && st.kb < kSampleBins) {
+#pragma unroll
+      for (int j = 0; j < kSampleChunkIpt; ++j) is |= (unsigned)(z[j] >= st.lo[1] && z[j] <= st.hi[1]) << j;
+    }
+    if (st.fb < st.b0) {
+#pragma unroll
+      for (int j = 0; j < kSampleChunkIpt; ++j) is |= (unsigned)(z[j] >= st.lo[2] && z[j] <= st.hi[2]) << j;
+    }
+  }
   // what the chunk keeps whole: its bins before the cuts
   const unsigned long long m = tid < min(st.b0, st.fb) ? l.mass[((size_t)r * l.chunks + c) * kSampleBins + tid] : 0ull;
   unsigned long long before, all;
-  unsigned none, none_all;
-  sample_block_scan<NT>(blk, m, 0u, before, none, all, none_all);
-  if (tid == 0) l.chunk_mass[r * l.chunks + c] = all;
-  if (!any) return;
-  const SampleLogBins bins = sample_log_bins(st.zmax, st.zmin, set.y);
-  unsigned is = 0;   // bit j: z[j] is a member
-#pragma unroll
-  for (int j = 0; j < kSampleChunkIpt; ++j) is |= (unsigned)(z[j] > -INFINITY && st.member(bins.of(z[j]))) << j;
-  if (is) atomicAdd(&n_here, __builtin_popcount(is));
-  __syncthreads();
-  const int n = n_here;
+  unsigned c_before, n;
+  sample_block_scan<NT>(blk, m, (unsigned)__builtin_popcount(is), before, c_before, all, n);
+  if (tid == 0) {
+    l.chunk_mass[r * l.chunks + c] = all;
+    if (n > 0 && n <= kSampleHere) first_here = atomicAdd(&l.state[r].n_members, (int)n);
+    n_here = 0;
+  }
   if (n == 0) return;
   float* const out_z = l.m_z + r * l.most;
   unsigned* const out_where = l.m_where + r * l.most;
@@ -1185,13 +1209,8 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_members_kernel(Sam
   };
   __syncthreads();
   if (n <= kSampleHere) {
-    if (tid == 0) {
-      first_here = atomicAdd(&l.state[r].n_members, n);
-      n_here = 0;
-    }
-    __syncthreads();
     if (is) {
-      int to = first_here + atomicAdd(&n_here, __builtin_popcount(is));
+      int to = first_here + (int)c_before;
 #pragma unroll
       for (int j = 0; j < kSampleChunkIpt; ++j)
         if (is >> j & 1) put(to++, z[j], 1);
@@ -1203,7 +1222,6 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_members_kernel(Sam
     m_key[i] = EMPTY;
     m_count[i] = 0;
   }
-  if (tid == 0) n_here = 0;
   __syncthreads();
 #pragma unroll
   for (int j = 0; j < kSampleChunkIpt; ++j) {
@@ -1380,18 +1398,46 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
     sh_tied = tied;
   }
   __syncthreads();
-  // ... and in that chunk: wave w owns codes [i0 + 1024 w, + 1024)
+  // ... and in that chunk: wave w owns codes [i0 + 1024 w, + 1024).  What is kept of it is listed first (the members are done with): an
+  // exponential for every step in which one of 64 codes is kept would take longer
   const int i0 = sh_chunk * kSampleChunk, w0 = i0 + w * 64 * kSampleChunkIpt;
-  unsigned long long sum = 0;
-  unsigned at_t = 0;
-#pragma unroll 4
+  float z[kSampleChunkIpt];
+  unsigned at_t = 0, is = 0;
+#pragma unroll
+  for (int j = 0; j < kSampleChunkIpt; ++j) z[j] = sample_logit(logits, w0 + j * 64 + lane, a.V);
+#pragma unroll
   for (int j = 0; j < kSampleChunkIpt; ++j) {
-    const float z = sample_logit(logits, w0 + j * 64 + lane, a.V);
-    sum += z > t ? mass.q(z, set.m) : 0ull;
-    at_t += z == t && ties > 0;
+    is |= (unsigned)(z[j] > t) << j;
+    at_t += z[j] == t && ties > 0;
   }
-  sum = sample_wave_sum(sum);
+  unsigned first, kept;
+  sample_block_scan<NT>(blk, 0ull, (unsigned)__builtin_popcount(is), before, first, all, kept);
   at_t = sample_wave_sum(at_t);
+  unsigned long long sum = 0;
+  if (kept <= kSampleMembers) {
+    if (tid < NT / 64) part[tid] = 0;
+#pragma unroll
+    for (int j = 0; j < kSampleChunkIpt; ++j) {
+      if (is >> j & 1) {
+        m_z[first] = z[j];
+        m_where[first++] = (unsigned)w;
+      }
+    }
+    __syncthreads();
+    for (unsigned i = tid; i < kept; i += NT) {
+      const unsigned long long q = mass.q(m_z[i], set.m);
+      if (q) atomicAdd(&part[m_where[i]], q);
+    }
+    __syncthreads();
+    sum = part[w];
+  } else {
+#pragma unroll
+    for (int j = 0; j < kSampleChunkIpt; ++j) {
+      sum += is >> j & 1 ? mass.q(z[j], set.m) : 0ull;
+      if (j & 1) __builtin_amdgcn_sched_barrier(0);
+    }
+    sum = sample_wave_sum(sum);
+  }
   if (lane == 0) {
     blk.m[w] = sum;
     blk.c[w] = at_t;
