@@ -1305,6 +1305,9 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
   if (tid == 0) {
     key_range[0] = ~0u;
     key_range[1] = 0;
+    sh_chunk = 0;   // (logits that change during the call: some chunk of the row all the same)
+    sh_before = 0;
+    sh_tied = 0;
   }
   __syncthreads();
   // f(logit, how many, chunk) for every member

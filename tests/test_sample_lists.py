@@ -222,6 +222,42 @@ def test_sample_borders_fall_on_the_exact_side():
     assert np.all(np.abs(got - n * e / e.sum()) <= 1.0)
 
 
+def hard_rows(V, g):
+    """Rows whose cuts fall among many codes: few values, values that hardly differ, far outliers, long tails."""
+    import torch
+    rand = lambda: torch.rand(V, generator=g, device="cuda")               # noqa: E731
+    low = torch.finfo(torch.float32).min
+    near, small = 1.0 + rand() * 1e-3, rand() * 1e-4
+    masked = near.clone()
+    masked[rand() < 0.5] = low
+    apart = small.clone()
+    apart[V // 3] = -50.0                                                  # all the others in one bin, all different
+    steps = (rand() * 4).floor()
+    clusters = torch.where(rand() < 0.5, rand() * 1e-5, 5.0 + rand() * 1e-5)
+    return torch.stack([torch.zeros(V, device="cuda"), steps, near, masked, apart, clusters, -torch.exp(rand() * 30 - 15), rand().log(),
+                        torch.full((V,), low, device="cuda"), (rand() * 1e6).floor() * 1e-3])
+
+
+@gpu
+@pytest.mark.parametrize("V", [200, 1024, 3000, 10240, 70001, 300001])
+def test_sample_rows_that_pile_up_in_a_few_bins(V):
+    import torch
+    g = torch.Generator("cuda").manual_seed(V)
+    z = hard_rows(V, g)
+    for s in (dict(p=0.5), dict(k=V // 3), dict(k=V // 2, p=0.7), dict(k=V // 2, p=0.7, m=0.999, T=0.3), dict(m=0.9995), dict(T=100.0, p=0.3), dict(T=1e-3, p=0.99)):
+        check_sample(z, torch.rand(len(z), generator=g, device="cuda", dtype=torch.float64), **s)
+
+
+@gpu
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_sample_long_rows_of_few_values(dtype):
+    import torch
+    g = torch.Generator("cuda").manual_seed(1)
+    z = (torch.randn(3, 1 << 20, generator=g, device="cuda") * 2.5).to(getattr(torch, dtype))
+    for s in (dict(p=0.9), dict(k=20000, p=0.5, m=1e-4), dict(T=3.0, p=0.99)):
+        check_sample(z, torch.rand(3, generator=g, device="cuda"), **s)
+
+
 @gpu
 def test_sample_settings_per_row_strides_and_types():
     import torch
@@ -437,6 +473,65 @@ def test_rows_of_any_type_stride_and_broadcast_gradients():
                  lambda: gr.combine(y.double()), lambda: gr.combine(y, w[:-1]), lambda: gr.combine(y, w.half()), lambda: gr.combine(y, w.cpu())):
         with pytest.raises(ValueError):
             call()
+
+
+@gpu
+def test_second_derivatives_are_refused_and_first_ones_with_their_graph_are_not():
+    import torch
+    g = torch.Generator("cuda").manual_seed(5)
+    gr = make_groups(g, 20, 2, 5, False)
+    x, y = torch.randn(20, 8, device="cuda", requires_grad=True), torch.randn(40, 8, device="cuda", requires_grad=True)
+    w = torch.rand(20, 2, device="cuda", requires_grad=True)
+    for out, leaves in ((gr.gather(x), (x,)), (gr.combine(y, w), (y, w)), (gr.combine(y), (y,))):
+        plain = torch.autograd.grad(out.square().sum(), leaves, retain_graph=True)
+        grads = torch.autograd.grad(out.square().sum(), leaves, create_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(plain, grads))
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            grads[0].sum().backward()
+
+
+@gpu
+def test_places_that_cannot_be_are_not_followed():
+    """RowGroups built from other tensors than group_rows made: a slot outside (n k,) counts as none."""
+    import torch
+    from qinco_amd import RowGroups
+    n, k = 6, 2
+    place = torch.tensor([[0, 1], [2, 12], [1 << 30, 3], [-7, 4], [5, -(1 << 31)], [6, 7]], dtype=torch.int32, device="cuda")
+    gr = RowGroups(torch.arange(12, dtype=torch.int32, device="cuda"), place, torch.tensor([0, -5], dtype=torch.int32, device="cuda"))
+    y = torch.arange(12.0, device="cuda")[:, None].expand(12, 20).contiguous()
+    assert gr.combine(y)[:, 0].tolist() == [1.0, 2.0, 3.0, 4.0, 5.0, 13.0]
+    assert gr.gather(torch.ones(n, 20, device="cuda")).shape == (12, 20)
+    for bad in ((place[:, 0], place, place[:, 0]), (place.reshape(-1), place, place.reshape(-1)[:1]), (place.reshape(-1)[:-1], place, place.reshape(-1)),
+                (place.reshape(-1).long(), place, place.reshape(-1)), (place.reshape(-1), place.T, place.reshape(-1))):
+        with pytest.raises(ValueError):
+            RowGroups(*bad)
+
+
+@gpu
+def test_rows_behind_four_giga_elements():
+    """2.3 G elements of y and of the gathered rows: places behind 32 bits of element offsets."""
+    import torch
+    from qinco_amd import group_rows
+    n, k, D = 1_150_000, 2, 1000
+    ids = torch.stack([torch.arange(n, device="cuda"), torch.arange(n, device="cuda")], 1)          # row r in places 2 r, 2 r + 1
+    gr = group_rows(ids, n)
+    assert torch.equal(gr.order, torch.arange(n * k, dtype=torch.int32, device="cuda"))
+    x = torch.randint(0, 256, (n, D), device="cuda", dtype=torch.uint8)
+    out = gr.gather(x)
+    for r in (0, 1, n // 2, n - 2, n - 1):
+        assert torch.equal(out[2 * r], x[r]) and torch.equal(out[2 * r + 1], x[r])
+    assert torch.equal(out[::2], x) and torch.equal(out[1::2], x)
+    del x
+    y = out.to(torch.bfloat16)
+    del out
+    w = torch.tensor([[1.0, -0.5]], device="cuda").expand(n, 2)
+    got = gr.combine(y, w)
+    assert torch.equal(got, y[::2] * 0.5)
+    dy, dw = gr._combine_grad(got, y, w.contiguous(), True, True)
+    assert torch.equal(dy[::2], got) and torch.equal(dy[1::2], got * -0.5)
+    for r in (0, n // 2, n - 1):
+        want = float((got[r].double() * y[2 * r].double()).sum())
+        assert abs(float(dw[r, 0]) - want) <= D * 2.0 ** -24 * want and float(dw[r, 0]) == float(dw[r, 1])
 
 
 @gpu
