@@ -116,16 +116,29 @@ static void launch_sample_wave(const SampleArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((sample_wave_kernel<T, R>), dim3((unsigned)g), dim3(64 * kSampleRowWaves), 0, st, a);
 }
 
+template <typename T, int G, int R>
+static void launch_sample_group(const SampleArgs& a, hipStream_t st) {
+  constexpr int ROWS = kSampleGroupThreads / G;
+  long g = (a.n + ROWS - 1) / ROWS;
+  if (g > 1 << 20) g = 1 << 20;
+  hipLaunchKernelGGL((sample_group_kernel<T, G, R>), dim3((unsigned)g), dim3(kSampleGroupThreads), 0, st, a);
+}
+
 template <typename T, int NT>
 static void launch_sample_block(const SampleArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((sample_block_kernel<T, NT>), dim3((unsigned)(a.n < 65536 ? a.n : 65536)), dim3(NT), (size_t)a.V * sizeof(T), st, a);
 }
 
+// By the length of a row alone (a row's code does not depend on its batch, nor does the kernel).  Each border with both sides measured, all
+// three cuts on: 65536 rows of 64 fp32 27 us with 16 lanes each, 52 with 64; 65536 of 256 bf16 89 us with 32 lanes, 107 with 64; 16384 of 512
+// fp32 46 us with 8 codes per lane of a wave, 97 with 16; 16384 of 1024 fp32 128 us with a wave, 179 with a workgroup; one row of 10240 fp32
+// 38 us with a workgroup, 48 split over several, 1000 of them 101 and 179.
 template <typename T>
 static int launch_sample(const SampleArgs& a, const SamplePlan& p, char* ws, hipStream_t st) {
   if (a.V > kSampleLongV) return launch_sample_long<T>(a, p, ws, st);
-  if (a.V <= 64) launch_sample_wave<T, 1>(a, st);
-  else if (a.V <= 256) launch_sample_wave<T, 4>(a, st);
+  if (a.V <= 64) launch_sample_group<T, 16, 4>(a, st);
+  else if (a.V <= 256) launch_sample_group<T, 32, 8>(a, st);
+  else if (a.V <= 512) launch_sample_wave<T, 8>(a, st);
   else if (a.V <= 1024) launch_sample_wave<T, 16>(a, st);
   else launch_sample_block<T, 256>(a, st);
   HIP_TRY(hipGetLastError());

@@ -230,6 +230,333 @@ __device__ __forceinline__ SampleBins sample_bins(float zmax, float zmin, double
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
+// G = 16 or 32 lanes per row, V <= G R: the row stays in registers (lane l holds codes l R ... l R + R - 1), no barrier anywhere.  What is done
+// once per row (scans, bounds, the logarithm) is two thirds of the instructions of a wave per row; here two or four rows share it.
+// Both cuts look at 64 bins of the row first (counts and masses by LDS atomics, 64 / G bins per lane), then at the few codes of the one bin
+// that the cut falls into.  A bin of more than 64 codes (heavy ties) is searched bit by bit instead.
+// ---------------------------------------------------------------------------------------------------------------------
+constexpr int kSampleGroupThreads = 256;
+struct SampleGroupLds {
+  unsigned long long mass[64];
+  unsigned long long m_mass[64];   // codes of the bin in question
+  unsigned count[64];
+  float m_z[64];
+  float t;                         // what one lane found for all
+  unsigned r;
+  unsigned long long q;
+};
+
+// over the G lanes of a row (16: a DPP row; 32: two of them)
+template <int G, typename T>
+__device__ __forceinline__ T sample_row_scan(T v) {   // inclusive
+  v += sample_dpp<0x111, 0xf>(v);
+  v += sample_dpp<0x112, 0xf>(v);
+  v += sample_dpp<0x114, 0xf>(v);
+  v += sample_dpp<0x118, 0xf>(v);
+  if (G == 32) v += sample_dpp<0x142, 0xa>(v);
+  return v;
+}
+template <int G, typename T>
+__device__ __forceinline__ T sample_row_last(T v) {   // the last lane's, in every lane
+  return G == 16 ? sample_dpp<0x15F, 0xf>(v) : __shfl(v, 31, 32);
+}
+template <int G, typename T>
+__device__ __forceinline__ T sample_row_sum(T v) {    // in every lane: by rotations
+  v += sample_dpp<0x128, 0xf>(v);
+  v += sample_dpp<0x124, 0xf>(v);
+  v += sample_dpp<0x122, 0xf>(v);
+  v += sample_dpp<0x121, 0xf>(v);
+  if (G == 32) v += __shfl_xor(v, 16, 32);
+  return v;
+}
+template <int G>
+__device__ __forceinline__ unsigned sample_row_max(unsigned v) {
+  v = max(v, sample_dpp<0x128, 0xf>(v));
+  v = max(v, sample_dpp<0x124, 0xf>(v));
+  v = max(v, sample_dpp<0x122, 0xf>(v));
+  v = max(v, sample_dpp<0x121, 0xf>(v));
+  if (G == 32) v = max(v, __shfl_xor(v, 16, 32));
+  return v;
+}
+
+template <typename T, int G, int R>
+__global__ void __launch_bounds__(kSampleGroupThreads) sample_group_kernel(SampleArgs a) {
+  constexpr int ROWS = kSampleGroupThreads / G, PB = 64 / G;   // rows of a workgroup, bins of a lane
+  __shared__ SampleGroupLds lds[ROWS];
+  SampleGroupLds& s = lds[threadIdx.x / G];
+  const int l = threadIdx.x % G, V = a.V, row_shift = (threadIdx.x & 63) / G * G;
+  // lanes of this row among a ballot's
+  auto mine = [&](unsigned long long ballot) { return (unsigned)(ballot >> row_shift) & (unsigned)((1ull << G) - 1); };
+  // (a row's lanes take every branch together: the loop and the branches below may part rows, never a row)
+  for (long row = (long)blockIdx.x * ROWS + threadIdx.x / G; row < a.n; row += (long)gridDim.x * ROWS) {
+    const T* logits = reinterpret_cast<const T*>(a.logits) + row * a.stride;
+    const SampleRow set = sample_row(a, row);
+    float z[R];
+    {
+      constexpr int U = R * sizeof(T) < 16 ? R : 16 / sizeof(T);   // codes of one load
+      struct alignas(sizeof(T)) Raw { T v[U]; };
+#pragma unroll
+      for (int j = 0; j < R; j += U) {
+        const int i = l * R + j;
+        if (i + U <= V) {
+          const Raw raw = *reinterpret_cast<const Raw*>(logits + i);
+#pragma unroll
+          for (int e = 0; e < U; ++e) {
+            const float x = GroupNum<T>::get(raw.v[e]);
+            z[j + e] = x == x ? x : -INFINITY;
+          }
+        } else {
+#pragma unroll
+          for (int e = 0; e < U; ++e) z[j + e] = sample_logit(logits, i + e, V);
+        }
+      }
+    }
+    float hi = z[0], lo = INFINITY;
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      hi = fmaxf(hi, z[j]);
+      lo = fminf(lo, z[j] > -INFINITY ? z[j] : INFINITY);
+    }
+    const float zmax = sample_unkey(sample_row_max<G>(sample_key(hi)));
+    if (zmax == -INFINITY) {
+      if (l == 0) sample_answer(a, row, -1, -INFINITY);
+      continue;
+    }
+    if (set.greedy) {
+      const int first = __builtin_ctz(mine(__ballot(hi == zmax)));
+      int at = 0;
+#pragma unroll
+      for (int j = R - 1; j >= 0; --j) at = z[j] == zmax ? j : at;
+      if (l == first) sample_answer(a, row, l * R + at, 0.f);
+      continue;
+    }
+    const SampleMass mass(zmax, set.y, a.F);
+    unsigned long long q[R];
+    unsigned floored = 0;   // bit j: cut by min-p
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const double e = mass.e(z[j]);
+      q[j] = mass.whole(e);
+      floored |= (e >= set.m ? 0u : 1u) << j;
+      if ((j & 1) == 1) __builtin_amdgcn_sched_barrier(0);   // (two exponentials at a time: more side by side only take registers)
+    }
+    float t = -INFINITY;
+    unsigned r = 0;
+    const bool by_count = set.k < V, by_mass = set.p < 1.0;
+    if (by_count || by_mass) {
+      const float zmin = sample_unkey(~sample_row_max<G>(~sample_key(lo)));
+      const SampleBins bins = sample_bins(zmax, zmin, set.y, 64);
+#pragma unroll
+      for (int j = 0; j < PB; ++j) {
+        s.mass[l * PB + j] = 0;
+        s.count[l * PB + j] = 0;
+      }
+      sample_wave_sync();
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        const int b = bins.of(z[j]);
+        if (z[j] > -INFINITY) atomicAdd(&s.count[b], 1u);
+        if (q[j]) atomicAdd(&s.mass[b], q[j]);
+      }
+      sample_wave_sync();
+      unsigned c_in[PB], c_sum = 0;
+      unsigned long long m_in[PB], m_sum = 0;
+#pragma unroll
+      for (int j = 0; j < PB; ++j) {
+        c_sum += c_in[j] = s.count[l * PB + j];
+        m_sum += m_in[j] = s.mass[l * PB + j];
+      }
+      const unsigned c_run = sample_row_scan<G>(c_sum), c_all = sample_row_last<G>(c_run);
+      const unsigned long long m_run = sample_row_scan<G>(m_sum);
+      unsigned long long total = sample_row_last<G>(m_run);   // mass of what top-k keeps
+      // codes of bin b into m_z, m_mass; their number
+      auto members = [&](int b) {
+        unsigned in = 0;
+#pragma unroll
+        for (int j = 0; j < R; ++j) in |= (unsigned)(z[j] > -INFINITY && bins.of(z[j]) == b) << j;
+        const unsigned n = __builtin_popcount(in), run = sample_row_scan<G>(n);
+        unsigned to = run - n;
+        if (in) {
+#pragma unroll
+          for (int j = 0; j < R; ++j) {
+            if (in >> j & 1) {
+              if (to < 64) {
+                s.m_z[to] = z[j];
+                s.m_mass[to] = q[j];
+              }
+              ++to;
+            }
+          }
+        }
+        sample_wave_sync();
+        return (int)sample_row_last<G>(run);
+      };
+      int kb = 64, n_kb = 0;        // the bin that top-k cuts, 64: none; its codes
+      unsigned long long qt = 0;    // mass of a code at t
+      if (by_count && (unsigned)set.k < c_all) {
+        unsigned want = (unsigned)set.k - (c_run - c_sum);
+        unsigned long long above = m_run - m_sum;
+        int b = l * PB;
+#pragma unroll
+        for (int j = 0; j < PB - 1; ++j) {
+          const bool on = b == l * PB + j && want > c_in[j];
+          want -= on ? c_in[j] : 0;
+          above += on ? m_in[j] : 0;
+          b += on;
+        }
+        const int src = __builtin_ctz(mine(__ballot(c_run >= (unsigned)set.k)));
+        want = __shfl(want, src, G);
+        above = __shfl(above, src, G);
+        kb = __shfl(b, src, G);
+        n_kb = members(kb);
+        if (n_kb <= 64) {
+          for (int i = l; i < n_kb; i += G) {
+            const float mz = s.m_z[i];
+            unsigned gt = 0, ge = 0;
+            for (int o = 0; o < n_kb; ++o) {
+              gt += s.m_z[o] > mz;
+              ge += s.m_z[o] >= mz;
+            }
+            if (gt < want && want <= ge) {   // (equal logits find the same)
+              s.t = mz;
+              s.r = want - gt;
+              s.q = s.m_mass[i];
+            }
+          }
+          sample_wave_sync();
+          t = s.t;
+          r = s.r;
+          qt = s.q;
+          unsigned long long in = 0;
+          if (by_mass)
+            for (int i = l; i < n_kb; i += G) in += s.m_z[i] > t ? s.m_mass[i] : 0ull;
+          total = above + sample_row_sum<G>(in) + r * qt;
+        } else {   // the largest t that at least k codes reach, a bit at a time
+          unsigned key = 0;
+          for (int b = 31; b >= 0; --b) {
+            const unsigned c = key | 1u << b;
+            unsigned n = 0;
+#pragma unroll
+            for (int j = 0; j < R; ++j) n += sample_key(z[j]) >= c;
+            if (sample_row_sum<G>(n) >= (unsigned)set.k) key = c;
+          }
+          t = sample_unkey(key);
+          unsigned n = 0;
+          unsigned long long m = 0;
+#pragma unroll
+          for (int j = 0; j < R; ++j) {
+            n += z[j] > t;
+            m += z[j] > t ? q[j] : 0ull;
+          }
+          r = (unsigned)set.k - sample_row_sum<G>(n);
+          qt = mass.q(t);
+          total = sample_row_sum<G>(m) + r * qt;
+        }
+      }
+      if (by_mass) {
+        const unsigned long long bound = sample_bound(set.p, total);
+        // (a bin that top-k cuts counts as reached: what it keeps of it is in `total`)
+        unsigned long long need = bound - (m_run - m_sum);
+        int b = l * PB;
+#pragma unroll
+        for (int j = 0; j < PB - 1; ++j) {
+          const bool on = b == l * PB + j && need > m_in[j];
+          need -= on ? m_in[j] : 0;
+          b += on;
+        }
+        const int src = __builtin_ctz(mine(__ballot(m_run >= bound)));
+        need = __shfl(need, src, G);
+        const int pb = __shfl(b, src, G);
+        const int n = pb == kb ? n_kb : members(pb);
+        if (n <= 64) {
+          s.r = 0;
+          sample_wave_sync();
+          unsigned long long in = 0;
+          for (int i = l; i < n; i += G) {
+            const float mz = s.m_z[i];
+            if (mz > t) {
+              const unsigned long long mq = s.m_mass[i];
+              unsigned long long gt = 0, eq = 0;
+              for (int o = 0; o < n; ++o) {
+                const float x = s.m_z[o];
+                const unsigned long long m = s.m_mass[o];
+                gt += x > mz ? m : 0ull;
+                eq += x == mz ? m : 0ull;
+              }
+              if (gt < need && need <= gt + eq) {
+                s.t = mz;
+                s.r = sample_ceil_div(need - gt, mq);
+              }
+              in += mq;
+            }
+          }
+          sample_wave_sync();
+          if (s.r) {
+            t = s.t;
+            r = s.r;
+          } else {   // on the ties that top-k kept
+            r = min(r, sample_ceil_div(need - sample_row_sum<G>(in), qt));
+          }
+        } else {
+          const unsigned kt = sample_key(t);
+          const unsigned long long at_t = r * qt;
+          unsigned key = 0;
+          for (int b = 31; b >= 0; --b) {
+            const unsigned c = key | 1u << b;
+            unsigned long long m = 0;
+#pragma unroll
+            for (int j = 0; j < R; ++j) m += sample_key(z[j]) >= c && z[j] > t ? q[j] : 0ull;
+            if (sample_row_sum<G>(m) + (kt >= c ? at_t : 0ull) >= bound) key = c;
+          }
+          const float x = sample_unkey(key);
+          unsigned long long m = 0;
+#pragma unroll
+          for (int j = 0; j < R; ++j) m += z[j] > x && z[j] > t ? q[j] : 0ull;
+          const unsigned rr = sample_ceil_div(bound - sample_row_sum<G>(m) - (kt > key ? at_t : 0ull), mass.q(x));
+          r = key == kt ? min(r, rr) : rr;
+          t = x;
+        }
+      }
+    }
+    // the draw: kept masses summed in index order
+    unsigned nth = 0;
+    if (r) {
+      unsigned ties = 0;
+#pragma unroll
+      for (int j = 0; j < R; ++j) ties += z[j] == t;
+      nth = sample_row_scan<G>(ties) - ties;
+    }
+    unsigned long long sum = 0;
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const bool tie = z[j] == t;
+      const bool kept = (z[j] > t || (tie && nth < r)) && !(floored >> j & 1);
+      nth += tie;
+      q[j] = kept ? q[j] : 0ull;
+      sum += q[j];
+    }
+    const unsigned long long run = sample_row_scan<G>(sum), total = sample_row_last<G>(run);
+    const unsigned long long target = sample_target(set.u, total);
+    if (run > target && run - sum <= target) {
+      unsigned long long upto = run - sum;
+      int at = 0;
+      float x = 0.f;
+      bool found = false;
+#pragma unroll
+      for (int j = 0; j < R; ++j) {
+        upto += q[j];
+        if (!found && upto > target) {
+          found = true;
+          at = j;
+          x = z[j];
+        }
+      }
+      sample_answer(a, row, l * R + at, mass.logp(x, total));
+    }
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
 // One wave per row, V <= 64 R: the row stays in registers (lane l holds codes l R ... l R + R - 1), no barrier anywhere.
 // Both cuts look at 64 bins of the row first (counts and masses by LDS atomics, scanned by the wave), then at the few codes of the one
 // bin that the cut falls into, a lane each.  A bin of more than 64 codes (heavy ties) is searched bit by bit instead.

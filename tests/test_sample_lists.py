@@ -158,7 +158,7 @@ SETTINGS = [dict(), dict(T=0.7, k=5), dict(p=0.9), dict(m=0.05), dict(T=1.3, k=5
 
 @gpu
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
-@pytest.mark.parametrize("n,V", [(1, 1), (3, 2), (5, 63), (4, 64), (4, 65), (300, 256), (7, 257), (3, 1000), (5, 1024), (5, 1025), (6, 4099),
+@pytest.mark.parametrize("n,V", [(1, 1), (3, 2), (5, 63), (4, 64), (4, 65), (300, 256), (7, 257), (9, 512), (9, 513), (3, 1000), (5, 1024), (5, 1025), (6, 4099),
                                  (2, 10240), (2, 10241), (2, 16384), (2, 16385), (2, 32769), (2, 70001), (1, (1 << 20) + 3)])
 def test_sample_sizes_and_settings(dtype, n, V):
     import torch
@@ -239,7 +239,7 @@ def hard_rows(V, g):
 
 
 @gpu
-@pytest.mark.parametrize("V", [200, 1024, 3000, 10240, 70001, 300001])
+@pytest.mark.parametrize("V", [60, 200, 500, 1024, 3000, 10240, 70001, 300001])
 def test_sample_rows_that_pile_up_in_a_few_bins(V):
     import torch
     g = torch.Generator("cuda").manual_seed(V)
