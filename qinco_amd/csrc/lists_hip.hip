@@ -184,9 +184,9 @@ struct GroupPlan {
 };
 }  // namespace
 
-// Entries per thread.  A tile has a cost of its own (tables of its digits), few tiles leave the chip empty.  Measured, a sort by 1024 lists
-// with 2 / 4 / 8 per thread: 2^17 entries 12.6 / 14.4 / 18.9 us, 2^18 14.4 / 15.4 / 19.5, 2^19 23.3 / 17.9 / 20.7, 2^20 43.4 / 28.4 / 24.5,
-// 2^22 151 / 104 / 67; by 2^20 lists 2^17 34.9 / 38.2 / 45.9, 2^18 41.8 / 43.7 / 50.5, 2^19 63.8 / 53.3 / 58.2, 2^20 112 / 79.6 / 70.3.
+// Entries per thread.  A tile has a cost of its own (tables of its digits), few tiles leave the chip empty.  Measured with 2 / 4 / 8 per
+// thread, a sort by 1024 lists: 2^17 entries 12.6 / 14.4 / 18.9 us, 2^18 14.4 / 15.4 / 19.5, 2^19 23.3 / 17.9 / 20.7, 2^20 43.4 / 28.4 / 24.5,
+// 2^22 151 / 104 / 67.
 static GroupPlan group_plan(int64_t N, int64_t E) {
   GroupPlan p{};
   const int all = bits_of((uint64_t)E);
@@ -229,6 +229,7 @@ static int launch_end(int* place, const int* went1, const int* went2, int64_t N,
   const unsigned follow = (unsigned)((N + 1023) / 1024);
   long g = ((long)E + 256) / 256;
   if (g > 4096) g = 4096;
+  if (start && shift <= kGroupMaxBits) g = ((long)E + (1 << shift) - 1) >> shift;   // a workgroup per bin
   hipLaunchKernelGGL(group_end_kernel, dim3(follow + (unsigned)g), dim3(256), 0, st, follow, place, went1, went2, (unsigned)N, keys, total,
                      start, shift, offsets, E);
   HIP_TRY(hipGetLastError());
