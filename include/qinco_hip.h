@@ -341,8 +341,8 @@ QINCO_API int qinco_group_rows(const void* lists, int code_dtype, int64_t row_st
                                int32_t* place, int32_t* offsets, int32_t* bad, void* workspace, int64_t workspace_bytes, void* stream);
 /* Rows of any type into list order: out[place[r, j]] = x[r]; slots behind *end (= offsets + n_lists) get zeros.  x rows are
  * x_stride_bytes apart, out is (n k) rows of row_bytes. */
-QINCO_API int qinco_group_gather(const void* x, int64_t x_stride_bytes, int64_t row_bytes, const int32_t* place, const int32_t* end,
-                                 int64_t n, int32_t k, void* out, void* stream);
+QINCO_API int qinco_group_gather(const void* x, int64_t x_stride_bytes, int64_t row_bytes, const int32_t* order, const int32_t* place,
+                                 const int32_t* end, int64_t n, int32_t k, void* out, void* stream);
 /* ... and back: out[r] = sum_j w[r, j] y[place[r, j]] over the entries that have a slot (a row without one: zeros), in 32 bits in the
  * order of j, rounded once.  weights (n, k) of w_dtype or NULL (ones: this is the gradient of the gather).  y (n k) rows of D elements,
  * y_stride elements apart; out (n, D).  A weight of an entry without a slot is not read. */

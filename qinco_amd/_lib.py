@@ -166,7 +166,7 @@ def load() -> C.CDLL:
     lib.qinco_group_workspace.restype = i64
     lib.qinco_group_rows.argtypes = [vp, i32, i64, i64, C.c_int32, i64, vp, vp, vp, vp, vp, i64, vp]
     lib.qinco_group_rows.restype = C.c_int
-    lib.qinco_group_gather.argtypes = [vp, i64, i64, vp, vp, i64, C.c_int32, vp, vp]
+    lib.qinco_group_gather.argtypes = [vp, i64, i64, vp, vp, vp, i64, C.c_int32, vp, vp]
     lib.qinco_group_gather.restype = C.c_int
     lib.qinco_group_combine.argtypes = [vp, i32, i64, C.c_int32, vp, i32, vp, i64, C.c_int32, vp, vp]
     lib.qinco_group_combine.restype = C.c_int

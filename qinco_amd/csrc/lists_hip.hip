@@ -318,16 +318,23 @@ static dim3 group_grid(const GroupRows& g) {
   return dim3((unsigned)b);
 }
 
-extern "C" int qinco_group_gather(const void* x, int64_t x_stride_bytes, int64_t row_bytes, const int32_t* place, const int32_t* end,
-                                  int64_t n, int32_t k, void* out, void* stream) {
+extern "C" int qinco_group_gather(const void* x, int64_t x_stride_bytes, int64_t row_bytes, const int32_t* order, const int32_t* place,
+                                  const int32_t* end, int64_t n, int32_t k, void* out, void* stream) {
   if (n < 0 || k < 1 || n > INT32_MAX / k || row_bytes < 1 || row_bytes > INT32_MAX || x_stride_bytes < 0)
     return fail(QINCO_ERR_INVALID, "qinco_group_gather: need n >= 0, k >= 1, n k < 2^31, 1 <= row_bytes < 2^31, a stride >= 0");
   if (n == 0) return QINCO_OK;
-  if (!x || !place || !end || !out) return fail(QINCO_ERR_INVALID, "qinco_group_gather: null buffer");
+  if (!x || !order || !place || !end || !out) return fail(QINCO_ERR_INVALID, "qinco_group_gather: null buffer");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   auto go = [&](auto t) {
     using T = decltype(t);
     const int64_t D = row_bytes / (int64_t)sizeof(T);
+    if (D == 1) {
+      const GroupRows g = group_rows_of(place, end, n, k, 1, 1);
+      const int64_t blocks = (g.N + 255) / 256;
+      hipLaunchKernelGGL(group_pull_kernel<T>, dim3((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20)), dim3(256), 0, st, g, order, (const T*)x,
+                         (long)(x_stride_bytes / (int64_t)sizeof(T)), (T*)out);
+      return;
+    }
     with_unit<T>(D, [&](auto e) {
       constexpr int E = decltype(e)::value;
       const GroupRows g = group_rows_of(place, end, n, k, D, E);

@@ -108,8 +108,8 @@ class RowGroups:
     def _gather(self, x):
         D, size, dev = x.shape[1], x.element_size(), x.device
         out = torch.empty((self.n * self.k, D), dtype=x.dtype, device=dev)
-        on_its_device(dev, _lib.load().qinco_group_gather, x.data_ptr(), x.stride(0) * size, D * size, self.place.data_ptr(), self._end,
-                      self.n, self.k, out.data_ptr())
+        on_its_device(dev, _lib.load().qinco_group_gather, x.data_ptr(), x.stride(0) * size, D * size, self.order.data_ptr(),
+                      self.place.data_ptr(), self._end, self.n, self.k, out.data_ptr())
         return out
 
     def _combine(self, y, weights):

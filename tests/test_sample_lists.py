@@ -98,10 +98,10 @@ def test_group_refusals_are_decided_on_the_host(lib):
     assert lib.qinco_group_workspace(-1, 8) == 0 and lib.qinco_group_workspace(4, 0) == 0 and lib.qinco_group_workspace(4, 1 << 25) == 0
     assert lib.qinco_group_workspace(0, 1) > 0
 
-    def gather(x=at, xs=4, rb=4, place=at, end=at, n=2, k=2, out=at):
-        return lib.qinco_group_gather(x, xs, rb, place, end, n, k, out, None)
+    def gather(x=at, xs=4, rb=4, order=at, place=at, end=at, n=2, k=2, out=at):
+        return lib.qinco_group_gather(x, xs, rb, order, place, end, n, k, out, None)
     assert gather(n=0) == 0
-    for bad in (dict(x=None), dict(xs=-1), dict(rb=0), dict(rb=1 << 31), dict(place=None), dict(end=None), dict(n=-1), dict(k=0), dict(out=None),
+    for bad in (dict(x=None), dict(xs=-1), dict(rb=0), dict(rb=1 << 31), dict(order=None), dict(place=None), dict(end=None), dict(n=-1), dict(k=0), dict(out=None),
                 dict(n=1 << 30, k=2)):
         assert gather(**bad) == -1, bad
 
@@ -332,6 +332,20 @@ def test_group_sizes(N):
 
 
 @gpu
+@pytest.mark.parametrize("N", [300001, 700001, 2100003])
+def test_group_many_entries(N):
+    import torch
+    g = torch.Generator("cuda").manual_seed(N)
+    for E in (1000, 70000, 1 << 20, 1 << 24):
+        r = torch.rand(N, generator=g, device="cuda", dtype=torch.float64)
+        ids = (r.pow(8) * E).long().clamp_(max=E - 1)                                # half of them in a few lists
+        ids[torch.rand(N, generator=g, device="cuda") < 0.1] = -1
+        check_group(ids, E, check=False)
+    check_group(torch.full((N,), 70001, device="cuda", dtype=torch.int32), 1 << 17)
+    check_group(torch.where(torch.arange(N, device="cuda") % 3 == 0, 5, 131000), 1 << 17)
+
+
+@gpu
 def test_group_matrices_columns_and_bad_ids():
     import torch
     from qinco_amd import group_rows
@@ -445,7 +459,7 @@ def test_rows_of_any_type_stride_and_broadcast_gradients():
     gr = make_groups(g, n, k, 40, True)
     order = gr.order.cpu().numpy()
     for dt in (torch.uint8, torch.int32, torch.int64, torch.float64, torch.bool):
-        for D in (1, 7, 8, 9, 16, 33):
+        for D in (1, 2, 4, 7, 8, 9, 16, 33):
             x = torch.randint(0, 100, (n, D + 5), generator=g, device="cuda").to(dt)
             for v in (x[:, :D], x[:, 2:2 + D], x.T.contiguous().T[:, :D], x[:1, :D].expand(n, D)):
                 got = gr.gather(v).cpu().numpy()
