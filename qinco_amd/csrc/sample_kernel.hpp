@@ -59,7 +59,8 @@ __device__ __forceinline__ SampleRow sample_row(const SampleArgs& a, long r) {
   const double T = a.T_rows ? (double)a.T_rows[r] : a.T;
   s.greedy = !(T > 0.0);
   s.y = s.greedy ? 1.0 : 1.4426950408889634074 * sample_reciprocal(T);
-  s.y = fmax(s.y, 1e-290);   // (T = inf: every finite logit has the same mass, and inf - inf stays out of the arithmetic)
+  // (T = inf: every finite logit has the same mass; 1 / T = inf: nothing but the largest has any.  0 * inf and inf - inf stay out of it)
+  s.y = fmin(fmax(s.y, 1e-290), 1e290);
   s.k = a.k_rows ? a.k_rows[r] : a.k;
   if (s.k <= 0 || s.k > a.V) s.k = a.V;
   s.p = a.p_rows ? (double)a.p_rows[r] : a.p;
@@ -166,12 +167,12 @@ __device__ __forceinline__ unsigned long long sample_target(double u, unsigned l
   const unsigned long long v = (unsigned long long)(u * (double)total);
   return v < total ? v : total - 1;
 }
-// smallest r with r q >= rem (q >= 1, r < 2^25)
+// smallest r with r q >= rem, at most 2^25 (the quotient in 64 bits is off by less than one)
 __device__ __forceinline__ unsigned sample_ceil_div(unsigned long long rem, unsigned long long q) {
   if (rem <= q) return rem ? 1 : 0;
-  unsigned r = (unsigned)((double)rem / (double)q);
-  while (r * q < rem) ++r;
-  while (r && (r - 1) * q >= rem) --r;
+  unsigned r = (unsigned)fmin(ceil((double)rem / (double)q), 0x1p25);
+  if ((r - 1) * q >= rem) --r;
+  if (r * q < rem) ++r;
   return r;
 }
 
@@ -1237,7 +1238,7 @@ struct SampleLogBins {
   }
 };
 __device__ __forceinline__ SampleLogBins sample_log_bins(float zmax, float zmin, double y) {
-  const float d = fminf(zmax - zmin, (float)fmin(54.0 / y, 3e38));
+  const float d = fminf(zmax - zmin, (float)fmin(fmax(54.0 / y, 1e-36), 3e38));
   return SampleLogBins{zmax, d > 0.f && zmax < INFINITY ? fminf(255.f / d, 3e38f) : 0.f};
 }
 

@@ -153,7 +153,7 @@ def check_sample(z, u, *, T=1.0, k=0, p=1.0, m=0.0, code_dtype=np.int64):
 
 
 SETTINGS = [dict(), dict(T=0.7, k=5), dict(p=0.9), dict(m=0.05), dict(T=1.3, k=50, p=0.8, m=0.01), dict(T=0.0), dict(k=1), dict(p=0.0), dict(m=1.0),
-            dict(p=1e-6), dict(T=1e-3, k=3, p=0.99)]
+            dict(p=1e-6), dict(T=1e-3, k=3, p=0.99), dict(T=1e-30, p=0.9), dict(T=1e30, p=0.5), dict(T=1e30, k=7, m=1.0)]
 
 
 @gpu
@@ -202,6 +202,22 @@ def test_sample_masks_infinities_nan_and_ties():
             u = torch.rand(40, generator=g, device="cuda")
             u[20:24] = torch.tensor([0.0, 1.0 - 2.0 ** -24, 0.5, 2.0 ** -30])
             check_sample(z, u, **s)
+
+
+@gpu
+@pytest.mark.parametrize("V", [40, 200, 500, 1000, 6000, 20000])
+def test_sample_temperatures_whose_reciprocal_overflows(V):
+    """1 / T is infinite: the largest logits share all the mass, wherever the cuts are."""
+    import torch
+    g = torch.Generator("cuda").manual_seed(V)
+    z = torch.randn(6, V, generator=g, device="cuda")
+    z[2:4] = torch.randint(-2, 3, (2, V), generator=g, device="cuda").float()
+    z[4, ::2] = -float("inf")
+    z[5] = 0.25
+    u = torch.tensor([0.0, 0.9, 0.3, 0.999, 0.5, 0.7], device="cuda")
+    for T in (1e-310, 5e-324, 2.3e-308, np.full(6, 1e-45, np.float32)):
+        for s in (dict(), dict(p=0.5), dict(k=3), dict(k=30, p=0.3), dict(m=0.5)):
+            check_sample(z, u, T=T, **s)
 
 
 @gpu
