@@ -8,7 +8,7 @@
 //
 // NUMBERS.  A random number next to a border between two codes must fall on the side that exact arithmetic gives it, whatever order
 // the sums are taken in: e is computed in 64 bits and held as a whole number of 2^-F, F = min(51, 62 - log2 V), and all sums are of
-// whole numbers (atomics in any order give the same bits, and so do the three forms below).
+// whole numbers (atomics in any order give the same bits, and so do the forms below).
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -947,7 +947,7 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
   __shared__ SampleFound found;
   __shared__ unsigned range[2][NT / 64], key_range[2];
   __shared__ float m_z[64];
-  __shared__ int n_listed;
+  __shared__ int n_listed[2];   // by top-k, by top-p
   __shared__ struct {
     float t;
     unsigned r;
@@ -1019,7 +1019,7 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
           if (q) atomicAdd(&bin_mass[b], q);
         }
       });
-      if (tid == 0) n_listed = 0;
+      if (tid < 2) n_listed[tid] = 0;
       __syncthreads();
       unsigned long long m = 0, m_before, total;
       unsigned c = 0, c_before, c_all;
@@ -1030,15 +1030,15 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
       }
       sample_block_scan<NT>(blk, m, c, m_before, c_before, total, c_all);
       // codes of bin b above t into m_z; their number
-      auto list = [&](int b) {
+      auto list = [&](int b, int cut) {
         each([&](float z) {
           if (z > t && bins.of(z) == b) {
-            const int to = atomicAdd(&n_listed, 1);
+            const int to = atomicAdd(&n_listed[cut], 1);
             if (to < 64) m_z[to] = z;
           }
         });
         __syncthreads();
-        return n_listed;
+        return n_listed[cut];
       };
       // the smallest and largest key of bin b above t
       auto keys_of = [&](int b, unsigned& first, unsigned& last) {
@@ -1084,7 +1084,7 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
         kb = found.bin;
         const unsigned want = found.count;
         k_above = found.mass;
-        const int n = list(kb);
+        const int n = list(kb, 0);
         if (n <= 64) {
           if (w == 0) {
             const float mz = lane < n ? m_z[lane] : -INFINITY;
@@ -1101,7 +1101,6 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
               cut.t = z_at;
               cut.r = want - sample_lane(gt, at);
               cut.in = in;
-              n_listed = 0;
             }
           }
           __syncthreads();
@@ -1119,7 +1118,6 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
           });
           t = sample_unkey(key);
           r = want - (unsigned)before;
-          if (tid == 0) n_listed = 0;
           unsigned long long in = 0, none;
           unsigned none_c, none_all;
           each([&](float z) {
@@ -1149,7 +1147,7 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
           __syncthreads();
           const int pb = found.bin;
           const unsigned long long need = bound - found.mass;
-          const int n = list(pb);
+          const int n = list(pb, 1);
           if (n <= 64) {
             if (w == 0) {
               const float mz = lane < n ? m_z[lane] : -INFINITY;
