@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kGroupThreads) group_small_kernel(GroupPass a,
       }
     }
     __syncthreads();
-      auto key_of = [&](int r) { return key[r]; };
+    auto key_of = [&](int r) { return key[r]; };
     if (a.bits <= 8) group_rank<8>(whist[w], key_of, shift, mask, rank, rounds);
     else group_rank<kGroupMaxBits>(whist[w], key_of, shift, mask, rank, rounds);
     __syncthreads();
@@ -685,9 +685,19 @@ __global__ void __launch_bounds__(256) group_combine_grad_kernel(GroupRows g, co
             }
           }
           if (dw) {
+            if (at < u * E) {   // the last unit's overlap counts once: zeros on both sides (0 inf would be NaN)
+#pragma unroll
+              for (int e = 0; e < E; ++e) {
+                if (at + e < u * E) {
+                  d.v[e] = T{};
+#pragma unroll
+                  for (int j = 0; j < J; ++j) v[j].v[e] = T{};
+                }
+              }
+            }
             float x[E];
 #pragma unroll
-            for (int e = 0; e < E; ++e) x[e] = at + e >= u * E ? GroupNum<T>::get(d.v[e]) : 0.f;   // (the overlap counts once)
+            for (int e = 0; e < E; ++e) x[e] = GroupNum<T>::get(d.v[e]);
 #pragma unroll
             for (int j = 0; j < J; ++j) {
               if (p[j] >= 0) {

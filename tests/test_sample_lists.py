@@ -450,6 +450,29 @@ def test_gather_and_combine_with_gradients(dtype, n, k, D):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
+def test_infinities_in_the_overlap_of_the_last_unit(dtype):
+    """A row's last 16 bytes overlap the ones before them: an infinity there is summed once, and times nothing else."""
+    import torch
+    g = torch.Generator("cuda").manual_seed(21)
+    gr = make_groups(g, 40, 3, 10, False)
+    for D in (9, 11, 13):
+        y = torch.rand(120, D, generator=g, device="cuda") + 0.5
+        y[::4, D - 3] = float("inf")
+        y[1::4, D - 2] = -float("inf")
+        y = y.to(getattr(torch, dtype))
+        d = (torch.rand(40, D, generator=g, device="cuda") + 0.5).to(y.dtype)
+        d[::5, D - 3] = float("inf")
+        w = torch.rand(40, 3, generator=g, device="cuda").requires_grad_()
+        dw, = torch.autograd.grad(gr.combine(y, w), w, d)
+        with np.errstate(invalid="ignore"):
+            want = (to64(d)[:, None] * to64(y)[gr.place.cpu().numpy()]).sum(2)
+        got, fin = to64(dw), np.isfinite(want)
+        assert np.array_equal(got[~fin], want[~fin], equal_nan=True) and 0 < fin.sum() < fin.size
+        assert np.all(np.abs(got[fin] - want[fin]) <= (D + 1) * 2.0 ** -24 * want[fin])      # (all terms positive)
+
+
+@gpu
 def test_gradients_against_differences():
     """Both operators are linear in the rows and in the weights: the difference over a step of 1 along a direction is the gradient's
     product with it, up to the rounding of two sums of some thousand terms of size 1 in 32 bits."""
