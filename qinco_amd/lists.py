@@ -10,7 +10,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .sample import _TYPES, on_device, on_its_device, row_type, unit_rows
+from .sample import _TYPES, as_stored, on_device, on_its_device, row_type, unit_rows
 
 MAX_LISTS = 1 << 24
 _IDS = {torch.int64: _lib.CODE_I64, torch.int32: _lib.CODE_I32, torch.uint8: _lib.CODE_U8}
@@ -77,8 +77,8 @@ class RowGroups:
 
     def _rows(self, t, rows: int, what: str):
         shape = on_device(t, what).shape
-        if len(shape) != 2 or shape[0] != rows or shape[1] < 1 or t.device != self.place.device:
-            raise ValueError(f"{what} must be ({rows}, D) with D >= 1 on {self.place.device}, got {tuple(t.shape)} on {t.device}")
+        if len(shape) != 2 or shape[0] != rows or not 1 <= shape[1] < 1 << 31 or t.device != self.place.device:
+            raise ValueError(f"{what} must be ({rows}, D) with 1 <= D < 2^31 on {self.place.device}, got {tuple(t.shape)} on {t.device}")
         return unit_rows(t)
 
     def gather(self, x):
@@ -99,7 +99,7 @@ class RowGroups:
         if weights is not None:
             if on_device(weights, "weights").shape != (self.n, self.k) or weights.dtype not in (torch.float32, y.dtype) or weights.device != y.device:
                 raise ValueError(f"weights must be ({self.n}, {self.k}) float32 or {y.dtype} on {y.device}, got {tuple(weights.shape)} {weights.dtype}")
-            weights = weights.contiguous()
+            weights = as_stored(weights).contiguous()
         if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
             return _Combine.apply(y, weights, self)
         return self._combine(y, weights)

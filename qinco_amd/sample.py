@@ -36,9 +36,14 @@ def row_type(t, what: str) -> int:
     return code
 
 
+def as_stored(t):
+    """The same tensor with its values in memory: a view that torch conjugates or negates on reading is copied."""
+    return t.resolve_conj().resolve_neg() if t.is_neg() or t.is_conj() else t
+
+
 def unit_rows(t):
     """The same 2-D tensor with neighbouring elements of a row next to each other (a copy only where they are not)."""
-    return t if t.shape[1] == 1 or t.stride(1) == 1 else t.contiguous()
+    return as_stored(t if t.shape[1] == 1 or t.stride(1) == 1 else t.contiguous())
 
 
 _current_device = torch.cuda.current_device
@@ -84,7 +89,7 @@ def sample_codes(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, c
     def rows(t, what, types):
         if on_device(t, what).shape != (n,) or t.dtype not in types or t.device != dev:
             raise ValueError(f"{what} must be ({n},) of {' or '.join(map(str, types))} on {dev}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-        return t.contiguous()
+        return as_stored(t).contiguous()
     u = rows(u, "u", _RANDOM)
     params = _lib.QincoSampleParams(_PARAMS_BYTES)
     keep = []                                          # (arrays made contiguous live until the call is enqueued)

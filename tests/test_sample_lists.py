@@ -529,6 +529,46 @@ def test_rows_of_any_type_stride_and_broadcast_gradients():
 
 
 @gpu
+def test_views_that_torch_conjugates_or_negates_on_reading():
+    import torch
+    from qinco_amd import sample_codes
+    g = torch.Generator("cuda").manual_seed(22)
+    n, k = 30, 2
+    gr = make_groups(g, n, k, 7, False)
+
+    def minus(*shape):                                         # the negated imaginary part, a view that holds the positive one
+        z = torch.complex(torch.zeros(shape, device="cuda"), torch.rand(shape, generator=g, device="cuda") + 0.5)
+        v = z.conj().imag
+        assert v.is_neg() and bool((v < 0).all())
+        return v
+    for D in (1, 6):
+        y, w = minus(n * k, D), minus(n, k)
+        assert torch.equal(gr.combine(y, w), gr.combine(y.clone(), w.clone())) and bool((gr.combine(y, w) > 0).all())
+        x = minus(n, D)
+        assert torch.equal(gr.gather(x), gr.gather(x.clone()))
+        c = torch.randn(n, D, generator=g, device="cuda", dtype=torch.complex64).conj()
+        assert c.is_conj() and torch.equal(gr.gather(c), c[gr.order.long() // k])
+    leaf = torch.rand(n, 1, generator=g, device="cuda").requires_grad_()
+    gr.gather(leaf).backward(minus(n * k, 1))
+    assert bool((leaf.grad < 0).all())
+    z = minus(1, 1)
+    assert torch.equal(sample_codes(z.expand(4, 1), torch.rand(4, device="cuda")), torch.zeros(4, dtype=torch.int64, device="cuda"))
+    z = torch.cat([minus(4, 5), torch.zeros(4, 5, device="cuda")], 1)
+    assert bool((sample_codes(z, torch.rand(4, device="cuda"), temperature=0.0) == 5).all())
+    z = minus(4, 5)
+    assert torch.equal(sample_codes(z, torch.rand(4, device="cuda"), temperature=0.0), z.argmax(1))
+
+
+@gpu
+def test_rows_too_long_are_refused():
+    import torch
+    gr = make_groups(torch.Generator("cuda").manual_seed(1), 1, 1, 1, False)
+    for f in (gr.gather, gr.combine):
+        with pytest.raises(ValueError, match="2\\^31"):
+            f(torch.zeros(1, 1, device="cuda").expand(1, (1 << 32) + 5))
+
+
+@gpu
 def test_second_derivatives_are_refused_and_first_ones_with_their_graph_are_not():
     import torch
     g = torch.Generator("cuda").manual_seed(5)
