@@ -41,7 +41,7 @@ def group_rows(lists, n_lists: int, check: bool = True) -> "RowGroups":
     bad = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
     need = lib.qinco_group_workspace(n * k, int(n_lists))
     ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    on_its_device(dev, lib.qinco_group_rows, lists.data_ptr(), code, lists.stride(0), n, k, int(n_lists), order.data_ptr(), place.data_ptr(),
+    on_its_device(dev.index, lib.qinco_group_rows, lists.data_ptr(), code, lists.stride(0), n, k, int(n_lists), order.data_ptr(), place.data_ptr(),
                   offsets.data_ptr(), bad.data_ptr() if check else None, ws.data_ptr(), need)
     if check and int(bad):
         raise IndexError(f"a list id is >= n_lists = {n_lists}")
@@ -66,10 +66,16 @@ class RowGroups:
         self._set(order, place, offsets)
 
     def _set(self, order, place, offsets):
-        self.order, self.place, self.offsets = order, place, offsets
+        self._tensors = order, place, offsets
         self.n, self.k = place.shape
         self.n_lists = offsets.numel() - 1
-        self._end = offsets.data_ptr() + 4 * self.n_lists   # address of the places in use
+        # what the library calls take (a call's time in Python counts: autograd runs backward passes on a thread of its own, with cold caches)
+        self._lib, self._index = _lib.load(), place.device.index
+        self._order, self._place, self._end = order.data_ptr(), place.data_ptr(), offsets.data_ptr() + 4 * self.n_lists   # (the places in use)
+
+    order = property(lambda self: self._tensors[0])
+    place = property(lambda self: self._tensors[1])
+    offsets = property(lambda self: self._tensors[2])
 
     def counts(self):
         """Entries of every list (n_lists,)."""
@@ -77,7 +83,7 @@ class RowGroups:
 
     def _rows(self, t, rows: int, what: str):
         shape = on_device(t, what).shape
-        if len(shape) != 2 or shape[0] != rows or not 1 <= shape[1] < 1 << 31 or t.device != self.place.device:
+        if len(shape) != 2 or shape[0] != rows or not 1 <= shape[1] < 1 << 31 or t.device.index != self._index:
             raise ValueError(f"{what} must be ({rows}, D) with 1 <= D < 2^31 on {self.place.device}, got {tuple(t.shape)} on {t.device}")
         return unit_rows(t)
 
@@ -104,28 +110,29 @@ class RowGroups:
             return _Combine.apply(y, weights, self)
         return self._combine(y, weights)
 
-    # -- the library calls; arguments are checked already
+    # -- the library calls; arguments are checked already, rows in unit_rows' form
     def _gather(self, x):
-        D, size, dev = x.shape[1], x.element_size(), x.device
-        out = torch.empty((self.n * self.k, D), dtype=x.dtype, device=dev)
-        on_its_device(dev, _lib.load().qinco_group_gather, x.data_ptr(), x.stride(0) * size, D * size, self.order.data_ptr(),
-                      self.place.data_ptr(), self._end, self.n, self.k, out.data_ptr())
+        D, size = x.shape[1], x.element_size()
+        out = x.new_empty((self.n * self.k, D))
+        on_its_device(self._index, self._lib.qinco_group_gather, x.data_ptr(), x.stride(0) * size, D * size, self._order, self._place,
+                      self._end, self.n, self.k, out.data_ptr())
         return out
 
     def _combine(self, y, weights):
-        D, dev = y.shape[1], y.device
-        out = torch.empty((self.n, D), dtype=y.dtype, device=dev)
-        wt, w_type = (weights.data_ptr(), _TYPES[weights.dtype]) if weights is not None else (None, 0)
-        on_its_device(dev, _lib.load().qinco_group_combine, y.data_ptr(), _TYPES[y.dtype], y.stride(0), D, wt, w_type, self.place.data_ptr(),
+        D, wt, w_type = y.shape[1], None, 0
+        out = y.new_empty((self.n, D))
+        if weights is not None:
+            wt, w_type = weights.data_ptr(), _TYPES[weights.dtype]
+        on_its_device(self._index, self._lib.qinco_group_combine, y.data_ptr(), _TYPES[y.dtype], y.stride(0), D, wt, w_type, self._place,
                       self.n, self.k, out.data_ptr())
         return out
 
     def _combine_grad(self, dout, y, weights, need_dy, need_dw):
-        D, dev = y.shape[1], y.device
-        dy = torch.empty((self.n * self.k, D), dtype=y.dtype, device=dev) if need_dy else None
-        dw = torch.empty((self.n, self.k), dtype=weights.dtype, device=dev) if need_dw else None
-        on_its_device(dev, _lib.load().qinco_group_combine_grad, dout.data_ptr(), dout.stride(0), y.data_ptr(), y.stride(0), _TYPES[y.dtype], D,
-                      weights.data_ptr(), _TYPES[weights.dtype], self.place.data_ptr(), self._end, self.n, self.k,
+        D = y.shape[1]
+        dy = y.new_empty((self.n * self.k, D)) if need_dy else None
+        dw = weights.new_empty((self.n, self.k)) if need_dw else None
+        on_its_device(self._index, self._lib.qinco_group_combine_grad, dout.data_ptr(), dout.stride(0), y.data_ptr(), y.stride(0),
+                      _TYPES[y.dtype], D, weights.data_ptr(), _TYPES[weights.dtype], self._place, self._end, self.n, self.k,
                       dy.data_ptr() if need_dy else None, dw.data_ptr() if need_dw else None)
         return dy, dw
 
@@ -139,7 +146,8 @@ def _combine_grad(ctx, dout):
     if not ctx.weighted:
         return ctx.groups._gather(dout), None, None
     y, weights = ctx.saved_tensors
-    return (*ctx.groups._combine_grad(dout, y, weights, ctx.needs_input_grad[0], ctx.needs_input_grad[1]), None)
+    need_dy, need_dw, _ = ctx.needs_input_grad
+    return (*ctx.groups._combine_grad(dout, y, weights, need_dy, need_dw), None)
 
 
 # Second derivatives are refused.  once_differentiable() costs as much as the rest of a small backward call, and without create_graph (the

@@ -43,22 +43,22 @@ def as_stored(t):
 
 def unit_rows(t):
     """The same 2-D tensor with neighbouring elements of a row next to each other (a copy only where they are not)."""
-    return as_stored(t if t.shape[1] == 1 or t.stride(1) == 1 else t.contiguous())
+    t = as_stored(t)
+    return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-_current_device = torch.cuda.current_device
+_current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 # the handle of a device's current stream without a Stream object around it (2 us of a call of 12), where this torch has it
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-def on_its_device(dev, call, *args) -> None:
-    """One library call on the current stream of `dev` (its last argument), with `dev` current: kernels are launched on a stream of the
-    current device."""
-    index = dev.index
+def on_its_device(index: int, call, *args) -> None:
+    """One library call on the current stream of device `index` (its last argument), with that device current: kernels are launched on a
+    stream of the current device."""
     if _current_device() == index:
         rc = call(*args, _raw_stream(index))
     else:
-        with torch.cuda.device(dev):
+        with torch.cuda.device(index):
             rc = call(*args, _raw_stream(index))
     if rc:
         _lib.check(rc)
@@ -126,6 +126,6 @@ def sample_codes(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, c
     logp = torch.empty(n, dtype=torch.float32, device=dev) if return_logp else None
     need = lib.qinco_sample_workspace(n, V)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
-    on_its_device(dev, lib.qinco_sample_codes, logits.data_ptr(), dtype, logits.stride(0), n, V, u.data_ptr(), u.dtype == torch.float64,
+    on_its_device(dev.index, lib.qinco_sample_codes, logits.data_ptr(), dtype, logits.stride(0), n, V, u.data_ptr(), u.dtype == torch.float64,
                   params, codes.data_ptr(), code, logp.data_ptr() if return_logp else None, ws.data_ptr() if need else None, need)
     return (codes, logp) if return_logp else codes
