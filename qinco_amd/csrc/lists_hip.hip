@@ -26,8 +26,10 @@ static bool known(int dtype) { return dtype == QINCO_T_F32 || dtype == QINCO_T_F
 // ---------------------------------------------------------------------------------------------
 // sampling
 // ---------------------------------------------------------------------------------------------
+static constexpr long kCUs = 256;
+static constexpr int kSampleBlockThreads = 1024, kSampleBlockCodes = 20;   // the largest workgroup per row, and codes per thread
 // V above which a row is split over workgroups
-static constexpr int64_t kSampleLongV = kSampleBlockV;
+static constexpr int64_t kSampleLongV = kSampleBlockThreads * kSampleBlockCodes;
 
 namespace {
 struct SamplePlan {
@@ -124,23 +126,32 @@ static void launch_sample_group(const SampleArgs& a, hipStream_t st) {
   hipLaunchKernelGGL((sample_group_kernel<T, G, R>), dim3((unsigned)g), dim3(kSampleGroupThreads), 0, st, a);
 }
 
-template <typename T, int NT>
+template <typename T, int NT, int R>
 static void launch_sample_block(const SampleArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((sample_block_kernel<T, NT>), dim3((unsigned)(a.n < 65536 ? a.n : 65536)), dim3(NT), (size_t)a.V * sizeof(T), st, a);
+  constexpr long MOST = 1 << 21;   // (threads of a launch: below 2^32)
+  for (long r0 = 0; r0 < a.n; r0 += MOST)
+    hipLaunchKernelGGL((sample_block_kernel<T, NT, R>), dim3((unsigned)(a.n - r0 < MOST ? a.n - r0 : MOST)), dim3(NT), 0, st, a, r0);
 }
 
-// By the length of a row alone (a row's code does not depend on its batch, nor does the kernel).  Each border with both sides measured, all
-// three cuts on: 65536 rows of 64 fp32 27 us with 16 lanes each, 52 with 64; 65536 of 256 bf16 89 us with 32 lanes, 107 with 64; 16384 of 512
-// fp32 46 us with 8 codes per lane of a wave, 97 with 16; 16384 of 1024 fp32 128 us with a wave, 179 with a workgroup; one row of 10240 fp32
-// 38 us with a workgroup, 48 split over several, 1000 of them 101 and 179.
+// By the length of a row, and above 1024 codes by whether there is a CU for every row: then more threads share one (a row's code depends on
+// neither).  Each border with both sides measured, all three cuts on, fp32: 65536 rows of 64 27 us with 16 lanes each, 52 with 64; 65536 of 256
+// (bf16) 89 us with 32 lanes, 107 with 64; 16384 of 512 40 us with a wave each, 75 with four, of 520 86 and 85; 8000 of 2000 70 us with 8
+// codes per thread, 83 with 20; of 4099 127 us with 256 threads, 171 with 512; of 10240 274 with 512 threads, 384 with 256, 435 with 1024; one
+// row of 20480 19 us with a workgroup, 44 split over several, 1000 of them 87 and 216.  One row of 2000 7.5 us with 512 threads, 9.0 with 256,
+// 300 of them 9.7 and 9.4; one of 4099 10.2 and 13.6; one of 10240 13.7 with 1024 threads, 15.0 with 512, 300 of them 27 and 21.
 template <typename T>
 static int launch_sample(const SampleArgs& a, const SamplePlan& p, char* ws, hipStream_t st) {
   if (a.V > kSampleLongV) return launch_sample_long<T>(a, p, ws, st);
   if (a.V <= 64) launch_sample_group<T, 16, 4>(a, st);
   else if (a.V <= 256) launch_sample_group<T, 32, 8>(a, st);
   else if (a.V <= 512) launch_sample_wave<T, 8>(a, st);
-  else if (a.V <= 1024) launch_sample_wave<T, 16>(a, st);
-  else launch_sample_block<T, 256>(a, st);
+  else if (a.V <= 256 * 4) launch_sample_block<T, 256, 4>(a, st);
+  else if (a.n <= kCUs && a.V <= 512 * 4) launch_sample_block<T, 512, 4>(a, st);
+  else if (a.n <= kCUs && a.V <= 512 * 12) launch_sample_block<T, 512, 12>(a, st);
+  else if (a.V <= 256 * 8) launch_sample_block<T, 256, 8>(a, st);
+  else if (a.V <= 256 * 20) launch_sample_block<T, 256, 20>(a, st);
+  else if (a.n > kCUs && a.V <= 512 * 20) launch_sample_block<T, 512, 20>(a, st);
+  else launch_sample_block<T, kSampleBlockThreads, kSampleBlockCodes>(a, st);
   HIP_TRY(hipGetLastError());
   return QINCO_OK;
 }

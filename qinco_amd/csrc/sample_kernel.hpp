@@ -932,20 +932,22 @@ __device__ __forceinline__ void sample_draw(const SampleArgs& a, long row, const
   }
 }
 
-// One workgroup per row, its logits in LDS (V of them, as they come): wave w owns a run of `steps` x 64 codes.  The codes of the bin that a
-// cut falls into are listed, and up to 64 of them compared by one wave, a lane each; more (heavy ties) are searched in bins.  The kernel
-// is bound by its barriers and the latency between them: four waves per row and several rows per CU, rather than sixteen waves.
-constexpr int kSampleBlockV = 10240;   // row + 21 KB of bins and scratch within the 64 KB of LDS that a launch may ask for without more ado
-template <typename T, int NT>
-__global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
-  extern __shared__ __align__(16) unsigned char sample_row_lds[];
-  T* row_z = reinterpret_cast<T*>(sample_row_lds);
-  constexpr int PB = kSampleBins / NT;
+// One workgroup per row, V <= NT R, the row and its masses in registers: thread t holds codes t steps ... t steps + steps - 1.  The codes of
+// the bin that a cut falls into are listed, and up to 64 of them compared by one wave, a lane each; more (heavy ties) are searched in bins.
+// One scan over the threads, of the mass above t and of the codes at t, gives the total and the thread that the draw falls on.  Every
+// exponential is taken once (of what top-k keeps alone, where nothing else wants them) and kept: with the row in LDS, taking them anew in
+// each pass, 8000 rows of 4099 fp16 went in 138 us without a cut and 206 with all three; so they go in 80 and 126 (34 of it up to the
+// largest logit), and one row of 10240 in 13 instead of 36.  Bound by instructions: 44 per exponential, about 25 per code for the rest.
+template <typename T, int NT, int R>
+__global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a, long row0) {
+  constexpr int PB = kSampleBins / NT, PAIR = 2;
+  static_assert(PB * NT == kSampleBins && R % 4 == 0 && R <= 32, "bins per thread, groups of a row, bits of a mask");
   __shared__ unsigned long long bin_mass[kSampleBins], part[kSampleBins];
   __shared__ unsigned bin_count[kSampleBins];
   __shared__ SampleBlock<NT> blk;
   __shared__ SampleFound found;
   __shared__ unsigned range[2][NT / 64], key_range[2];
+  __shared__ unsigned long long m_mass[64];
   __shared__ float m_z[64];
   __shared__ int n_listed[2];   // by top-k, by top-p
   __shared__ struct {
@@ -954,259 +956,305 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a) {
     unsigned long long in;
   } cut;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, V = a.V;
-  const int steps = (V + NT - 1) / NT, w0 = w * steps * 64;
-  for (long row = blockIdx.x; row < a.n; row += gridDim.x) {
-    const T* logits = reinterpret_cast<const T*>(a.logits) + row * a.stride;
-    const SampleRow set = sample_row(a, row);
-    float hi = -INFINITY, lo = INFINITY;
-#pragma unroll 4
-    for (int j = 0; j < steps; ++j) {
-      const int i = w0 + j * 64 + lane;
-      const float z = sample_logit(logits, i, V);
-      if (i < V) row_z[i] = logits[i];
-      hi = fmaxf(hi, z);
-      lo = fminf(lo, z > -INFINITY ? z : INFINITY);
-    }
-    // f(z) for every code of this thread that can be drawn (a thread reads what it wrote)
-    auto each = [&](auto f) {
-#pragma unroll 2
-      for (int j = 0; j < steps; ++j) {
-        const float z = sample_logit(row_z, w0 + j * 64 + lane, V);
-        if (z > -INFINITY) f(z);
+  const int steps = (V + NT - 1) / NT, i0 = tid * steps;
+  const long row = row0 + blockIdx.x;
+  const T* logits = reinterpret_cast<const T*>(a.logits) + row * a.stride;
+  const SampleRow set = sample_row(a, row);
+  float z[R], hi = -INFINITY, lo = INFINITY;
+#pragma unroll
+  for (int j = 0; j < R; j += 4) {
+    if (j + 4 <= steps && i0 + j + 4 <= V) {
+      GroupUnit<T, 4> u;
+      u.load(logits + i0 + j);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x = GroupNum<T>::get(u.v[e]);
+        z[j + e] = x == x ? x : -INFINITY;
       }
-    };
-    unsigned khi = sample_wave_max(sample_key(hi)), klo = sample_wave_max(~sample_key(lo));
-    if (lane == 0) {
-      range[0][w] = khi;
-      range[1][w] = klo;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[j + e] = j + e < steps ? sample_logit(logits, i0 + j + e, V) : -INFINITY;
     }
-    for (int b = tid; b < kSampleBins; b += NT) {
-      bin_mass[b] = 0;
-      bin_count[b] = 0;
+  }
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    hi = fmaxf(hi, z[j]);
+    lo = fminf(lo, z[j] > -INFINITY ? z[j] : INFINITY);
+  }
+  // f(j, logit) for this thread's codes, two at a time.  (The logit in a form that what is made of it is not kept from one pass to the
+  // next, nor taken out of a loop: a key or a bin is fewer instructions than a spilled register.)
+  auto each = [&](auto f) {
+#pragma unroll
+    for (int j = 0; j < R; j += PAIR) {
+      if (j < steps) {
+#pragma unroll
+        for (int e = 0; e < PAIR; ++e) {
+          float x = z[j + e];
+          asm volatile("" : "+v"(x));
+          f(j + e, x);
+        }
+      }
     }
+  };
+  unsigned khi = sample_wave_max(sample_key(hi)), klo = sample_wave_max(~sample_key(lo));
+  if (lane == 0) {
+    range[0][w] = khi;
+    range[1][w] = klo;
+  }
+#pragma unroll
+  for (int j = 0; j < PB; ++j) {
+    bin_mass[tid + j * NT] = 0;
+    bin_count[tid + j * NT] = 0;
+  }
+  if (tid < 2) n_listed[tid] = 0;
+  __syncthreads();
+  khi = sample_wave_max(lane < NT / 64 ? range[0][lane] : 0u);
+  klo = sample_wave_max(lane < NT / 64 ? range[1][lane] : 0u);
+  const float zmax = sample_unkey(khi);
+  if (zmax == -INFINITY || set.greedy) {
+    unsigned first = 0;   // complement of the lowest index of the largest logit
+#pragma unroll
+    for (int j = R - 1; j >= 0; --j)
+      if (z[j] == zmax) first = ~(unsigned)(i0 + j);
+    first = sample_wave_max(first);
     __syncthreads();
-    khi = sample_wave_max(lane < NT / 64 ? range[0][lane] : 0u);
-    klo = sample_wave_max(lane < NT / 64 ? range[1][lane] : 0u);
-    const float zmax = sample_unkey(khi);
-    if (zmax == -INFINITY || set.greedy) {
-      unsigned first = 0;   // complement of the lowest index of the largest logit
-      for (int j = steps - 1; j >= 0; --j)
-        if (sample_logit(row_z, w0 + j * 64 + lane, V) == zmax) first = max(first, ~(unsigned)(w0 + j * 64 + lane));
-      first = sample_wave_max(first);
-      __syncthreads();
-      if (lane == 0) range[0][w] = first;
-      __syncthreads();
-      first = ~sample_wave_max(lane < NT / 64 ? range[0][lane] : 0u);
-      if (tid == 0) {
-        if (zmax == -INFINITY) sample_answer(a, row, -1, -INFINITY);
-        else sample_answer(a, row, (long)first, 0.f);
-      }
-      __syncthreads();
-      continue;
+    if (lane == 0) range[0][w] = first;
+    __syncthreads();
+    first = ~sample_wave_max(lane < NT / 64 ? range[0][lane] : 0u);
+    if (tid == 0) {
+      if (zmax == -INFINITY) sample_answer(a, row, -1, -INFINITY);
+      else sample_answer(a, row, (long)first, 0.f);
     }
-    const SampleMass mass(zmax, set.y, a.F);
-    float t = -INFINITY;
-    unsigned r = 0;
-    unsigned long long qt = 0;   // mass of a code at t
-    const bool by_mass = set.p < 1.0;
-    if (set.k < V || by_mass) {
-      const SampleBins bins = sample_bins(zmax, sample_unkey(~klo), set.y, kSampleBins);
-      each([&](float z) {
-        const int b = bins.of(z);
+    return;
+  }
+  const SampleMass mass(zmax, set.y, a.F);
+  unsigned long long q[R];
+  unsigned floored = 0;   // bit j: cut by min-p
+  auto weigh = [&](float least) {
+#pragma unroll
+    for (int j = 0; j < R; ++j) q[j] = 0;
+    each([&](int j, float x) {
+      if (x >= least) {
+        const double e = mass.e(x);
+        q[j] = mass.whole(e);
+        floored |= (e >= set.m ? 0u : 1u) << j;
+      }
+    });
+  };
+  float t = -INFINITY;
+  unsigned r = 0;
+  const bool by_mass = set.p < 1.0;
+  if (by_mass) weigh(-INFINITY);
+  if (set.k < V || by_mass) {
+    const SampleBins bins = sample_bins(zmax, sample_unkey(~klo), set.y, kSampleBins);
+    each([&](int j, float x) {
+      if (x > -INFINITY) {
+        const int b = bins.of(x);
         atomicAdd(&bin_count[b], 1u);
-        if (by_mass) {
-          const unsigned long long q = mass.q(z);
-          if (q) atomicAdd(&bin_mass[b], q);
+        if (by_mass && q[j]) atomicAdd(&bin_mass[b], q[j]);
+      }
+    });
+    __syncthreads();
+    unsigned long long m = 0, m_before, total;
+    unsigned c = 0, c_before, c_all;
+#pragma unroll
+    for (int j = 0; j < PB; ++j) {
+      m += bin_mass[tid * PB + j];
+      c += bin_count[tid * PB + j];
+    }
+    sample_block_scan<NT>(blk, m, c, m_before, c_before, total, c_all);
+    // codes of bin b above t into m_z, m_mass; their number
+    auto list = [&](int b, int which) {
+      each([&](int j, float x) {
+        if (x > t && bins.of(x) == b) {
+          const int to = atomicAdd(&n_listed[which], 1);
+          if (to < 64) {
+            m_z[to] = x;
+            m_mass[to] = by_mass ? q[j] : 0ull;
+          }
         }
       });
-      if (tid < 2) n_listed[tid] = 0;
       __syncthreads();
-      unsigned long long m = 0, m_before, total;
-      unsigned c = 0, c_before, c_all;
-#pragma unroll
-      for (int j = 0; j < PB; ++j) {
-        m += bin_mass[tid * PB + j];
-        c += bin_count[tid * PB + j];
+      return n_listed[which];
+    };
+    // the smallest and largest key of bin b above t
+    auto keys_of = [&](int b, unsigned& first, unsigned& last) {
+      if (tid == 0) {
+        key_range[0] = ~0u;
+        key_range[1] = 0;
       }
-      sample_block_scan<NT>(blk, m, c, m_before, c_before, total, c_all);
-      // codes of bin b above t into m_z; their number
-      auto list = [&](int b, int cut) {
-        each([&](float z) {
-          if (z > t && bins.of(z) == b) {
-            const int to = atomicAdd(&n_listed[cut], 1);
-            if (to < 64) m_z[to] = z;
+      __syncthreads();
+      unsigned l = ~0u, h = 0;
+      each([&](int j, float x) {
+        if (x > t && bins.of(x) == b) {
+          l = min(l, sample_key(x));
+          h = max(h, sample_key(x));
+        }
+      });
+      if (h) {
+        atomicMin(&key_range[0], l);
+        atomicMax(&key_range[1], h);
+      }
+      __syncthreads();
+      first = key_range[0];
+      last = key_range[1];
+    };
+    int kb = kSampleBins;                          // the bin that top-k cuts
+    unsigned long long k_above = 0, k_in = 0;      // mass before that bin, and in it above t
+    unsigned long long qt = 0;                     // mass of a code at t
+    if ((unsigned)set.k < c_all) {
+      if (c_before < (unsigned)set.k && (unsigned)set.k <= c_before + c) {
+        unsigned cr = c_before;
+        unsigned long long mr = m_before;
+#pragma unroll
+        for (int j = 0; j < PB; ++j) {
+          const unsigned n = bin_count[tid * PB + j];
+          if (cr < (unsigned)set.k && (unsigned)set.k <= cr + n) {
+            found.bin = tid * PB + j;
+            found.count = (unsigned)set.k - cr;
+            found.mass = mr;
           }
-        });
-        __syncthreads();
-        return n_listed[cut];
-      };
-      // the smallest and largest key of bin b above t
-      auto keys_of = [&](int b, unsigned& first, unsigned& last) {
-        if (tid == 0) {
-          key_range[0] = ~0u;
-          key_range[1] = 0;
+          cr += n;
+          mr += bin_mass[tid * PB + j];
+        }
+      }
+      __syncthreads();
+      kb = found.bin;
+      const unsigned want = found.count;
+      k_above = found.mass;
+      const int n = list(kb, 0);
+      if (n <= 64) {
+        if (w == 0) {
+          const float mz = lane < n ? m_z[lane] : -INFINITY;
+          unsigned gt = 0, ge = 0;
+          for (int i = 0; i < n; ++i) {
+            const float o = __uint_as_float(sample_lane(__float_as_uint(mz), i));
+            gt += o > mz;
+            ge += o >= mz;
+          }
+          const int at = __builtin_ctzll(__ballot(lane < n && gt < want && want <= ge));
+          const float z_at = __uint_as_float(sample_lane(__float_as_uint(mz), at));
+          const unsigned long long in = by_mass ? sample_wave_sum(mz > z_at ? m_mass[lane] : 0ull) : 0ull;
+          if (lane == 0) {
+            cut.t = z_at;
+            cut.r = want - sample_lane(gt, at);
+            cut.in = in;
+          }
         }
         __syncthreads();
-        unsigned l = ~0u, h = 0;
-        each([&](float z) {
-          if (z > t && bins.of(z) == b) {
-            l = min(l, sample_key(z));
-            h = max(h, sample_key(z));
-          }
+        t = cut.t;
+        r = cut.r;
+        k_in = cut.in;
+      } else {
+        unsigned first, last;
+        keys_of(kb, first, last);
+        unsigned long long before;
+        const unsigned key = sample_search<NT>(blk, found, part, first, last, want, before, [&](auto f) {
+          each([&](int j, float x) {
+            if (x > -INFINITY && bins.of(x) == kb) f(sample_key(x), [] { return 1ull; });
+          });
         });
-        if (h) {
-          atomicMin(&key_range[0], l);
-          atomicMax(&key_range[1], h);
+        t = sample_unkey(key);
+        r = want - (unsigned)before;
+        if (by_mass) {
+          unsigned long long in = 0, none;
+          unsigned none_c, none_all;
+          each([&](int j, float x) {
+            if (x > t && bins.of(x) == kb) in += q[j];
+          });
+          sample_block_scan<NT>(blk, in, 0u, none, none_c, k_in, none_all);
         }
-        __syncthreads();
-        first = key_range[0];
-        last = key_range[1];
-      };
-      int kb = kSampleBins;                          // the bin that top-k cuts
-      unsigned long long k_above = 0, k_in = 0;      // mass before that bin, and in it above t
-      if ((unsigned)set.k < c_all) {
-        if (c_before < (unsigned)set.k && (unsigned)set.k <= c_before + c) {
-          unsigned cr = c_before;
-          unsigned long long mr = m_before;
+      }
+      if (by_mass) {
+        qt = mass.q(t);
+        total = k_above + k_in + r * qt;
+      }
+    }
+    if (by_mass) {
+      const unsigned long long bound = sample_bound(set.p, total);
+      if (kb < kSampleBins && bound > k_above + k_in) {   // on the ties that top-k kept
+        r = min(r, sample_ceil_div(bound - k_above - k_in, qt));
+      } else {
+        if (m_before < bound && bound <= m_before + m) {
 #pragma unroll
           for (int j = 0; j < PB; ++j) {
-            const unsigned n = bin_count[tid * PB + j];
-            if (cr < (unsigned)set.k && (unsigned)set.k <= cr + n) {
+            const unsigned long long n = bin_mass[tid * PB + j];
+            if (m_before < bound && bound <= m_before + n) {
               found.bin = tid * PB + j;
-              found.count = (unsigned)set.k - cr;
-              found.mass = mr;
+              found.mass = m_before;
             }
-            cr += n;
-            mr += bin_mass[tid * PB + j];
+            m_before += n;
           }
         }
         __syncthreads();
-        kb = found.bin;
-        const unsigned want = found.count;
-        k_above = found.mass;
-        const int n = list(kb, 0);
+        const int pb = found.bin;
+        const unsigned long long need = bound - found.mass;
+        const int n = list(pb, 1);
         if (n <= 64) {
           if (w == 0) {
             const float mz = lane < n ? m_z[lane] : -INFINITY;
-            unsigned gt = 0, ge = 0;
+            const unsigned long long mq = lane < n ? m_mass[lane] : 0ull;
+            unsigned long long gt = 0, ge = 0;
             for (int i = 0; i < n; ++i) {
               const float o = __uint_as_float(sample_lane(__float_as_uint(mz), i));
-              gt += o > mz;
-              ge += o >= mz;
+              const unsigned long long v = sample_lane(mq, i);
+              gt += o > mz ? v : 0ull;
+              ge += o >= mz ? v : 0ull;
             }
-            const int at = __builtin_ctzll(__ballot(lane < n && gt < want && want <= ge));
-            const float z_at = __uint_as_float(sample_lane(__float_as_uint(mz), at));
-            const unsigned long long in = by_mass ? sample_wave_sum(mz > z_at ? mass.q(mz) : 0ull) : 0ull;
-            if (lane == 0) {
-              cut.t = z_at;
-              cut.r = want - sample_lane(gt, at);
-              cut.in = in;
+            const int at = __builtin_ctzll(__ballot(lane < n && gt < need && need <= ge));
+            if (lane == at) {
+              cut.t = mz;
+              cut.r = sample_ceil_div(need - gt, mq);
             }
           }
           __syncthreads();
           t = cut.t;
           r = cut.r;
-          k_in = cut.in;
         } else {
           unsigned first, last;
-          keys_of(kb, first, last);
+          keys_of(pb, first, last);
           unsigned long long before;
-          const unsigned key = sample_search<NT>(blk, found, part, first, last, want, before, [&](auto f) {
-            each([&](float z) {
-              if (bins.of(z) == kb) f(sample_key(z), [] { return 1ull; });
+          const unsigned key = sample_search<NT>(blk, found, part, first, last, need, before, [&](auto f) {
+            each([&](int j, float x) {
+              if (x > t && bins.of(x) == pb) f(sample_key(x), [&] { return q[j]; });
             });
           });
           t = sample_unkey(key);
-          r = want - (unsigned)before;
-          unsigned long long in = 0, none;
-          unsigned none_c, none_all;
-          each([&](float z) {
-            if (z > t && bins.of(z) == kb) in += mass.q(z);
-          });
-          sample_block_scan<NT>(blk, in, 0u, none, none_c, k_in, none_all);
-        }
-        qt = mass.q(t);
-        total = k_above + k_in + r * qt;
-      }
-      if (by_mass) {
-        const unsigned long long bound = sample_bound(set.p, total);
-        if (kb < kSampleBins && bound > k_above + k_in) {   // on the ties that top-k kept
-          r = min(r, sample_ceil_div(bound - k_above - k_in, qt));
-        } else {
-          if (m_before < bound && bound <= m_before + m) {
-#pragma unroll
-            for (int j = 0; j < PB; ++j) {
-              const unsigned long long n = bin_mass[tid * PB + j];
-              if (m_before < bound && bound <= m_before + n) {
-                found.bin = tid * PB + j;
-                found.mass = m_before;
-              }
-              m_before += n;
-            }
-          }
-          __syncthreads();
-          const int pb = found.bin;
-          const unsigned long long need = bound - found.mass;
-          const int n = list(pb, 1);
-          if (n <= 64) {
-            if (w == 0) {
-              const float mz = lane < n ? m_z[lane] : -INFINITY;
-              const unsigned long long mq = lane < n ? mass.q(mz) : 0ull;
-              unsigned long long gt = 0, ge = 0;
-              for (int i = 0; i < n; ++i) {
-                const float o = __uint_as_float(sample_lane(__float_as_uint(mz), i));
-                const unsigned long long q = sample_lane(mq, i);
-                gt += o > mz ? q : 0ull;
-                ge += o >= mz ? q : 0ull;
-              }
-              const int at = __builtin_ctzll(__ballot(lane < n && gt < need && need <= ge));
-              if (lane == at) {
-                cut.t = mz;
-                cut.r = sample_ceil_div(need - gt, mq);
-              }
-            }
-            __syncthreads();
-            t = cut.t;
-            r = cut.r;
-          } else {
-            unsigned first, last;
-            keys_of(pb, first, last);
-            unsigned long long before;
-            const unsigned key = sample_search<NT>(blk, found, part, first, last, need, before, [&](auto f) {
-              each([&](float z) {
-                if (z > t && bins.of(z) == pb) f(sample_key(z), [&] { return mass.q(z); });
-              });
-            });
-            t = sample_unkey(key);
-            r = sample_ceil_div(need - before, mass.q(t));
-          }
+          r = sample_ceil_div(need - before, mass.q(t));
         }
       }
-      qt = r ? mass.q(t, set.m) : 0ull;
     }
-    // kept masses, wave by wave
-    unsigned at_t = 0;
-    unsigned long long sum = 0;
-    each([&](float z) {
-      at_t += z == t && r > 0;
-      if (z > t) sum += mass.q(z, set.m);
+  }
+  if (!by_mass) weigh(t);   // (of what top-k kept alone)
+  unsigned at_t = 0;
+  unsigned long long sum = 0;
+  const unsigned long long qt = r ? mass.q(t, set.m) : 0ull;
+  each([&](int j, float x) {
+    at_t += x == t && r > 0;
+    sum += x > t && !(floored >> j & 1) ? q[j] : 0ull;
+  });
+  unsigned long long run, above;
+  unsigned seen, all_t;
+  sample_block_scan<NT>(blk, sum, at_t, run, seen, above, all_t);
+  const unsigned long long total = above + min(all_t, r) * qt, target = sample_target(set.u, total);
+  run += min(seen, r) * qt;
+  const unsigned long long here = sum + (min(seen + at_t, r) - min(seen, r)) * qt;
+  if (run <= target && target < run + here) {
+    int at = 0;
+    float z_at = 0.f;
+    bool drawn = false;
+    each([&](int j, float x) {
+      const bool tie = x == t && r > 0;
+      if (x > t && !(floored >> j & 1)) run += q[j];
+      if (tie && seen < r) run += qt;
+      seen += tie;
+      if (!drawn && run > target) {
+        drawn = true;
+        at = j;
+        z_at = x;
+      }
     });
-    at_t = sample_wave_sum(at_t);
-    sum = sample_wave_sum(sum);
-    if (lane == 0) {
-      blk.m[w] = sum;
-      blk.c[w] = at_t;
-    }
-    __syncthreads();
-    unsigned long long total = 0;
-    unsigned seen = 0;
-#pragma unroll 1
-    for (int v = 0; v < NT / 64; ++v) {
-      total += blk.m[v] + min(blk.c[v], r > seen ? r - seen : 0u) * qt;
-      seen += blk.c[v];
-    }
-    sample_draw<T, NT>(a, row, row_z, 0, steps, mass, set.m, t, r, qt, blk, 0ull, 0u, sample_target(set.u, total), total);
-    __syncthreads();
+    sample_answer(a, row, i0 + at, mass.logp(z_at, total));
   }
 }
 

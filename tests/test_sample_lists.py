@@ -159,11 +159,12 @@ SETTINGS = [dict(), dict(T=0.7, k=5), dict(p=0.9), dict(m=0.05), dict(T=1.3, k=5
 @gpu
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("n,V", [(1, 1), (3, 2), (5, 63), (4, 64), (4, 65), (300, 256), (7, 257), (9, 512), (9, 513), (3, 1000), (5, 1024), (5, 1025), (6, 4099),
-                                 (2, 10240), (2, 10241), (2, 16384), (2, 16385), (2, 32769), (2, 70001), (1, (1 << 20) + 3)])
+                                 (2, 2048), (2, 6145), (2, 10240), (2, 10241), (2, 16385), (2, 20480), (2, 20481), (2, 32769), (2, 70001), (1, (1 << 20) + 3),
+                                 (257, 1025), (257, 2049), (257, 5121), (257, 10241)])
 def test_sample_sizes_and_settings(dtype, n, V):
     import torch
     g = torch.Generator("cuda").manual_seed(n * 1000003 + V)
-    for i, s in enumerate(SETTINGS if V < 100000 else SETTINGS[:5]):
+    for i, s in enumerate(SETTINGS if n * V < 100000 else SETTINGS[:5]):
         z = (torch.randn(n, V, generator=g, device="cuda") * 2.5).to(getattr(torch, dtype))
         check_sample(z, torch.rand(n, generator=g, device="cuda"), **s)
 
@@ -173,7 +174,7 @@ def test_sample_masks_infinities_nan_and_ties():
     import torch
     g = torch.Generator("cuda").manual_seed(5)
     inf, low = float("inf"), torch.finfo(torch.float32).min
-    for V in (2, 64, 200, 256, 1500, 40000):
+    for V, rep in ((2, 1), (64, 1), (200, 1), (256, 1), (500, 1), (900, 1), (1500, 1), (1500, 7), (4000, 7), (5001, 1), (6000, 7), (11000, 1), (40000, 1)):
         z = torch.randn(40, V, generator=g, device="cuda")
         z[0] = -inf                                    # nothing left
         z[1] = float("nan")
@@ -198,8 +199,9 @@ def test_sample_masks_infinities_nan_and_ties():
         z[15] = -torch.arange(V, device="cuda").float()
         z[16:24] = torch.randint(-2, 3, (8, V), generator=g, device="cuda").float()
         z[24:28, : V // 2] = -inf
-        for s in SETTINGS:
-            u = torch.rand(40, generator=g, device="cuda")
+        z = z.repeat(rep, 1)                           # (more rows than a card has CUs go another way)
+        for s in SETTINGS if rep == 1 else SETTINGS[:5]:
+            u = torch.rand(40 * rep, generator=g, device="cuda")
             u[20:24] = torch.tensor([0.0, 1.0 - 2.0 ** -24, 0.5, 2.0 ** -30])
             check_sample(z, u, **s)
 
@@ -255,7 +257,7 @@ def hard_rows(V, g):
 
 
 @gpu
-@pytest.mark.parametrize("V", [60, 200, 500, 1024, 3000, 10240, 70001, 300001])
+@pytest.mark.parametrize("V", [60, 200, 500, 1024, 2000, 3000, 10240, 20480, 70001, 300001])
 def test_sample_rows_that_pile_up_in_a_few_bins(V):
     import torch
     g = torch.Generator("cuda").manual_seed(V)
