@@ -111,38 +111,47 @@ static int launch_sample_long(const SampleArgs& a, const SamplePlan& p, char* ws
   return QINCO_OK;
 }
 
+// f(workgroups, first row): launches of `rows` rows per workgroup of `threads`, each of fewer than 2^32 threads.  (A loop over rows inside the
+// kernels would have the compiler take what all rows share out of it, into registers that the rows' own values need.)
+template <typename F>
+static void sample_launches(int64_t n, int rows, int threads, F f) {
+  const int64_t most = ((int64_t)1 << 31) / threads * rows;
+  for (int64_t r0 = 0; r0 < n; r0 += most) f(dim3((unsigned)(((n - r0 < most ? n - r0 : most) + rows - 1) / rows)), (long)r0);
+}
+
 template <typename T, int R>
 static void launch_sample_wave(const SampleArgs& a, hipStream_t st) {
-  long g = (a.n + kSampleRowWaves - 1) / kSampleRowWaves;
-  if (g > 1 << 20) g = 1 << 20;
-  hipLaunchKernelGGL((sample_wave_kernel<T, R>), dim3((unsigned)g), dim3(64 * kSampleRowWaves), 0, st, a);
+  sample_launches(a.n, kSampleRowWaves, 64 * kSampleRowWaves, [&](dim3 grid, long r0) {
+    hipLaunchKernelGGL((sample_wave_kernel<T, R>), grid, dim3(64 * kSampleRowWaves), 0, st, a, r0);
+  });
 }
 
 template <typename T, int G, int R>
 static void launch_sample_group(const SampleArgs& a, hipStream_t st) {
-  constexpr int ROWS = kSampleGroupThreads / G;
-  long g = (a.n + ROWS - 1) / ROWS;
-  if (g > 1 << 20) g = 1 << 20;
-  hipLaunchKernelGGL((sample_group_kernel<T, G, R>), dim3((unsigned)g), dim3(kSampleGroupThreads), 0, st, a);
+  sample_launches(a.n, kSampleGroupThreads / G, kSampleGroupThreads, [&](dim3 grid, long r0) {
+    hipLaunchKernelGGL((sample_group_kernel<T, G, R>), grid, dim3(kSampleGroupThreads), 0, st, a, r0);
+  });
 }
 
 template <typename T, int NT, int R>
 static void launch_sample_block(const SampleArgs& a, hipStream_t st) {
-  constexpr long MOST = 1 << 21;   // (threads of a launch: below 2^32)
-  for (long r0 = 0; r0 < a.n; r0 += MOST)
-    hipLaunchKernelGGL((sample_block_kernel<T, NT, R>), dim3((unsigned)(a.n - r0 < MOST ? a.n - r0 : MOST)), dim3(NT), 0, st, a, r0);
+  sample_launches(a.n, 1, NT, [&](dim3 grid, long r0) { hipLaunchKernelGGL((sample_block_kernel<T, NT, R>), grid, dim3(NT), 0, st, a, r0); });
 }
 
-// By the length of a row, and above 1024 codes by whether there is a CU for every row: then more threads share one (a row's code depends on
-// neither).  Each border with both sides measured, all three cuts on, fp32: 65536 rows of 64 27 us with 16 lanes each, 52 with 64; 65536 of 256
-// (bf16) 89 us with 32 lanes, 107 with 64; 16384 of 512 40 us with a wave each, 75 with four, of 520 86 and 85; 8000 of 2000 70 us with 8
-// codes per thread, 83 with 20; of 4099 127 us with 256 threads, 171 with 512; of 10240 274 with 512 threads, 384 with 256, 435 with 1024; one
-// row of 20480 19 us with a workgroup, 44 split over several, 1000 of them 87 and 216.  One row of 2000 7.5 us with 512 threads, 9.0 with 256,
-// 300 of them 9.7 and 9.4; one of 4099 10.2 and 13.6; one of 10240 13.7 with 1024 threads, 15.0 with 512, 300 of them 27 and 21.
+// By the length of a row, and where the rows alone do not fill the card with more lanes to each (a row's code depends on neither).  Each
+// border with both sides measured, all three cuts on, fp32.  65536 rows of 64 23 us with 16 lanes each; of 128 36 us with 16 lanes, 65 with 32;
+// of 256 67 us with 32, 78 with 64.  With a wave each or fewer lanes, one row of 128 or 256 4.7 and 6.4 us, 2048 rows of 256 6.7 and 7.8, 4096
+// 8.9 and 8.6; 2048 of 128 6.3 and 7.7, 8192 12.5 and 8.6.  16384 of 512 36 us with a wave each, 75 with four, of 520 86 and 85; 8000 of 2000
+// 70 us with 8 codes per thread, 83 with 20; of 4099 127 us with 256 threads, 171 with 512; of 10240 274 with 512 threads, 384 with 256, 435
+// with 1024; one row of 20480 19 us with a workgroup, 44 split over several, 1000 of them 87 and 216.  One row of 2000 7.5 us with 512
+// threads, 9.0 with 256, 300 of them 9.7 and 9.4; one of 4099 10.2 and 13.6; one of 10240 13.7 with 1024 threads, 15.0 with 512, 300 of them
+// 27 and 21.
 template <typename T>
 static int launch_sample(const SampleArgs& a, const SamplePlan& p, char* ws, hipStream_t st) {
   if (a.V > kSampleLongV) return launch_sample_long<T>(a, p, ws, st);
   if (a.V <= 64) launch_sample_group<T, 16, 4>(a, st);
+  else if (a.n <= 8 * kCUs && a.V <= 256) launch_sample_wave<T, 4>(a, st);   // (two waves per SIMD)
+  else if (a.V <= 128) launch_sample_group<T, 16, 8>(a, st);
   else if (a.V <= 256) launch_sample_group<T, 32, 8>(a, st);
   else if (a.V <= 512) launch_sample_wave<T, 8>(a, st);
   else if (a.V <= 256 * 4) launch_sample_block<T, 256, 4>(a, st);

@@ -281,279 +281,279 @@ __device__ __forceinline__ unsigned sample_row_max(unsigned v) {
 }
 
 template <typename T, int G, int R>
-__global__ void __launch_bounds__(kSampleGroupThreads) sample_group_kernel(SampleArgs a) {
+__global__ void __launch_bounds__(kSampleGroupThreads) sample_group_kernel(SampleArgs a, long row0) {
   constexpr int ROWS = kSampleGroupThreads / G, PB = 64 / G;   // rows of a workgroup, bins of a lane
   __shared__ SampleGroupLds lds[ROWS];
   SampleGroupLds& s = lds[threadIdx.x / G];
   const int l = threadIdx.x % G, V = a.V, row_shift = (threadIdx.x & 63) / G * G;
   // lanes of this row among a ballot's
   auto mine = [&](unsigned long long ballot) { return (unsigned)(ballot >> row_shift) & (unsigned)((1ull << G) - 1); };
-  // (a row's lanes take every branch together: the loop and the branches below may part rows, never a row)
-  for (long row = (long)blockIdx.x * ROWS + threadIdx.x / G; row < a.n; row += (long)gridDim.x * ROWS) {
-    const T* logits = reinterpret_cast<const T*>(a.logits) + row * a.stride;
-    const SampleRow set = sample_row(a, row);
-    float z[R];
-    {
-      constexpr int U = R * sizeof(T) < 16 ? R : 16 / sizeof(T);   // codes of one load
-      struct alignas(sizeof(T)) Raw { T v[U]; };
+  // (a row's lanes take every branch together: the branches below may part rows, never a row)
+  const long row = row0 + (long)blockIdx.x * ROWS + threadIdx.x / G;
+  if (row >= a.n) return;
+  const T* logits = reinterpret_cast<const T*>(a.logits) + row * a.stride;
+  const SampleRow set = sample_row(a, row);
+  float z[R];
+  {
+    constexpr int U = R * sizeof(T) < 16 ? R : 16 / sizeof(T);   // codes of one load
+    struct alignas(sizeof(T)) Raw { T v[U]; };
 #pragma unroll
-      for (int j = 0; j < R; j += U) {
-        const int i = l * R + j;
-        if (i + U <= V) {
-          const Raw raw = *reinterpret_cast<const Raw*>(logits + i);
+    for (int j = 0; j < R; j += U) {
+      const int i = l * R + j;
+      if (i + U <= V) {
+        const Raw raw = *reinterpret_cast<const Raw*>(logits + i);
 #pragma unroll
-          for (int e = 0; e < U; ++e) {
-            const float x = GroupNum<T>::get(raw.v[e]);
-            z[j + e] = x == x ? x : -INFINITY;
+        for (int e = 0; e < U; ++e) {
+          const float x = GroupNum<T>::get(raw.v[e]);
+          z[j + e] = x == x ? x : -INFINITY;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < U; ++e) z[j + e] = sample_logit(logits, i + e, V);
+      }
+    }
+  }
+  float hi = z[0], lo = INFINITY;
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    hi = fmaxf(hi, z[j]);
+    lo = fminf(lo, z[j] > -INFINITY ? z[j] : INFINITY);
+  }
+  const float zmax = sample_unkey(sample_row_max<G>(sample_key(hi)));
+  if (zmax == -INFINITY) {
+    if (l == 0) sample_answer(a, row, -1, -INFINITY);
+    return;
+  }
+  if (set.greedy) {
+    const int first = __builtin_ctz(mine(__ballot(hi == zmax)));
+    int at = 0;
+#pragma unroll
+    for (int j = R - 1; j >= 0; --j) at = z[j] == zmax ? j : at;
+    if (l == first) sample_answer(a, row, l * R + at, 0.f);
+    return;
+  }
+  const SampleMass mass(zmax, set.y, a.F);
+  unsigned long long q[R];
+  unsigned floored = 0;   // bit j: cut by min-p
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const double e = mass.e(z[j]);
+    q[j] = mass.whole(e);
+    floored |= (e >= set.m ? 0u : 1u) << j;
+    if ((j & 1) == 1) __builtin_amdgcn_sched_barrier(0);   // (two exponentials at a time: more side by side only take registers)
+  }
+  float t = -INFINITY;
+  unsigned r = 0;
+  const bool by_count = set.k < V, by_mass = set.p < 1.0;
+  if (by_count || by_mass) {
+    const float zmin = sample_unkey(~sample_row_max<G>(~sample_key(lo)));
+    const SampleBins bins = sample_bins(zmax, zmin, set.y, 64);
+#pragma unroll
+    for (int j = 0; j < PB; ++j) {
+      s.mass[l * PB + j] = 0;
+      s.count[l * PB + j] = 0;
+    }
+    sample_wave_sync();
+#pragma unroll
+    for (int j = 0; j < R; ++j) {
+      const int b = bins.of(z[j]);
+      if (z[j] > -INFINITY) atomicAdd(&s.count[b], 1u);
+      if (q[j]) atomicAdd(&s.mass[b], q[j]);
+    }
+    sample_wave_sync();
+    unsigned c_in[PB], c_sum = 0;
+    unsigned long long m_in[PB], m_sum = 0;
+#pragma unroll
+    for (int j = 0; j < PB; ++j) {
+      c_sum += c_in[j] = s.count[l * PB + j];
+      m_sum += m_in[j] = s.mass[l * PB + j];
+    }
+    const unsigned c_run = sample_row_scan<G>(c_sum), c_all = sample_row_last<G>(c_run);
+    const unsigned long long m_run = sample_row_scan<G>(m_sum);
+    unsigned long long total = sample_row_last<G>(m_run);   // mass of what top-k keeps
+    // codes of bin b into m_z, m_mass; their number
+    auto members = [&](int b) {
+      unsigned in = 0;
+#pragma unroll
+      for (int j = 0; j < R; ++j) in |= (unsigned)(z[j] > -INFINITY && bins.of(z[j]) == b) << j;
+      const unsigned n = __builtin_popcount(in), run = sample_row_scan<G>(n);
+      unsigned to = run - n;
+      if (in) {
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+          if (in >> j & 1) {
+            if (to < 64) {
+              s.m_z[to] = z[j];
+              s.m_mass[to] = q[j];
+            }
+            ++to;
           }
-        } else {
-#pragma unroll
-          for (int e = 0; e < U; ++e) z[j + e] = sample_logit(logits, i + e, V);
         }
       }
-    }
-    float hi = z[0], lo = INFINITY;
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-      hi = fmaxf(hi, z[j]);
-      lo = fminf(lo, z[j] > -INFINITY ? z[j] : INFINITY);
-    }
-    const float zmax = sample_unkey(sample_row_max<G>(sample_key(hi)));
-    if (zmax == -INFINITY) {
-      if (l == 0) sample_answer(a, row, -1, -INFINITY);
-      continue;
-    }
-    if (set.greedy) {
-      const int first = __builtin_ctz(mine(__ballot(hi == zmax)));
-      int at = 0;
-#pragma unroll
-      for (int j = R - 1; j >= 0; --j) at = z[j] == zmax ? j : at;
-      if (l == first) sample_answer(a, row, l * R + at, 0.f);
-      continue;
-    }
-    const SampleMass mass(zmax, set.y, a.F);
-    unsigned long long q[R];
-    unsigned floored = 0;   // bit j: cut by min-p
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-      const double e = mass.e(z[j]);
-      q[j] = mass.whole(e);
-      floored |= (e >= set.m ? 0u : 1u) << j;
-      if ((j & 1) == 1) __builtin_amdgcn_sched_barrier(0);   // (two exponentials at a time: more side by side only take registers)
-    }
-    float t = -INFINITY;
-    unsigned r = 0;
-    const bool by_count = set.k < V, by_mass = set.p < 1.0;
-    if (by_count || by_mass) {
-      const float zmin = sample_unkey(~sample_row_max<G>(~sample_key(lo)));
-      const SampleBins bins = sample_bins(zmax, zmin, set.y, 64);
-#pragma unroll
-      for (int j = 0; j < PB; ++j) {
-        s.mass[l * PB + j] = 0;
-        s.count[l * PB + j] = 0;
-      }
       sample_wave_sync();
+      return (int)sample_row_last<G>(run);
+    };
+    int kb = 64, n_kb = 0;        // the bin that top-k cuts, 64: none; its codes
+    unsigned long long qt = 0;    // mass of a code at t
+    if (by_count && (unsigned)set.k < c_all) {
+      unsigned want = (unsigned)set.k - (c_run - c_sum);
+      unsigned long long above = m_run - m_sum;
+      int b = l * PB;
 #pragma unroll
-      for (int j = 0; j < R; ++j) {
-        const int b = bins.of(z[j]);
-        if (z[j] > -INFINITY) atomicAdd(&s.count[b], 1u);
-        if (q[j]) atomicAdd(&s.mass[b], q[j]);
+      for (int j = 0; j < PB - 1; ++j) {
+        const bool on = b == l * PB + j && want > c_in[j];
+        want -= on ? c_in[j] : 0;
+        above += on ? m_in[j] : 0;
+        b += on;
       }
-      sample_wave_sync();
-      unsigned c_in[PB], c_sum = 0;
-      unsigned long long m_in[PB], m_sum = 0;
-#pragma unroll
-      for (int j = 0; j < PB; ++j) {
-        c_sum += c_in[j] = s.count[l * PB + j];
-        m_sum += m_in[j] = s.mass[l * PB + j];
-      }
-      const unsigned c_run = sample_row_scan<G>(c_sum), c_all = sample_row_last<G>(c_run);
-      const unsigned long long m_run = sample_row_scan<G>(m_sum);
-      unsigned long long total = sample_row_last<G>(m_run);   // mass of what top-k keeps
-      // codes of bin b into m_z, m_mass; their number
-      auto members = [&](int b) {
-        unsigned in = 0;
-#pragma unroll
-        for (int j = 0; j < R; ++j) in |= (unsigned)(z[j] > -INFINITY && bins.of(z[j]) == b) << j;
-        const unsigned n = __builtin_popcount(in), run = sample_row_scan<G>(n);
-        unsigned to = run - n;
-        if (in) {
-#pragma unroll
-          for (int j = 0; j < R; ++j) {
-            if (in >> j & 1) {
-              if (to < 64) {
-                s.m_z[to] = z[j];
-                s.m_mass[to] = q[j];
-              }
-              ++to;
-            }
+      const int src = __builtin_ctz(mine(__ballot(c_run >= (unsigned)set.k)));
+      want = __shfl(want, src, G);
+      above = __shfl(above, src, G);
+      kb = __shfl(b, src, G);
+      n_kb = members(kb);
+      if (n_kb <= 64) {
+        for (int i = l; i < n_kb; i += G) {
+          const float mz = s.m_z[i];
+          unsigned gt = 0, ge = 0;
+          for (int o = 0; o < n_kb; ++o) {
+            gt += s.m_z[o] > mz;
+            ge += s.m_z[o] >= mz;
+          }
+          if (gt < want && want <= ge) {   // (equal logits find the same)
+            s.t = mz;
+            s.r = want - gt;
+            s.q = s.m_mass[i];
           }
         }
         sample_wave_sync();
-        return (int)sample_row_last<G>(run);
-      };
-      int kb = 64, n_kb = 0;        // the bin that top-k cuts, 64: none; its codes
-      unsigned long long qt = 0;    // mass of a code at t
-      if (by_count && (unsigned)set.k < c_all) {
-        unsigned want = (unsigned)set.k - (c_run - c_sum);
-        unsigned long long above = m_run - m_sum;
-        int b = l * PB;
+        t = s.t;
+        r = s.r;
+        qt = s.q;
+        unsigned long long in = 0;
+        if (by_mass)
+          for (int i = l; i < n_kb; i += G) in += s.m_z[i] > t ? s.m_mass[i] : 0ull;
+        total = above + sample_row_sum<G>(in) + r * qt;
+      } else {   // the largest t that at least k codes reach, a bit at a time
+        unsigned key = 0;
+        for (int b = 31; b >= 0; --b) {
+          const unsigned c = key | 1u << b;
+          unsigned n = 0;
 #pragma unroll
-        for (int j = 0; j < PB - 1; ++j) {
-          const bool on = b == l * PB + j && want > c_in[j];
-          want -= on ? c_in[j] : 0;
-          above += on ? m_in[j] : 0;
-          b += on;
+          for (int j = 0; j < R; ++j) n += sample_key(z[j]) >= c;
+          if (sample_row_sum<G>(n) >= (unsigned)set.k) key = c;
         }
-        const int src = __builtin_ctz(mine(__ballot(c_run >= (unsigned)set.k)));
-        want = __shfl(want, src, G);
-        above = __shfl(above, src, G);
-        kb = __shfl(b, src, G);
-        n_kb = members(kb);
-        if (n_kb <= 64) {
-          for (int i = l; i < n_kb; i += G) {
-            const float mz = s.m_z[i];
-            unsigned gt = 0, ge = 0;
-            for (int o = 0; o < n_kb; ++o) {
-              gt += s.m_z[o] > mz;
-              ge += s.m_z[o] >= mz;
+        t = sample_unkey(key);
+        unsigned n = 0;
+        unsigned long long m = 0;
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+          n += z[j] > t;
+          m += z[j] > t ? q[j] : 0ull;
+        }
+        r = (unsigned)set.k - sample_row_sum<G>(n);
+        qt = mass.q(t);
+        total = sample_row_sum<G>(m) + r * qt;
+      }
+    }
+    if (by_mass) {
+      const unsigned long long bound = sample_bound(set.p, total);
+      // (a bin that top-k cuts counts as reached: what it keeps of it is in `total`)
+      unsigned long long need = bound - (m_run - m_sum);
+      int b = l * PB;
+#pragma unroll
+      for (int j = 0; j < PB - 1; ++j) {
+        const bool on = b == l * PB + j && need > m_in[j];
+        need -= on ? m_in[j] : 0;
+        b += on;
+      }
+      const int src = __builtin_ctz(mine(__ballot(m_run >= bound)));
+      need = __shfl(need, src, G);
+      const int pb = __shfl(b, src, G);
+      const int n = pb == kb ? n_kb : members(pb);
+      if (n <= 64) {
+        s.r = 0;
+        sample_wave_sync();
+        unsigned long long in = 0;
+        for (int i = l; i < n; i += G) {
+          const float mz = s.m_z[i];
+          if (mz > t) {
+            const unsigned long long mq = s.m_mass[i];
+            unsigned long long gt = 0, eq = 0;
+            for (int o = 0; o < n; ++o) {
+              const float x = s.m_z[o];
+              const unsigned long long m = s.m_mass[o];
+              gt += x > mz ? m : 0ull;
+              eq += x == mz ? m : 0ull;
             }
-            if (gt < want && want <= ge) {   // (equal logits find the same)
+            if (gt < need && need <= gt + eq) {
               s.t = mz;
-              s.r = want - gt;
-              s.q = s.m_mass[i];
+              s.r = sample_ceil_div(need - gt, mq);
             }
+            in += mq;
           }
-          sample_wave_sync();
+        }
+        sample_wave_sync();
+        if (s.r) {
           t = s.t;
           r = s.r;
-          qt = s.q;
-          unsigned long long in = 0;
-          if (by_mass)
-            for (int i = l; i < n_kb; i += G) in += s.m_z[i] > t ? s.m_mass[i] : 0ull;
-          total = above + sample_row_sum<G>(in) + r * qt;
-        } else {   // the largest t that at least k codes reach, a bit at a time
-          unsigned key = 0;
-          for (int b = 31; b >= 0; --b) {
-            const unsigned c = key | 1u << b;
-            unsigned n = 0;
-#pragma unroll
-            for (int j = 0; j < R; ++j) n += sample_key(z[j]) >= c;
-            if (sample_row_sum<G>(n) >= (unsigned)set.k) key = c;
-          }
-          t = sample_unkey(key);
-          unsigned n = 0;
+        } else {   // on the ties that top-k kept
+          r = min(r, sample_ceil_div(need - sample_row_sum<G>(in), qt));
+        }
+      } else {
+        const unsigned kt = sample_key(t);
+        const unsigned long long at_t = r * qt;
+        unsigned key = 0;
+        for (int b = 31; b >= 0; --b) {
+          const unsigned c = key | 1u << b;
           unsigned long long m = 0;
 #pragma unroll
-          for (int j = 0; j < R; ++j) {
-            n += z[j] > t;
-            m += z[j] > t ? q[j] : 0ull;
-          }
-          r = (unsigned)set.k - sample_row_sum<G>(n);
-          qt = mass.q(t);
-          total = sample_row_sum<G>(m) + r * qt;
+          for (int j = 0; j < R; ++j) m += sample_key(z[j]) >= c && z[j] > t ? q[j] : 0ull;
+          if (sample_row_sum<G>(m) + (kt >= c ? at_t : 0ull) >= bound) key = c;
         }
-      }
-      if (by_mass) {
-        const unsigned long long bound = sample_bound(set.p, total);
-        // (a bin that top-k cuts counts as reached: what it keeps of it is in `total`)
-        unsigned long long need = bound - (m_run - m_sum);
-        int b = l * PB;
+        const float x = sample_unkey(key);
+        unsigned long long m = 0;
 #pragma unroll
-        for (int j = 0; j < PB - 1; ++j) {
-          const bool on = b == l * PB + j && need > m_in[j];
-          need -= on ? m_in[j] : 0;
-          b += on;
-        }
-        const int src = __builtin_ctz(mine(__ballot(m_run >= bound)));
-        need = __shfl(need, src, G);
-        const int pb = __shfl(b, src, G);
-        const int n = pb == kb ? n_kb : members(pb);
-        if (n <= 64) {
-          s.r = 0;
-          sample_wave_sync();
-          unsigned long long in = 0;
-          for (int i = l; i < n; i += G) {
-            const float mz = s.m_z[i];
-            if (mz > t) {
-              const unsigned long long mq = s.m_mass[i];
-              unsigned long long gt = 0, eq = 0;
-              for (int o = 0; o < n; ++o) {
-                const float x = s.m_z[o];
-                const unsigned long long m = s.m_mass[o];
-                gt += x > mz ? m : 0ull;
-                eq += x == mz ? m : 0ull;
-              }
-              if (gt < need && need <= gt + eq) {
-                s.t = mz;
-                s.r = sample_ceil_div(need - gt, mq);
-              }
-              in += mq;
-            }
-          }
-          sample_wave_sync();
-          if (s.r) {
-            t = s.t;
-            r = s.r;
-          } else {   // on the ties that top-k kept
-            r = min(r, sample_ceil_div(need - sample_row_sum<G>(in), qt));
-          }
-        } else {
-          const unsigned kt = sample_key(t);
-          const unsigned long long at_t = r * qt;
-          unsigned key = 0;
-          for (int b = 31; b >= 0; --b) {
-            const unsigned c = key | 1u << b;
-            unsigned long long m = 0;
-#pragma unroll
-            for (int j = 0; j < R; ++j) m += sample_key(z[j]) >= c && z[j] > t ? q[j] : 0ull;
-            if (sample_row_sum<G>(m) + (kt >= c ? at_t : 0ull) >= bound) key = c;
-          }
-          const float x = sample_unkey(key);
-          unsigned long long m = 0;
-#pragma unroll
-          for (int j = 0; j < R; ++j) m += z[j] > x && z[j] > t ? q[j] : 0ull;
-          const unsigned rr = sample_ceil_div(bound - sample_row_sum<G>(m) - (kt > key ? at_t : 0ull), mass.q(x));
-          r = key == kt ? min(r, rr) : rr;
-          t = x;
-        }
+        for (int j = 0; j < R; ++j) m += z[j] > x && z[j] > t ? q[j] : 0ull;
+        const unsigned rr = sample_ceil_div(bound - sample_row_sum<G>(m) - (kt > key ? at_t : 0ull), mass.q(x));
+        r = key == kt ? min(r, rr) : rr;
+        t = x;
       }
     }
-    // the draw: kept masses summed in index order
-    unsigned nth = 0;
-    if (r) {
-      unsigned ties = 0;
+  }
+  // the draw: kept masses summed in index order
+  unsigned nth = 0;
+  if (r) {
+    unsigned ties = 0;
 #pragma unroll
-      for (int j = 0; j < R; ++j) ties += z[j] == t;
-      nth = sample_row_scan<G>(ties) - ties;
-    }
-    unsigned long long sum = 0;
+    for (int j = 0; j < R; ++j) ties += z[j] == t;
+    nth = sample_row_scan<G>(ties) - ties;
+  }
+  unsigned long long sum = 0;
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const bool tie = z[j] == t;
+    const bool kept = (z[j] > t || (tie && nth < r)) && !(floored >> j & 1);
+    nth += tie;
+    q[j] = kept ? q[j] : 0ull;
+    sum += q[j];
+  }
+  const unsigned long long run = sample_row_scan<G>(sum), total = sample_row_last<G>(run);
+  const unsigned long long target = sample_target(set.u, total);
+  if (run > target && run - sum <= target) {
+    unsigned long long upto = run - sum;
+    int at = 0;
+    float x = 0.f;
+    bool found = false;
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      const bool tie = z[j] == t;
-      const bool kept = (z[j] > t || (tie && nth < r)) && !(floored >> j & 1);
-      nth += tie;
-      q[j] = kept ? q[j] : 0ull;
-      sum += q[j];
-    }
-    const unsigned long long run = sample_row_scan<G>(sum), total = sample_row_last<G>(run);
-    const unsigned long long target = sample_target(set.u, total);
-    if (run > target && run - sum <= target) {
-      unsigned long long upto = run - sum;
-      int at = 0;
-      float x = 0.f;
-      bool found = false;
-#pragma unroll
-      for (int j = 0; j < R; ++j) {
-        upto += q[j];
-        if (!found && upto > target) {
-          found = true;
-          at = j;
-          x = z[j];
-        }
+      upto += q[j];
+      if (!found && upto > target) {
+        found = true;
+        at = j;
+        x = z[j];
       }
-      sample_answer(a, row, l * R + at, mass.logp(x, total));
     }
+    sample_answer(a, row, l * R + at, mass.logp(x, total));
   }
 }
 
@@ -595,193 +595,193 @@ struct SampleWaveRow {
 };
 
 template <typename T, int R>
-__global__ void __launch_bounds__(64 * kSampleRowWaves) sample_wave_kernel(SampleArgs a) {
+__global__ void __launch_bounds__(64 * kSampleRowWaves) sample_wave_kernel(SampleArgs a, long row0) {
   __shared__ SampleWaveLds lds[kSampleRowWaves];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // (known to be the same in every lane: the row's settings are scalars)
   SampleWaveLds& s = lds[wave];
   const int lane = threadIdx.x & 63, V = a.V;
-  for (long row = (long)blockIdx.x * kSampleRowWaves + wave; row < a.n; row += (long)gridDim.x * kSampleRowWaves) {
-    const T* logits = reinterpret_cast<const T*>(a.logits) + row * a.stride;
-    const SampleRow set = sample_row(a, row);
-    SampleWaveRow<R> w;
-    float hi = -INFINITY, lo = INFINITY;
+  const long row = row0 + (long)blockIdx.x * kSampleRowWaves + wave;
+  if (row >= a.n) return;
+  const T* logits = reinterpret_cast<const T*>(a.logits) + row * a.stride;
+  const SampleRow set = sample_row(a, row);
+  SampleWaveRow<R> w;
+  float hi = -INFINITY, lo = INFINITY;
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    w.z[j] = sample_logit(logits, lane * R + j, V);
+    hi = fmaxf(hi, w.z[j]);
+    lo = fminf(lo, w.z[j] > -INFINITY ? w.z[j] : INFINITY);
+  }
+  const float zmax = sample_unkey(sample_wave_max(sample_key(hi)));
+  if (zmax == -INFINITY) {
+    if (lane == 0) sample_answer(a, row, -1, -INFINITY);
+    return;
+  }
+  if (set.greedy) {
+    const int first = __builtin_ctzll(__ballot(hi == zmax));
+    int at = 0;
+#pragma unroll
+    for (int j = R - 1; j >= 0; --j) at = w.z[j] == zmax ? j : at;
+    if (lane == first) sample_answer(a, row, lane * R + at, 0.f);
+    return;
+  }
+  const SampleMass mass(zmax, set.y, a.F);
+  unsigned floored = 0;   // bit j: cut by min-p
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const double e = mass.e(w.z[j]);
+    w.q[j] = mass.whole(e);
+    floored |= (e >= set.m ? 0u : 1u) << j;
+    if ((j & 3) == 3) __builtin_amdgcn_sched_barrier(0);   // (four exponentials at a time: more side by side only take registers)
+  }
+  float t = -INFINITY;
+  unsigned r = 0;
+  const bool by_count = set.k < V, by_mass = set.p < 1.0;
+  if (by_count || by_mass) {
+    const float zmin = sample_unkey(~sample_wave_max(~sample_key(lo)));
+    const SampleBins bins = sample_bins(zmax, zmin, set.y, 64);
+    s.mass[lane] = 0;
+    s.count[lane] = 0;
+    sample_wave_sync();
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      w.z[j] = sample_logit(logits, lane * R + j, V);
-      hi = fmaxf(hi, w.z[j]);
-      lo = fminf(lo, w.z[j] > -INFINITY ? w.z[j] : INFINITY);
-    }
-    const float zmax = sample_unkey(sample_wave_max(sample_key(hi)));
-    if (zmax == -INFINITY) {
-      if (lane == 0) sample_answer(a, row, -1, -INFINITY);
-      continue;
-    }
-    if (set.greedy) {
-      const int first = __builtin_ctzll(__ballot(hi == zmax));
-      int at = 0;
-#pragma unroll
-      for (int j = R - 1; j >= 0; --j) at = w.z[j] == zmax ? j : at;
-      if (lane == first) sample_answer(a, row, lane * R + at, 0.f);
-      continue;
-    }
-    const SampleMass mass(zmax, set.y, a.F);
-    unsigned floored = 0;   // bit j: cut by min-p
-#pragma unroll
-    for (int j = 0; j < R; ++j) {
-      const double e = mass.e(w.z[j]);
-      w.q[j] = mass.whole(e);
-      floored |= (e >= set.m ? 0u : 1u) << j;
-      if ((j & 3) == 3) __builtin_amdgcn_sched_barrier(0);   // (four exponentials at a time: more side by side only take registers)
-    }
-    float t = -INFINITY;
-    unsigned r = 0;
-    const bool by_count = set.k < V, by_mass = set.p < 1.0;
-    if (by_count || by_mass) {
-      const float zmin = sample_unkey(~sample_wave_max(~sample_key(lo)));
-      const SampleBins bins = sample_bins(zmax, zmin, set.y, 64);
-      s.mass[lane] = 0;
-      s.count[lane] = 0;
-      sample_wave_sync();
-#pragma unroll
-      for (int j = 0; j < R; ++j) {
-        if (w.z[j] > -INFINITY) {
-          const int b = bins.of(w.z[j]);
-          atomicAdd(&s.count[b], 1u);
-          atomicAdd(&s.mass[b], w.q[j]);
-        }
+      if (w.z[j] > -INFINITY) {
+        const int b = bins.of(w.z[j]);
+        atomicAdd(&s.count[b], 1u);
+        atomicAdd(&s.mass[b], w.q[j]);
       }
+    }
+    sample_wave_sync();
+    const unsigned c_in = s.count[lane], c_run = sample_wave_scan(c_in);
+    const unsigned long long m_in = s.mass[lane], m_run = sample_wave_scan(m_in);
+    unsigned long long total = sample_lane(m_run, 63);   // mass of what top-k keeps
+    int kb = 64;                                         // the bin that top-k cuts, 64: none
+    int n_kb = 0;
+    unsigned long long qt = 0;                           // mass of a code at t
+    if (by_count && (unsigned)set.k < sample_lane(c_run, 63)) {
+      kb = __builtin_ctzll(__ballot(c_run >= (unsigned)set.k));
+      const unsigned want = (unsigned)set.k - (sample_lane(c_run, kb) - sample_lane(c_in, kb));
+      const unsigned long long above = sample_lane(m_run, kb) - sample_lane(m_in, kb);
+      n_kb = w.members(s, bins, kb);
       sample_wave_sync();
-      const unsigned c_in = s.count[lane], c_run = sample_wave_scan(c_in);
-      const unsigned long long m_in = s.mass[lane], m_run = sample_wave_scan(m_in);
-      unsigned long long total = sample_lane(m_run, 63);   // mass of what top-k keeps
-      int kb = 64;                                         // the bin that top-k cuts, 64: none
-      int n_kb = 0;
-      unsigned long long qt = 0;                           // mass of a code at t
-      if (by_count && (unsigned)set.k < sample_lane(c_run, 63)) {
-        kb = __builtin_ctzll(__ballot(c_run >= (unsigned)set.k));
-        const unsigned want = (unsigned)set.k - (sample_lane(c_run, kb) - sample_lane(c_in, kb));
-        const unsigned long long above = sample_lane(m_run, kb) - sample_lane(m_in, kb);
-        n_kb = w.members(s, bins, kb);
-        sample_wave_sync();
-        if (n_kb >= 0) {
-          const float mz = lane < n_kb ? s.m_z[lane] : -INFINITY;
-          const unsigned long long mq = lane < n_kb ? s.m_mass[lane] : 0ull;
-          unsigned gt = 0, ge = 0;
-          for (int i = 0; i < n_kb; ++i) {
-            const float o = __uint_as_float(sample_lane(__float_as_uint(mz), i));
-            gt += o > mz;
-            ge += o >= mz;
-          }
-          const int at = __builtin_ctzll(__ballot(lane < n_kb && gt < want && want <= ge));
-          t = __uint_as_float(sample_lane(__float_as_uint(mz), at));
-          r = want - sample_lane(gt, at);
-          qt = sample_lane(mq, at);
-          total = above + sample_wave_sum(mz > t ? mq : 0ull) + r * qt;
-        } else {   // the largest t that at least k keys reach, a bit at a time
-          unsigned key = 0;
-          for (int b = 31; b >= 0; --b) {
-            const unsigned c = key | 1u << b;
-            unsigned n = 0;
-#pragma unroll
-            for (int j = 0; j < R; ++j) n += (unsigned)__builtin_popcountll(__ballot(sample_key(w.z[j]) >= c));
-            if (n >= (unsigned)set.k) key = c;
-          }
-          t = sample_unkey(key);
+      if (n_kb >= 0) {
+        const float mz = lane < n_kb ? s.m_z[lane] : -INFINITY;
+        const unsigned long long mq = lane < n_kb ? s.m_mass[lane] : 0ull;
+        unsigned gt = 0, ge = 0;
+        for (int i = 0; i < n_kb; ++i) {
+          const float o = __uint_as_float(sample_lane(__float_as_uint(mz), i));
+          gt += o > mz;
+          ge += o >= mz;
+        }
+        const int at = __builtin_ctzll(__ballot(lane < n_kb && gt < want && want <= ge));
+        t = __uint_as_float(sample_lane(__float_as_uint(mz), at));
+        r = want - sample_lane(gt, at);
+        qt = sample_lane(mq, at);
+        total = above + sample_wave_sum(mz > t ? mq : 0ull) + r * qt;
+      } else {   // the largest t that at least k keys reach, a bit at a time
+        unsigned key = 0;
+        for (int b = 31; b >= 0; --b) {
+          const unsigned c = key | 1u << b;
           unsigned n = 0;
-          unsigned long long m = 0;
 #pragma unroll
-          for (int j = 0; j < R; ++j) {
-            n += (unsigned)__builtin_popcountll(__ballot(w.z[j] > t));
-            m += w.z[j] > t ? w.q[j] : 0ull;
-          }
-          r = (unsigned)set.k - n;
-          qt = mass.q(t);
-          total = sample_wave_sum(m) + r * qt;
+          for (int j = 0; j < R; ++j) n += (unsigned)__builtin_popcountll(__ballot(sample_key(w.z[j]) >= c));
+          if (n >= (unsigned)set.k) key = c;
         }
+        t = sample_unkey(key);
+        unsigned n = 0;
+        unsigned long long m = 0;
+#pragma unroll
+        for (int j = 0; j < R; ++j) {
+          n += (unsigned)__builtin_popcountll(__ballot(w.z[j] > t));
+          m += w.z[j] > t ? w.q[j] : 0ull;
+        }
+        r = (unsigned)set.k - n;
+        qt = mass.q(t);
+        total = sample_wave_sum(m) + r * qt;
       }
-      if (by_mass) {
-        const unsigned long long bound = sample_bound(set.p, total);
-        // (a bin that top-k cuts counts as reached: what it keeps of it is in `total`)
-        const unsigned long long reach = __ballot(m_run >= bound);
-        const int pb = min(reach ? __builtin_ctzll(reach) : 63, kb);
-        const unsigned long long need = bound - (sample_lane(m_run, pb) - sample_lane(m_in, pb));
-        const int n = pb == kb ? n_kb : w.members(s, bins, pb);
-        sample_wave_sync();
-        if (n >= 0) {
-          const float mz = lane < n ? s.m_z[lane] : -INFINITY;
-          unsigned long long mq = lane < n ? s.m_mass[lane] : 0ull;
-          if (!(mz > t)) mq = 0;
-          unsigned long long gt = 0, ge = 0;
-          for (int i = 0; i < n; ++i) {
-            const float o = __uint_as_float(sample_lane(__float_as_uint(mz), i));
-            const unsigned long long m = sample_lane(mq, i);
-            gt += o > mz ? m : 0ull;
-            ge += o >= mz ? m : 0ull;
-          }
-          const unsigned long long hit = __ballot(mz > t && gt < need && need <= ge);
-          if (hit) {   // (else it falls on the ties that top-k kept)
-            const int at = __builtin_ctzll(hit);
-            t = __uint_as_float(sample_lane(__float_as_uint(mz), at));
-            r = sample_ceil_div(need - sample_lane(gt, at), sample_lane(mq, at));
-          } else {
-            r = min(r, sample_ceil_div(need - sample_wave_sum(mq), qt));
-          }
+    }
+    if (by_mass) {
+      const unsigned long long bound = sample_bound(set.p, total);
+      // (a bin that top-k cuts counts as reached: what it keeps of it is in `total`)
+      const unsigned long long reach = __ballot(m_run >= bound);
+      const int pb = min(reach ? __builtin_ctzll(reach) : 63, kb);
+      const unsigned long long need = bound - (sample_lane(m_run, pb) - sample_lane(m_in, pb));
+      const int n = pb == kb ? n_kb : w.members(s, bins, pb);
+      sample_wave_sync();
+      if (n >= 0) {
+        const float mz = lane < n ? s.m_z[lane] : -INFINITY;
+        unsigned long long mq = lane < n ? s.m_mass[lane] : 0ull;
+        if (!(mz > t)) mq = 0;
+        unsigned long long gt = 0, ge = 0;
+        for (int i = 0; i < n; ++i) {
+          const float o = __uint_as_float(sample_lane(__float_as_uint(mz), i));
+          const unsigned long long m = sample_lane(mq, i);
+          gt += o > mz ? m : 0ull;
+          ge += o >= mz ? m : 0ull;
+        }
+        const unsigned long long hit = __ballot(mz > t && gt < need && need <= ge);
+        if (hit) {   // (else it falls on the ties that top-k kept)
+          const int at = __builtin_ctzll(hit);
+          t = __uint_as_float(sample_lane(__float_as_uint(mz), at));
+          r = sample_ceil_div(need - sample_lane(gt, at), sample_lane(mq, at));
         } else {
-          const unsigned kt = sample_key(t);
-          const unsigned long long at_t = r * qt;
-          unsigned key = 0;
-          for (int b = 31; b >= 0; --b) {
-            const unsigned c = key | 1u << b;
-            unsigned long long m = 0;
-#pragma unroll
-            for (int j = 0; j < R; ++j) m += sample_key(w.z[j]) >= c && w.z[j] > t ? w.q[j] : 0ull;
-            if (sample_wave_sum(m) + (kt >= c ? at_t : 0ull) >= bound) key = c;
-          }
-          const float z = sample_unkey(key);
+          r = min(r, sample_ceil_div(need - sample_wave_sum(mq), qt));
+        }
+      } else {
+        const unsigned kt = sample_key(t);
+        const unsigned long long at_t = r * qt;
+        unsigned key = 0;
+        for (int b = 31; b >= 0; --b) {
+          const unsigned c = key | 1u << b;
           unsigned long long m = 0;
 #pragma unroll
-          for (int j = 0; j < R; ++j) m += w.z[j] > z && w.z[j] > t ? w.q[j] : 0ull;
-          const unsigned rr = sample_ceil_div(bound - sample_wave_sum(m) - (kt > key ? at_t : 0ull), mass.q(z));
-          r = key == kt ? min(r, rr) : rr;
-          t = z;
+          for (int j = 0; j < R; ++j) m += sample_key(w.z[j]) >= c && w.z[j] > t ? w.q[j] : 0ull;
+          if (sample_wave_sum(m) + (kt >= c ? at_t : 0ull) >= bound) key = c;
         }
+        const float z = sample_unkey(key);
+        unsigned long long m = 0;
+#pragma unroll
+        for (int j = 0; j < R; ++j) m += w.z[j] > z && w.z[j] > t ? w.q[j] : 0ull;
+        const unsigned rr = sample_ceil_div(bound - sample_wave_sum(m) - (kt > key ? at_t : 0ull), mass.q(z));
+        r = key == kt ? min(r, rr) : rr;
+        t = z;
       }
     }
-    // the draw: kept masses summed in index order
-    unsigned ties = 0, nth = 0;
-    if (r) {
+  }
+  // the draw: kept masses summed in index order
+  unsigned ties = 0, nth = 0;
+  if (r) {
 #pragma unroll
-      for (int j = 0; j < R; ++j) ties += w.z[j] == t;
-      nth = sample_wave_scan(ties) - ties;
-    }
-    unsigned long long sum = 0;
+    for (int j = 0; j < R; ++j) ties += w.z[j] == t;
+    nth = sample_wave_scan(ties) - ties;
+  }
+  unsigned long long sum = 0;
+#pragma unroll
+  for (int j = 0; j < R; ++j) {
+    const bool tie = w.z[j] == t;
+    const bool kept = (w.z[j] > t || (tie && nth < r)) && !(floored >> j & 1);
+    nth += tie;
+    w.q[j] = kept ? w.q[j] : 0ull;
+    sum += w.q[j];
+  }
+  const unsigned long long run = sample_wave_scan(sum), total = sample_lane(run, 63);
+  const unsigned long long target = sample_target(set.u, total);
+  const int first = __builtin_ctzll(__ballot(run > target));
+  if (lane == first) {
+    unsigned long long upto = run - sum;
+    int at = 0;
+    float z = 0.f;
+    bool found = false;
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      const bool tie = w.z[j] == t;
-      const bool kept = (w.z[j] > t || (tie && nth < r)) && !(floored >> j & 1);
-      nth += tie;
-      w.q[j] = kept ? w.q[j] : 0ull;
-      sum += w.q[j];
-    }
-    const unsigned long long run = sample_wave_scan(sum), total = sample_lane(run, 63);
-    const unsigned long long target = sample_target(set.u, total);
-    const int first = __builtin_ctzll(__ballot(run > target));
-    if (lane == first) {
-      unsigned long long upto = run - sum;
-      int at = 0;
-      float z = 0.f;
-      bool found = false;
-#pragma unroll
-      for (int j = 0; j < R; ++j) {
-        upto += w.q[j];
-        if (!found && upto > target) {
-          found = true;
-          at = j;
-          z = w.z[j];
-        }
+      upto += w.q[j];
+      if (!found && upto > target) {
+        found = true;
+        at = j;
+        z = w.z[j];
       }
-      sample_answer(a, row, lane * R + at, mass.logp(z, total));
     }
+    sample_answer(a, row, lane * R + at, mass.logp(z, total));
   }
 }
 

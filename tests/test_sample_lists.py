@@ -160,7 +160,7 @@ SETTINGS = [dict(), dict(T=0.7, k=5), dict(p=0.9), dict(m=0.05), dict(T=1.3, k=5
 @pytest.mark.parametrize("dtype", ["float32", "float16", "bfloat16"])
 @pytest.mark.parametrize("n,V", [(1, 1), (3, 2), (5, 63), (4, 64), (4, 65), (300, 256), (7, 257), (9, 512), (9, 513), (3, 1000), (5, 1024), (5, 1025), (6, 4099),
                                  (2, 2048), (2, 6145), (2, 10240), (2, 10241), (2, 16385), (2, 20480), (2, 20481), (2, 32769), (2, 70001), (1, (1 << 20) + 3),
-                                 (257, 1025), (257, 2049), (257, 5121), (257, 10241)])
+                                 (2500, 100), (2500, 128), (2500, 200), (2500, 256), (257, 1025), (257, 2049), (257, 5121), (257, 10241)])
 def test_sample_sizes_and_settings(dtype, n, V):
     import torch
     g = torch.Generator("cuda").manual_seed(n * 1000003 + V)
@@ -174,7 +174,7 @@ def test_sample_masks_infinities_nan_and_ties():
     import torch
     g = torch.Generator("cuda").manual_seed(5)
     inf, low = float("inf"), torch.finfo(torch.float32).min
-    for V, rep in ((2, 1), (64, 1), (200, 1), (256, 1), (500, 1), (900, 1), (1500, 1), (1500, 7), (4000, 7), (5001, 1), (6000, 7), (11000, 1), (40000, 1)):
+    for V, rep in ((2, 1), (64, 1), (100, 1), (100, 52), (200, 1), (200, 52), (256, 1), (500, 1), (900, 1), (1500, 1), (1500, 7), (4000, 7), (5001, 1), (6000, 7), (11000, 1), (40000, 1)):
         z = torch.randn(40, V, generator=g, device="cuda")
         z[0] = -inf                                    # nothing left
         z[1] = float("nan")
