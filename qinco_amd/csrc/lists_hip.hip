@@ -91,20 +91,28 @@ static int launch_sample_long(const SampleArgs& a, const SamplePlan& p, char* ws
   l.m_z = reinterpret_cast<float*>(ws + p.m_z);
   l.m_where = reinterpret_cast<unsigned*>(ws + p.m_where);
   l.most = (int)p.most;
+  l.uncut = !a.k_rows && !a.p_rows && !a.m_rows && (a.k <= 0 || a.k >= a.V) && a.p >= 1.0 && !(a.m > 0.0);
   for (long r0 = 0; r0 < a.n; r0 += p.rows) {
     const long rows = a.n - r0 < p.rows ? a.n - r0 : (long)p.rows;
     l.row0 = r0;
     const dim3 grid((unsigned)(rows * p.chunks)), block(kSampleChunkThreads);
     hipLaunchKernelGGL(sample_range_kernel<T>, grid, block, 0, st, a, l);
     HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL(sample_bins_kernel<T>, grid, block, 0, st, a, l);
-    HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL(sample_sum_bins_kernel, dim3((unsigned)(rows * (kSampleBins / 64))), dim3(1024), 0, st, l);
-    HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL(sample_cuts_kernel, dim3((unsigned)rows), dim3(1024), 0, st, a, l);
-    HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL(sample_members_kernel<T>, grid, block, 0, st, a, l);
-    HIP_TRY(hipGetLastError());
+    if (l.uncut) {
+      hipLaunchKernelGGL(sample_mass_kernel<T>, grid, block, 0, st, a, l);
+      HIP_TRY(hipGetLastError());
+    } else {
+      hipLaunchKernelGGL(sample_bins_kernel<T>, grid, block, 0, st, a, l);
+      HIP_TRY(hipGetLastError());
+      if (p.chunks > kSampleFewChunks) {
+        hipLaunchKernelGGL(sample_sum_bins_kernel, dim3((unsigned)(rows * (kSampleBins / 64))), dim3(1024), 0, st, l);
+        HIP_TRY(hipGetLastError());
+      }
+      hipLaunchKernelGGL(sample_cuts_kernel, dim3((unsigned)rows), dim3(1024), 0, st, a, l);
+      HIP_TRY(hipGetLastError());
+      hipLaunchKernelGGL(sample_members_kernel<T>, grid, block, 0, st, a, l);
+      HIP_TRY(hipGetLastError());
+    }
     hipLaunchKernelGGL(sample_finish_kernel<T>, dim3((unsigned)rows), block, 0, st, a, l);
     HIP_TRY(hipGetLastError());
   }

@@ -873,62 +873,44 @@ __device__ __forceinline__ unsigned sample_search(SampleBlock<NT>& blk, SampleFo
   }
 }
 
-// The draw among the codes that the workgroup's waves own, [w_first + w 64 steps, + 64 steps) each, with `run` of mass and `seen` codes at
-// t before the first wave's; blk holds every wave's mass above t and codes at t.  The wave that the target falls into has its steps of 64
-// codes taken by all waves side by side, and the one that it falls into draws.  `z`: the row.  Barriers inside: every thread.
-template <typename T, int NT>
-__device__ __forceinline__ void sample_draw(const SampleArgs& a, long row, const T* z, int w_first, int steps, const SampleMass& mass, double m,
+// The draw among N codes per thread, in the order of their threads, with `run` of mass and `seen` codes at t before the first thread's: codes
+// above t, and those at t that are among the first r.  index(j) = the code that z[j] is the logit of.  Barriers inside: every thread.
+template <int NT, int N, typename Index>
+__device__ __forceinline__ void sample_draw(const SampleArgs& a, long row, const float (&z)[N], Index index, const SampleMass& mass, double m,
                                             float t, unsigned r, unsigned long long qt, SampleBlock<NT>& blk, unsigned long long run,
                                             unsigned seen, unsigned long long target, unsigned long long total) {
-  constexpr int NW = NT / 64;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6, per = (steps + NW - 1) / NW;   // steps of one wave
-  int at_wave = 0;
-#pragma unroll 1
-  for (; at_wave < NW - 1; ++at_wave) {
-    const unsigned long long next = run + blk.m[at_wave] + min(blk.c[at_wave], r > seen ? r - seen : 0u) * qt;
-    if (target < next) break;
-    run = next;
-    seen += blk.c[at_wave];
+  unsigned long long q[N], sum = 0;
+  unsigned at_t = 0;
+#pragma unroll
+  for (int j = 0; j < N; ++j) {
+    q[j] = 0;
+    if (z[j] > t) q[j] = mass.q(z[j], m);
+    sum += q[j];
+    at_t += z[j] == t && r > 0;
+    if (j & 1) __builtin_amdgcn_sched_barrier(0);
   }
-  const int first = w_first + at_wave * 64 * steps, j0 = w * per, j1 = min(j0 + per, steps);
-  unsigned long long sum = 0;
-  unsigned ties = 0;
-  for (int j = j0; j < j1; ++j) {
-    const float x = sample_logit(z, first + j * 64 + lane, a.V);
-    sum += x > t ? mass.q(x, m) : 0ull;
-    ties += x == t && r > 0;
-  }
-  sum = sample_wave_sum(sum);
-  ties = sample_wave_sum(ties);
-  __syncthreads();
-  if (lane == 0) {
-    blk.m[w] = sum;
-    blk.c[w] = ties;
-  }
-  __syncthreads();
-#pragma unroll 1
-  for (int v = 0; v < w; ++v) {
-    run += blk.m[v] + min(blk.c[v], r > seen ? r - seen : 0u) * qt;
-    seen += blk.c[v];
-  }
-  const unsigned long long here = sum + min(ties, r > seen ? r - seen : 0u) * qt;
+  unsigned long long before, all;
+  unsigned c_before, c_all;
+  sample_block_scan<NT>(blk, sum, at_t, before, c_before, all, c_all);
+  run += before + (min(seen + c_before, r) - min(seen, r)) * qt;
+  seen += c_before;
+  const unsigned long long here = sum + (min(seen + at_t, r) - min(seen, r)) * qt;
   if (run <= target && target < run + here) {
-#pragma unroll 1
-    for (int j = j0; j < j1; ++j) {
-      const int i = first + j * 64 + lane;
-      const float x = sample_logit(z, i, a.V);
-      const bool tie = r > 0 && x == t;
-      const unsigned long long at = __ballot(tie);
-      const unsigned nth = seen + __builtin_popcountll(at & ((1ull << lane) - 1));
-      const unsigned long long incl = run + sample_wave_scan(x > t ? mass.q(x, m) : (tie && nth < r ? qt : 0ull));
-      const unsigned long long hit = __ballot(incl > target);
-      if (hit) {
-        if (lane == (int)__builtin_ctzll(hit)) sample_answer(a, row, i, mass.logp(x, total));
-        break;
+    int at = 0;
+    float x = 0.f;
+    bool drawn = false;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const bool tie = z[j] == t && r > 0;
+      run += q[j] + (tie && seen < r ? qt : 0ull);
+      seen += tie;
+      if (!drawn && run > target) {
+        drawn = true;
+        at = index(j);
+        x = z[j];
       }
-      run = sample_lane(incl, 63);
-      seen += __builtin_popcountll(at);
     }
+    sample_answer(a, row, at, mass.logp(x, total));
   }
 }
 
@@ -1270,6 +1252,8 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a, long 
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kSampleChunkThreads = 1024, kSampleChunkIpt = 16, kSampleChunk = kSampleChunkThreads * kSampleChunkIpt;
 constexpr int kSampleMaxChunks = 1024;          // V <= 2^24
+constexpr int kSampleFewChunks = 4;             // up to which the bins are summed where the cuts are found (500 rows of 50000: 154 us, 169
+                                                // with a launch of its own; one row of 130000, eight chunks, 39 and 37)
 constexpr int kSampleHere = 2048;               // members of a chunk listed one by one; with more, equal ones as one
 constexpr int kSampleMembers = 4096;            // members of a row that the last kernel holds in LDS
 
@@ -1304,6 +1288,7 @@ struct SampleState {                   // of a row
 struct SampleLong {
   long row0;                           // first row of the batch
   int chunks;
+  int uncut;                           // no row has a cut: state is not there
   int most;                            // members that a row's list holds (with more the last kernel searches the row itself)
   unsigned long long* best;            // [row][chunk] key of the largest logit << 32 | ~lowest index that holds it
   unsigned* least;                     // [row][chunk] ~key of the smallest logit that is not -inf
@@ -1437,6 +1422,35 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_bins_kernel(Sample
   if (tid == 0) l.floor[r * l.chunks + c] = floor;
 }
 
+// Where no row has a cut the mass of every chunk is all that the last kernel needs: three launches (one row of 50000 fp32 21 us, 16 of 2^20
+// 47; with bins, cuts and members all the same 32 and 67).
+template <typename T>
+__global__ void __launch_bounds__(kSampleChunkThreads) sample_mass_kernel(SampleArgs a, SampleLong l) {
+  __shared__ unsigned sh[3];
+  __shared__ unsigned long long part[kSampleChunkThreads / 64];
+  const long r = blockIdx.x / l.chunks;
+  const int c = blockIdx.x - (int)(r * l.chunks), lane = threadIdx.x & 63;
+  const SampleRow set = sample_row(a, l.row0 + r);
+  float z[kSampleChunkIpt];
+  sample_load_chunk(a, reinterpret_cast<const T*>(a.logits) + (l.row0 + r) * a.stride, c * kSampleChunk, z);
+  const SampleRange g = sample_range(l, r, sh);
+  if (g.zmax == -INFINITY || set.greedy) return;
+  const SampleMass mass(g.zmax, set.y, a.F);
+  unsigned long long sum = 0;
+#pragma unroll
+  for (int j = 0; j < kSampleChunkIpt; ++j) {
+    sum += mass.q(z[j]);
+    if (j & 1) __builtin_amdgcn_sched_barrier(0);
+  }
+  sum = sample_wave_sum(sum);
+  if (lane == 0) part[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  if (threadIdx.x < 64) {
+    sum = sample_wave_sum(lane < kSampleChunkThreads / 64 ? part[lane] : 0ull);
+    if (lane == 0) l.chunk_mass[r * l.chunks + c] = sum;
+  }
+}
+
 // bins summed over the chunks: a workgroup owns 64 bins of a row, its 16 waves every 16th chunk
 __global__ void __launch_bounds__(1024) sample_sum_bins_kernel(SampleLong l) {
   __shared__ unsigned long long mass[16][64];
@@ -1486,8 +1500,21 @@ __global__ void __launch_bounds__(1024) sample_cuts_kernel(SampleArgs a, SampleL
   }
   __syncthreads();
   if (g.zmax > -INFINITY && !set.greedy) {
-    const unsigned long long m = l.row_mass[r * kSampleBins + tid];
-    const unsigned n = l.row_count[r * kSampleBins + tid];
+    unsigned long long m = 0;
+    unsigned n = 0;
+    if (l.chunks <= kSampleFewChunks) {
+#pragma unroll
+      for (int c = 0; c < kSampleFewChunks; ++c) {
+        if (c < l.chunks) {
+          const size_t o = ((size_t)r * l.chunks + c) * kSampleBins + tid;
+          m += l.mass[o];
+          n += l.count[o];
+        }
+      }
+    } else {
+      m = l.row_mass[r * kSampleBins + tid];
+      n = l.row_count[r * kSampleBins + tid];
+    }
     int f = kSampleBins;
     for (int c = tid; c < l.chunks; c += NT) f = min(f, l.floor[r * l.chunks + c]);
     if (f < kSampleBins) atomicMin(&st.fb, f);
@@ -1654,14 +1681,23 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
   __shared__ unsigned m_where[kSampleMembers];
   __shared__ unsigned long long chunk[kSampleMaxChunks];
   __shared__ unsigned chunk_ties[kSampleMaxChunks];
-  __shared__ unsigned key_range[2];
+  __shared__ unsigned key_range[2], sh_range[3];
   __shared__ int sh_chunk;
   __shared__ unsigned sh_tied;
   __shared__ unsigned long long sh_before;
   const long r = blockIdx.x, row = l.row0 + r;
   const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
   const SampleRow set = sample_row(a, row);
-  const SampleState st = l.state[r];
+  SampleState st{};
+  if (l.uncut) {
+    const SampleRange g = sample_range(l, r, sh_range);
+    st.zmax = g.zmax;
+    st.zmin = g.zmin;
+    st.first = g.first;
+    st.kb = st.b0 = st.b1 = st.fb = kSampleBins;
+  } else {
+    st = l.state[r];
+  }
   if (st.zmax == -INFINITY || set.greedy) {
     if (tid == 0) {
       if (st.zmax == -INFINITY) sample_answer(a, row, -1, -INFINITY);
@@ -1775,52 +1811,48 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
     sh_tied = tied;
   }
   __syncthreads();
-  // ... and in that chunk: wave w owns codes [i0 + 1024 w, + 1024).  What is kept of it is listed first (the members are done with): an
-  // exponential for every step in which one of 64 codes is kept would take longer
-  const int i0 = sh_chunk * kSampleChunk, w0 = i0 + w * 64 * kSampleChunkIpt;
+  // ... and in that chunk, 16 neighbouring codes per thread.  Where few of them are kept these are listed first, in their order (the members
+  // are done with), and shared out anew: an exponential for every step in which one of a wave's 64 codes is kept would take longer
+  const int i0 = sh_chunk * kSampleChunk, mine0 = tid * kSampleChunkIpt;
   float z[kSampleChunkIpt];
-  unsigned at_t = 0, is = 0;
 #pragma unroll
-  for (int j = 0; j < kSampleChunkIpt; ++j) z[j] = sample_logit(logits, w0 + j * 64 + lane, a.V);
+  for (int j = 0; j < kSampleChunkIpt; j += 4) {
+    const int i = i0 + mine0 + j;
+    if (i + 4 <= a.V) {
+      GroupUnit<T, 4> u;
+      u.load(logits + i);
 #pragma unroll
-  for (int j = 0; j < kSampleChunkIpt; ++j) {
-    is |= (unsigned)(z[j] > t) << j;
-    at_t += z[j] == t && ties > 0;
+      for (int e = 0; e < 4; ++e) {
+        const float x = GroupNum<T>::get(u.v[e]);
+        z[j + e] = x == x ? x : -INFINITY;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) z[j + e] = sample_logit(logits, i + e, a.V);
+    }
   }
+  unsigned is = 0;
+#pragma unroll
+  for (int j = 0; j < kSampleChunkIpt; ++j) is |= (unsigned)(z[j] > t || (z[j] == t && ties > 0)) << j;
   unsigned first, kept;
   sample_block_scan<NT>(blk, 0ull, (unsigned)__builtin_popcount(is), before, first, all, kept);
-  at_t = sample_wave_sum(at_t);
-  unsigned long long sum = 0;
   if (kept <= kSampleMembers) {
-    if (tid < NT / 64) part[tid] = 0;
 #pragma unroll
     for (int j = 0; j < kSampleChunkIpt; ++j) {
       if (is >> j & 1) {
         m_z[first] = z[j];
-        m_where[first++] = (unsigned)w;
+        m_where[first++] = (unsigned)(mine0 + j);
       }
     }
     __syncthreads();
-    for (unsigned i = tid; i < kept; i += NT) {
-      const unsigned long long q = mass.q(m_z[i], set.m);
-      if (q) atomicAdd(&part[m_where[i]], q);
-    }
-    __syncthreads();
-    sum = part[w];
-  } else {
+    constexpr int N = kSampleMembers / NT;
+    float x[N];
 #pragma unroll
-    for (int j = 0; j < kSampleChunkIpt; ++j) {
-      sum += is >> j & 1 ? mass.q(z[j], set.m) : 0ull;
-      if (j & 1) __builtin_amdgcn_sched_barrier(0);
-    }
-    sum = sample_wave_sum(sum);
+    for (int j = 0; j < N; ++j) x[j] = tid * N + j < (int)kept ? m_z[tid * N + j] : -INFINITY;
+    sample_draw<NT>(a, row, x, [&](int j) { return i0 + (int)m_where[tid * N + j]; }, mass, set.m, t, ties, qt, blk, sh_before, sh_tied, target, total);
+  } else {
+    sample_draw<NT>(a, row, z, [&](int j) { return i0 + mine0 + j; }, mass, set.m, t, ties, qt, blk, sh_before, sh_tied, target, total);
   }
-  if (lane == 0) {
-    blk.m[w] = sum;
-    blk.c[w] = at_t;
-  }
-  __syncthreads();
-  sample_draw<T, NT>(a, row, logits, i0, kSampleChunkIpt, mass, set.m, t, ties, qt, blk, sh_before, sh_tied, target, total);
 }
 
 }  // namespace qinco
