@@ -35,13 +35,16 @@ def group_rows(lists, n_lists: int, check: bool = True) -> "RowGroups":
     if k > 1:
         lists = unit_rows(lists)
     dev = lists.device
-    order = torch.empty(n * k, dtype=torch.int32, device=dev)
-    place = torch.empty((n, k), dtype=torch.int32, device=dev)
-    offsets = torch.empty(int(n_lists) + 1, dtype=torch.int32, device=dev)
+    N, E = n * k, int(n_lists)
+    need = lib.qinco_group_workspace(N, E)
+    if need <= 1 << 16:   # few entries: the call is all that counts, and one allocation is 2 us less of it than four
+        ws, order, place, offsets = torch.empty(need // 4 + 2 * N + E + 1, dtype=torch.int32, device=dev).split_with_sizes((need // 4, N, N, E + 1))
+        place = place.view(n, k)
+    else:
+        order, place, offsets = (torch.empty(s, dtype=torch.int32, device=dev) for s in (N, (n, k), E + 1))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
     bad = torch.zeros(1, dtype=torch.int32, device=dev) if check else None
-    need = lib.qinco_group_workspace(n * k, int(n_lists))
-    ws = torch.empty(need, dtype=torch.uint8, device=dev)
-    on_its_device(dev.index, lib.qinco_group_rows, lists.data_ptr(), code, lists.stride(0), n, k, int(n_lists), order.data_ptr(), place.data_ptr(),
+    on_its_device(dev.index, lib.qinco_group_rows, lists.data_ptr(), code, lists.stride(0), n, k, E, order.data_ptr(), place.data_ptr(),
                   offsets.data_ptr(), bad.data_ptr() if check else None, ws.data_ptr(), need)
     if check and int(bad):
         raise IndexError(f"a list id is >= n_lists = {n_lists}")

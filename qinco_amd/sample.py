@@ -13,7 +13,8 @@ import torch
 
 from . import _lib
 
-_CODES = {np.dtype(np.int64): _lib.CODE_I64, np.dtype(np.int32): _lib.CODE_I32}
+_CODES = {np.dtype(np.int64): (_lib.CODE_I64, torch.int64), np.dtype(np.int32): (_lib.CODE_I32, torch.int32)}
+_CODES[np.int64], _CODES[np.int32] = _CODES[np.dtype(np.int64)], _CODES[np.dtype(np.int32)]
 
 
 _RANDOM, _FLOAT, _INT = (torch.float32, torch.float64), (torch.float32,), (torch.int32,)
@@ -64,6 +65,13 @@ def on_its_device(index: int, call, *args) -> None:
         _lib.check(rc)
 
 
+def _rows(t, n: int, dev, what: str, types):
+    """A value per row, on the logits' device."""
+    if on_device(t, what).shape != (n,) or t.dtype not in types or t.device != dev:
+        raise ValueError(f"{what} must be ({n},) of {' or '.join(map(str, types))} on {dev}, got {tuple(t.shape)} {t.dtype} on {t.device}")
+    return as_stored(t).contiguous()
+
+
 def sample_codes(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, code_dtype=np.int64, return_logp: bool = False):
     """One code per row of `logits` (n, V) float32 / float16 / bfloat16 from the given random numbers `u` (n,) in [0, 1), float32 or
     float64; torch CUDA tensors, asynchronous on the current stream.  Returns codes (n,) of `code_dtype` (int64 or int32) [and the log
@@ -78,54 +86,50 @@ def sample_codes(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, c
 
     temperature, top_p, min_p (float32) and top_k (int32) may be tensors (n,) with a value per row; there a temperature <= 0 is 0."""
     lib = _lib.load()
-    on_device(logits, "logits")
-    if logits.dim() != 2 or logits.shape[1] < 1:
-        raise ValueError(f"logits must be (n, V) with V >= 1, got {tuple(logits.shape)}")
+    shape = on_device(logits, "logits").shape
+    if len(shape) != 2 or shape[1] < 1:
+        raise ValueError(f"logits must be (n, V) with V >= 1, got {tuple(shape)}")
     dtype = row_type(logits, "logits")
     logits = unit_rows(logits)
-    n, V = logits.shape
+    n, V = shape
     dev = logits.device
-
-    def rows(t, what, types):
-        if on_device(t, what).shape != (n,) or t.dtype not in types or t.device != dev:
-            raise ValueError(f"{what} must be ({n},) of {' or '.join(map(str, types))} on {dev}, got {tuple(t.shape)} {t.dtype} on {t.device}")
-        return as_stored(t).contiguous()
-    u = rows(u, "u", _RANDOM)
+    u = _rows(u, n, dev, "u", _RANDOM)
+    code = _CODES.get(code_dtype) or _CODES.get(np.dtype(code_dtype))
+    if code is None:
+        raise ValueError("code_dtype must be int64 or int32 (a row with nothing to draw answers -1)")
     params = _lib.QincoSampleParams(_PARAMS_BYTES)
     keep = []                                          # (arrays made contiguous live until the call is enqueued)
     if isinstance(temperature, torch.Tensor):
-        keep.append(rows(temperature, "temperature", _FLOAT))
+        keep.append(_rows(temperature, n, dev, "temperature", _FLOAT))
         params.temperature_rows = keep[-1].data_ptr()
     else:
         params.temperature = temperature = float(temperature)
         if not 0.0 <= temperature < math.inf:
             raise ValueError(f"temperature must be finite and >= 0, got {temperature}")
     if isinstance(top_k, torch.Tensor):
-        keep.append(rows(top_k, "top_k", _INT))
+        keep.append(_rows(top_k, n, dev, "top_k", _INT))
         params.top_k_rows = keep[-1].data_ptr()
     else:
-        params.top_k = min(max(int(top_k), 0), V)
+        top_k = int(top_k)
+        params.top_k = top_k if 0 < top_k < V else 0
     if isinstance(top_p, torch.Tensor):
-        keep.append(rows(top_p, "top_p", _FLOAT))
+        keep.append(_rows(top_p, n, dev, "top_p", _FLOAT))
         params.top_p_rows = keep[-1].data_ptr()
     else:
         params.top_p = top_p = float(top_p)
         if top_p != top_p:
             raise ValueError("top_p must be a number")
     if isinstance(min_p, torch.Tensor):
-        keep.append(rows(min_p, "min_p", _FLOAT))
+        keep.append(_rows(min_p, n, dev, "min_p", _FLOAT))
         params.min_p_rows = keep[-1].data_ptr()
     else:
         params.min_p = min_p = float(min_p)
         if not min_p <= 1.0:
             raise ValueError(f"min_p must be at most 1, got {min_p}")
-    code = _CODES.get(np.dtype(code_dtype))
-    if code is None:
-        raise ValueError("code_dtype must be int64 or int32 (a row with nothing to draw answers -1)")
-    codes = torch.empty(n, dtype=torch.int64 if code == _lib.CODE_I64 else torch.int32, device=dev)
+    codes = torch.empty(n, dtype=code[1], device=dev)
     logp = torch.empty(n, dtype=torch.float32, device=dev) if return_logp else None
     need = lib.qinco_sample_workspace(n, V)
     ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
     on_its_device(dev.index, lib.qinco_sample_codes, logits.data_ptr(), dtype, logits.stride(0), n, V, u.data_ptr(), u.dtype == torch.float64,
-                  params, codes.data_ptr(), code, logp.data_ptr() if return_logp else None, ws.data_ptr() if need else None, need)
+                  params, codes.data_ptr(), code[0], logp.data_ptr() if return_logp else None, ws.data_ptr() if need else None, need)
     return (codes, logp) if return_logp else codes
