@@ -55,6 +55,7 @@ struct GroupPass {
   unsigned* total;                       // entries that have a list
   int* bad;                              // nullable: set to 1 if an id is >= E
   int shift, bits, first, last;
+  int tiles;                             // few: counts are as the histogram left them, every workgroup sums them itself; 0: scanned
 };
 
 // one wave's counter of a digit in LDS: read and bumped by lanes of the same wave, whose LDS accesses execute in order
@@ -222,8 +223,20 @@ __global__ void __launch_bounds__(kGroupThreads) group_scatter_kernel(GroupPass 
   for (int j = 0; j < BPT; ++j) {
     const int b = tid * bpt + j;
     const bool in = j < bpt && b < bins;
-    mine[j] = in ? a.totals[b] : 0;
-    earlier[j] = in ? a.counts[(size_t)blockIdx.x * bins + b] : 0;
+    mine[j] = earlier[j] = 0;
+    if (a.tiles) {
+      if (in) {
+#pragma unroll 8
+        for (int t = 0; t < a.tiles; ++t) {
+          const unsigned c = a.counts[(size_t)t * bins + b];
+          mine[j] += c;
+          earlier[j] += t < (int)blockIdx.x ? c : 0;
+        }
+      }
+    } else if (in) {
+      mine[j] = a.totals[b];
+      earlier[j] = a.counts[(size_t)blockIdx.x * bins + b];
+    }
     s += mine[j];
   }
   for (int b = tid * 2; b < bins; b += kGroupThreads * 2)   // (two 16-bit counters per store; of one bin there are two all the same)

@@ -212,6 +212,11 @@ struct GroupPlan {
 };
 }  // namespace
 
+// Counts (tiles times bins) up to which every workgroup of the scatter sums them itself, a launch less per pass (summed there / by a kernel of
+// their own: 16384 entries by 1024 lists, 16 tiles of 1024 bins, 10.2 / 11.5 us, 32768 12.1 / 11.6; by 65536 lists, two passes of 256 bins, 32
+// tiles 20.8 / 23.8, 64 24.1 / 24.8, 96 27.7 / 25.5; 8192 by 2048 12.6 / 12.9, 16384 16.2 / 13.0)
+static constexpr int64_t kGroupFewCounts = 1 << 14;
+
 // Entries per thread.  A tile has a cost of its own (tables of its digits), few tiles leave the chip empty.  Measured with 2 / 4 / 8 per
 // thread, a sort by 1024 lists: 2^17 entries 12.6 / 14.4 / 18.9 us, 2^18 14.4 / 15.4 / 19.5, 2^19 23.3 / 17.9 / 20.7, 2^20 43.4 / 28.4 / 24.5,
 // 2^22 151 / 104 / 67.
@@ -290,6 +295,7 @@ extern "C" int qinco_group_rows(const void* lists, int code_dtype, int64_t row_s
   a.bad = bad;
   a.bits = p.bits;
   a.first = a.last = 1;
+  a.tiles = p.tiles << p.bits <= kGroupFewCounts ? (int)p.tiles : 0;
   if (N <= kGroupTile) {
     const bool search = E > (unsigned)kGroupSmallOffsets;
     a.key_out = search ? ws + p.keys : nullptr;
@@ -314,8 +320,10 @@ extern "C" int qinco_group_rows(const void* lists, int code_dtype, int64_t row_s
     a.offsets = p.passes == 1 ? offsets : nullptr;
     with_ipt(p.ipt, [&](auto ipt) { hipLaunchKernelGGL((group_hist_kernel<decltype(ipt)::value>), grid, block, 0, st, a); });
     HIP_TRY(hipGetLastError());
-    hipLaunchKernelGGL(group_scan_kernel, dim3((unsigned)((bins + 63) / 64)), dim3(1024), 0, st, a.counts, a.totals, (int)p.tiles, bins);
-    HIP_TRY(hipGetLastError());
+    if (!a.tiles) {
+      hipLaunchKernelGGL(group_scan_kernel, dim3((unsigned)((bins + 63) / 64)), dim3(1024), 0, st, a.counts, a.totals, (int)p.tiles, bins);
+      HIP_TRY(hipGetLastError());
+    }
     with_ipt(p.ipt, [&](auto ipt) { hipLaunchKernelGGL((group_scatter_kernel<decltype(ipt)::value>), grid, block, 0, st, a); });
     HIP_TRY(hipGetLastError());
   }

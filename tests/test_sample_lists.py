@@ -329,7 +329,7 @@ def check_group(ids, E, **kw):
 
 
 @gpu
-@pytest.mark.parametrize("N", [0, 1, 63, 64, 65, 511, 513, 4095, 4096, 4097, 8193, 100003])
+@pytest.mark.parametrize("N", [0, 1, 63, 64, 65, 511, 513, 4095, 4096, 4097, 8193, 20001, 100003])
 def test_group_sizes(N):
     import torch
     g = torch.Generator("cuda").manual_seed(N)
