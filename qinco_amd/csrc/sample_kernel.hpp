@@ -918,8 +918,9 @@ __device__ __forceinline__ void sample_draw(const SampleArgs& a, long row, const
 // the bin that a cut falls into are listed, and up to 64 of them compared by one wave, a lane each; more (heavy ties) are searched in bins.
 // One scan over the threads, of the mass above t and of the codes at t, gives the total and the thread that the draw falls on.  Every
 // exponential is taken once (of what top-k keeps alone, where nothing else wants them) and kept: with the row in LDS, taking them anew in
-// each pass, 8000 rows of 4099 fp16 went in 138 us without a cut and 206 with all three; so they go in 80 and 126 (34 of it up to the
-// largest logit), and one row of 10240 in 13 instead of 36.  Bound by instructions: 44 per exponential, about 25 per code for the rest.
+// each pass, 8000 rows of 4099 fp16 went in 138 us without a cut and 206 with all three; so they go in 80 and 126, and one row of 10240
+// in 13 instead of 36.  Bound by instructions: 74 vector ones per code without a cut, 111 with all three, issued four fifths of the time.
+// (Loads of 16 bytes for two-byte types, eight codes, are worth 1 us of the 80.)
 template <typename T, int NT, int R>
 __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a, long row0) {
   constexpr int PB = kSampleBins / NT, PAIR = 2;
