@@ -2,7 +2,8 @@
 
 `group_rows` sorts the entries of (n, k) list ids by list: the IVF column of a code matrix (k = 1, filling an index, reference
 qinco/search/search_utils.py:121-162) or the k nearest centroids of `KnnSearcher.search` (multi-probe, a router).  `RowGroups.gather`
-carries rows into that order, `RowGroups.combine` brings them back with weights; both have gradients.
+carries rows into that order, `RowGroups.combine` brings them back with weights; both have gradients.  All of it can be captured into a graph
+(`check=False`); a captured backward pass wants leaves that no eager graph holds at the same time, as torch's own operators do.
 """
 from __future__ import annotations
 

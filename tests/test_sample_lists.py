@@ -708,6 +708,41 @@ def test_two_graphs_replay_the_eager_results():
 
 
 @gpu
+def test_a_graph_of_forward_and_backward_replays_the_eager_gradients():
+    """Leaves made inside the captured run: no eager graph of theirs lives beside it."""
+    import torch
+    from qinco_amd import group_rows
+    g = torch.Generator("cuda").manual_seed(17)
+    n, k, D, E = 700, 3, 40, 90
+
+    def inputs():
+        return (torch.randint(-1, E, (n, k), generator=g, device="cuda"), torch.randn(n, D, generator=g, device="cuda"),
+                torch.rand(n, k, generator=g, device="cuda"), torch.randn(n, D, generator=g, device="cuda"))
+
+    def work(ids, x, w, d):
+        x, w = x.detach().requires_grad_(), w.detach().requires_grad_()
+        gr = group_rows(ids, E, check=False)
+        out = gr.combine(gr.gather(x) * 2.0, w)
+        return (out.detach(), *torch.autograd.grad(out, (x, w), d))
+    static = inputs()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(3):
+            work(*static)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        outs = work(*static)
+    for _ in range(4):
+        for t, v in zip(static, inputs()):
+            t.copy_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(outs, work(*static)))
+
+
+@gpu
 def test_together_with_the_search_and_the_look_up_decoder():
     """Codes drawn step by step from a prior's logits, decoded by the look-up decoder, the reconstructions sent to their two nearest lists
     (k-nearest-list search), scaled there and brought back with weights."""
