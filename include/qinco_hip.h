@@ -312,7 +312,8 @@ enum { QINCO_T_F32 = 0, QINCO_T_F16 = 1, QINCO_T_BF16 = 2 };
  * which the kept mass, summed in index order, exceeds u[r] times its total; logp_out[r] (nullable) its log probability among the kept.
  * T <= 0: the largest logit's lowest index, log probability 0.  A row with nothing to draw: -1 and -inf.  u: (n) in [0, 1), values
  * outside are taken as the nearest end, NaN as 0.  All decisions are taken on whole-number sums of 64-bit exponentials: the same
- * inputs give the same codes, whatever the launch.
+ * inputs give the same codes, whatever the launch, and p and u decide as in exact arithmetic unless they lie within 2^-43 of a border
+ * (V <= 20480; 2^-39 at 2^20 codes, 2^-35 at 2^24).
  * The settings: arrays of one value per row, or NULL and the scalar.  top_k <= 0 or >= V, top_p >= 1, min_p <= 0 switch a cut off.
  * workspace: qinco_sample_workspace(n, V) bytes of device memory that no other running call uses.  Device pointers, asynchronous. */
 typedef struct {

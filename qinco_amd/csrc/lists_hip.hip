@@ -35,7 +35,7 @@ namespace {
 struct SamplePlan {
   int64_t rows, chunks;                                                          // rows of a batch
   int64_t most;                                                                  // members that a row's list holds
-  int64_t best, least, floor, mass, count, row_mass, row_count, state, chunk_mass, m_z, m_where, bytes;   // byte offsets
+  int64_t best, least, sum, floor, mass, count, row_mass, row_count, state, chunk_mass, m_z, m_where, bytes;   // byte offsets
 };
 }  // namespace
 
@@ -57,6 +57,7 @@ static SamplePlan sample_plan(int64_t n, int64_t V) {
   const int64_t R = p.rows, RC = R * p.chunks;
   take(p.best, RC * 8);
   take(p.least, RC * 4);
+  take(p.sum, RC * 4);
   take(p.floor, RC * 4);
   take(p.mass, RC * kSampleBins * 8);
   take(p.count, RC * kSampleBins * 4);
@@ -81,6 +82,7 @@ static int launch_sample_long(const SampleArgs& a, const SamplePlan& p, char* ws
   l.chunks = (int)p.chunks;
   l.best = reinterpret_cast<unsigned long long*>(ws + p.best);
   l.least = reinterpret_cast<unsigned*>(ws + p.least);
+  l.sum = reinterpret_cast<float*>(ws + p.sum);
   l.floor = reinterpret_cast<int*>(ws + p.floor);
   l.mass = reinterpret_cast<unsigned long long*>(ws + p.mass);
   l.count = reinterpret_cast<unsigned*>(ws + p.count);
@@ -192,7 +194,7 @@ extern "C" int qinco_sample_codes(const void* logits, int dtype, int64_t row_str
   const int lv = bits_of((uint64_t)V);
   SampleArgs a{logits, (long)row_stride, (long)n, (int)V, u, u_is_f64 != 0, params->temperature_rows, params->temperature, params->top_k_rows,
                params->top_k, params->top_p_rows, params->top_p, params->min_p_rows, params->min_p, codes_out,
-               code_dtype == QINCO_CODE_I64, logp_out, 62 - lv < 51 ? 62 - lv : 51};
+               code_dtype == QINCO_CODE_I64, logp_out, lv > 0 ? lv - 1 : 0};
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   char* ws = reinterpret_cast<char*>(workspace);
   if (dtype == QINCO_T_F32) return launch_sample<float>(a, p, ws, st);

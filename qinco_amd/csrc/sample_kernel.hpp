@@ -6,9 +6,12 @@
 // top-p, in bins: of the row first (linear in z), then of the codes of the one bin that the cut falls into; nothing is sorted.  The code
 // is the lowest kept index at which the running kept mass passes u times its total.
 //
-// NUMBERS.  A random number next to a border between two codes must fall on the side that exact arithmetic gives it, whatever order
-// the sums are taken in: e is computed in 64 bits and held as a whole number of 2^-F, F = min(51, 62 - log2 V), and all sums are of
-// whole numbers (atomics in any order give the same bits, and so do the forms below).
+// NUMBERS.  e is computed in 64 bits (good to 2^-44 of itself) and held as a whole number of 2^(down - 61) in 64 bits, and all sums are of
+// whole numbers: atomics in any order give the same bits, and so do the forms below.  `down` lets a row's sum fit 62 bits.  Up to 512 codes it is
+// log2 V rounded up, less 1; beyond, it goes by the row's own sum, estimated first: a row of one large logit keeps nearly all the bits for the far
+// ones.  (One unit for all rows of a length, 2^-38 at 2^24 codes, lost a tail of 2^-15 of the row whole.)  A cut and a draw fall on the side that
+// exact arithmetic gives them unless p or u lies within 2^-44 + V 2^-53 (V <= 512) or 2^-44 + 2.25 V 2^-61 of a border, 2^-39 at 2^20 codes and
+// 2^-35 at 2^24; a sum in fp64, one code after the other, is good to V 2^-53.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -36,7 +39,7 @@ struct SampleArgs {
   void* codes;
   int codes_i64;
   float* logp;          // nullable
-  int F;
+  int down;             // V <= 512: of every row (SampleMass)
 };
 
 // the row's settings, with every switched-off cut in the form that keeps everything
@@ -96,11 +99,13 @@ constexpr unsigned kSampleKeyMasked = 0x007FFFFFu;   // sample_key(-inf)
 
 // the row's own constants
 struct SampleMass {
-  double zmax, y, scale;
+  struct Power { double b; int k; };   // 2^k b
+  double zmax, y, least;
+  int down;
   double c[12];   // of 2^f: (ln 2)^n / n!
   // top: max z.  An infinite one stands as a number above all others: what equals it has an argument above 0, everything else one far below
-  __device__ __forceinline__ SampleMass(float top, double log2e_T, int F)
-      : zmax(top < INFINITY ? (double)top : 1.7e308), y(log2e_T), scale(__hiloint2double((1023 + F) << 20, 0)) {
+  __device__ __forceinline__ SampleMass(float top, double log2e_T, int down_) : zmax(top < INFINITY ? (double)top : 1.7e308), y(log2e_T) {
+    scale(down_);
     constexpr double l = 0.69314718055994530942;
     c[0] = 1.0;
     c[1] = l;
@@ -110,28 +115,34 @@ struct SampleMass {
 #pragma unroll
     for (int n = 1; n < 12; ++n) asm("" : "+s"(c[n]));
   }
-  // log2 of e = exp((z - max z) / T); at -150 the mass is zero
-  __device__ __forceinline__ double arg(float z) const { return fmin(fmax(((double)z - zmax) * y, -150.0), 0.0); }
-  // 2^x for -150 <= x <= 0: x = k + f with |f| <= 1/2 (the sum with 1.5 2^52 rounds x to k and leaves it in the low word), the series of
-  // exp(f ln 2) to the 11th power (what is left out is below (ln 2 / 2)^12 / 12! = 7e-15), and k added to the exponent.
-  __device__ __forceinline__ double exp2(double x) const {
-    const double k = x + 0x1.8p52, f = x - (k - 0x1.8p52);
-    double e = c[11];
+  // masses as whole numbers of 2^(down_ - 61); at 2^least one is zero: least rounds to down_ - 61, a quarter below it
+  __device__ __forceinline__ void scale(int down_) {
+    down = down_;
+    least = (double)(down_ - 61) - 0.25;
+  }
+  // log2 of e = exp((z - max z) / T)
+  __device__ __forceinline__ double arg(float z) const { return fmin(fmax(((double)z - zmax) * y, least), 0.0); }
+  // 2^x for -62 < x <= 0: x = k + f with |f| <= 1/2 (the sum with 1.5 2^52 rounds x to k and leaves it in the low word), b = the series of
+  // exp(f ln 2) to the 11th power (what is left out is below (ln 2 / 2)^12 / 12! = 7e-15)
+  __device__ __forceinline__ Power power(float z) const {
+    const double x = arg(z), k = x + 0x1.8p52, f = x - (k - 0x1.8p52);
+    double b = c[11];
 #pragma unroll
-    for (int n = 10; n >= 0; --n) e = fma(e, f, c[n]);
-    return __hiloint2double(__double2hiint(e) + (__double2loint(k) << 20), __double2loint(e));
+    for (int n = 10; n >= 0; --n) b = fma(b, f, c[n]);
+    return Power{b, __double2loint(k)};
   }
-  __device__ __forceinline__ double e(float z) const { return exp2(arg(z)); }
-  // as a whole number of 2^-F (scale = 2^F <= 2^51: the sum with 2^52 rounds it to one, ties to even)
-  __device__ __forceinline__ unsigned long long whole(double e) const {
-    return (unsigned long long)__double_as_longlong(fma(e, scale, 0x1p52)) & ((1ull << 52) - 1);
+  static __device__ __forceinline__ double value(Power e) { return __hiloint2double(__double2hiint(e.b) + (e.k << 20), __double2loint(e.b)); }
+  // b < 1.42 in 52 bits (the sum with 2^52 rounds it to 2^-51), the sum's exponent shifted out, then down to the unit: at least 2, at most 63
+  // places, what falls off is dropped
+  __device__ __forceinline__ unsigned long long whole(Power e) const {
+    return ((unsigned long long)__double_as_longlong(fma(e.b, 0x1p51, 0x1p52)) << 12) >> (2 + down - e.k);
   }
-  __device__ __forceinline__ unsigned long long q(float z) const { return whole(e(z)); }
+  __device__ __forceinline__ unsigned long long q(float z) const { return whole(power(z)); }
   __device__ __forceinline__ unsigned long long q(float z, double m) const {   // ... zero for what min-p cuts
-    const double v = e(z);
-    return v >= m ? whole(v) : 0ull;
+    const Power e = power(z);
+    return value(e) >= m ? whole(e) : 0ull;
   }
-  // natural logarithm of a code's share of `total` (1 <= total / scale < 2^25): total / scale = 2^k b with 2/3 < b <= 4/3, and
+  // natural logarithm of a code's share of `total` (1 <= total 2^(down - 61) < 2^25): that is 2^k b with 2/3 < b <= 4/3, and
   // log b = 2 (s + s^3 / 3 + s^5 / 5 + ...), s = (b - 1) / (b + 1), |s| <= 1/5, to s^19 (what is left out is below 1e-15)
   __device__ __forceinline__ float logp(float z, unsigned long long total) const {
     const double v = (double)total;
@@ -141,7 +152,7 @@ struct SampleMass {
       b *= 0.5;
       ++k;
     }
-    k -= (__double2hiint(scale) >> 20) - 1023;
+    k -= 61 - down;
     const double s = (b - 1.0) * sample_reciprocal(b + 1.0), s2 = s * s;
     double p = 1.0 / 19.0;
     p = fma(p, s2, 1.0 / 17.0);
@@ -185,6 +196,8 @@ template <int CTRL, int ROWS>
 __device__ __forceinline__ unsigned long long sample_dpp(unsigned long long v) {
   return (unsigned long long)sample_dpp<CTRL, ROWS>((unsigned)(v >> 32)) << 32 | sample_dpp<CTRL, ROWS>((unsigned)v);
 }
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float sample_dpp(float v) { return __uint_as_float(sample_dpp<CTRL, ROWS>(__float_as_uint(v))); }
 template <typename T>
 __device__ __forceinline__ T sample_wave_scan(T v) {   // inclusive
   v += sample_dpp<0x111, 0xf>(v);
@@ -199,6 +212,7 @@ __device__ __forceinline__ unsigned sample_lane(unsigned v, int lane) { return (
 __device__ __forceinline__ unsigned long long sample_lane(unsigned long long v, int lane) {
   return (unsigned long long)sample_lane((unsigned)(v >> 32), lane) << 32 | sample_lane((unsigned)v, lane);
 }
+__device__ __forceinline__ float sample_lane(float v, int lane) { return __uint_as_float(sample_lane(__float_as_uint(v), lane)); }
 template <typename T>
 __device__ __forceinline__ T sample_wave_sum(T v) { return sample_lane(sample_wave_scan(v), 63); }
 __device__ __forceinline__ unsigned sample_wave_max(unsigned v) {
@@ -217,7 +231,7 @@ __device__ __forceinline__ void sample_wave_sync() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// Bins of the first look at a row, linear in z: 0 holds the largest logit, the last one the smallest, or whatever lies 54 or more powers
+// Bins of the first look at a row, linear in z: 0 holds the largest logit, the last one the smallest, or whatever lies 62 or more powers
 // of two below it (no mass).  fp32 subtraction and product are monotone and a NaN (both infinite) goes to the last bin with everything
 // that can be below it, so a bin never holds a logit above one of an earlier bin.
 struct SampleBins {
@@ -225,7 +239,7 @@ struct SampleBins {
   __device__ __forceinline__ int of(float z) const { return (int)fminf((zmax - z) * c, last); }
 };
 __device__ __forceinline__ SampleBins sample_bins(float zmax, float zmin, double y, int bins) {
-  const float range = fminf((zmax - zmin) * (float)y, 54.f);   // (any c > 0 will do: its rounding moves bins, not codes)
+  const float range = fminf((zmax - zmin) * (float)y, 62.f);   // (any c > 0 will do: its rounding moves bins, not codes)
   const float c = range > 0.f ? fminf((float)bins * (float)y * __builtin_amdgcn_rcpf(range), 3e38f) : 0.f;
   return SampleBins{zmax, zmax < INFINITY ? c : 0.f, (float)(bins - 1)};
 }
@@ -332,14 +346,14 @@ __global__ void __launch_bounds__(kSampleGroupThreads) sample_group_kernel(Sampl
     if (l == first) sample_answer(a, row, l * R + at, 0.f);
     return;
   }
-  const SampleMass mass(zmax, set.y, a.F);
+  const SampleMass mass(zmax, set.y, a.down);
   unsigned long long q[R];
   unsigned floored = 0;   // bit j: cut by min-p
 #pragma unroll
   for (int j = 0; j < R; ++j) {
-    const double e = mass.e(z[j]);
+    const SampleMass::Power e = mass.power(z[j]);
     q[j] = mass.whole(e);
-    floored |= (e >= set.m ? 0u : 1u) << j;
+    floored |= (mass.value(e) >= set.m ? 0u : 1u) << j;
     if ((j & 1) == 1) __builtin_amdgcn_sched_barrier(0);   // (two exponentials at a time: more side by side only take registers)
   }
   float t = -INFINITY;
@@ -595,7 +609,7 @@ struct SampleWaveRow {
 };
 
 template <typename T, int R>
-__global__ void __launch_bounds__(64 * kSampleRowWaves) sample_wave_kernel(SampleArgs a, long row0) {
+__global__ void __launch_bounds__(64 * kSampleRowWaves, 5) sample_wave_kernel(SampleArgs a, long row0) {
   __shared__ SampleWaveLds lds[kSampleRowWaves];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);   // (known to be the same in every lane: the row's settings are scalars)
   SampleWaveLds& s = lds[wave];
@@ -625,13 +639,13 @@ __global__ void __launch_bounds__(64 * kSampleRowWaves) sample_wave_kernel(Sampl
     if (lane == first) sample_answer(a, row, lane * R + at, 0.f);
     return;
   }
-  const SampleMass mass(zmax, set.y, a.F);
+  const SampleMass mass(zmax, set.y, a.down);
   unsigned floored = 0;   // bit j: cut by min-p
 #pragma unroll
   for (int j = 0; j < R; ++j) {
-    const double e = mass.e(w.z[j]);
+    const SampleMass::Power e = mass.power(w.z[j]);
     w.q[j] = mass.whole(e);
-    floored |= (e >= set.m ? 0u : 1u) << j;
+    floored |= (mass.value(e) >= set.m ? 0u : 1u) << j;
     if ((j & 3) == 3) __builtin_amdgcn_sched_barrier(0);   // (four exponentials at a time: more side by side only take registers)
   }
   float t = -INFINITY;
@@ -929,7 +943,7 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a, long 
   __shared__ unsigned bin_count[kSampleBins];
   __shared__ SampleBlock<NT> blk;
   __shared__ SampleFound found;
-  __shared__ unsigned range[2][NT / 64], key_range[2];
+  __shared__ unsigned range[2][NT / 64], key_range[2], upper;
   __shared__ unsigned long long m_mass[64];
   __shared__ float m_z[64];
   __shared__ int n_listed[2];   // by top-k, by top-p
@@ -990,6 +1004,7 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a, long 
     bin_count[tid + j * NT] = 0;
   }
   if (tid < 2) n_listed[tid] = 0;
+  if (tid == 0) upper = 0;
   __syncthreads();
   khi = sample_wave_max(lane < NT / 64 ? range[0][lane] : 0u);
   klo = sample_wave_max(lane < NT / 64 ? range[1][lane] : 0u);
@@ -1010,19 +1025,27 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a, long 
     }
     return;
   }
-  const SampleMass mass(zmax, set.y, a.F);
+  SampleMass mass(zmax, set.y, 0);
   unsigned long long q[R];
   unsigned floored = 0;   // bit j: cut by min-p
+  // masses of the codes from `least` on, then down to what their sum leaves room for: it is below (the sum of their upper 17 bits + V) 2^47
   auto weigh = [&](float least) {
 #pragma unroll
     for (int j = 0; j < R; ++j) q[j] = 0;
+    unsigned sum = 0;
     each([&](int j, float x) {
       if (x >= least) {
-        const double e = mass.e(x);
+        const SampleMass::Power e = mass.power(x);
         q[j] = mass.whole(e);
-        floored |= (e >= set.m ? 0u : 1u) << j;
+        floored |= (mass.value(e) >= set.m ? 0u : 1u) << j;
+        sum += (unsigned)(q[j] >> 47);
       }
     });
+    sum = sample_wave_sum(sum);
+    if (lane == 0) atomicAdd(&upper, sum);
+    __syncthreads();
+    mass.scale(max(17 - __builtin_clz((unsigned)__builtin_amdgcn_readfirstlane((int)upper) + (unsigned)V), 0));
+    each([&](int j, float) { q[j] >>= mass.down; });
   };
   float t = -INFINITY;
   unsigned r = 0;
@@ -1258,7 +1281,7 @@ constexpr int kSampleFewChunks = 4;             // up to which the bins are summ
 constexpr int kSampleHere = 2048;               // members of a chunk listed one by one; with more, equal ones as one
 constexpr int kSampleMembers = 4096;            // members of a row that the last kernel holds in LDS
 
-// Bins of such a row: 128 to a power of two of 1 + s (max z - z), eight powers down to where nothing has mass (54 / y) or the smallest
+// Bins of such a row: 128 to a power of two of 1 + s (max z - z), eight powers down to where nothing has mass (62 / y) or the smallest
 // logit.  Next to the largest logit they are 30 times as fine as linear ones (logits that hardly differ, beside masks of the type's lowest
 // value, would all lie in one of those), where a cut of ordinary logits falls twice as coarse.  Sum, product and the bits of a positive fp32 are monotone; a NaN goes to the last bin.
 struct SampleLogBins {
@@ -1269,13 +1292,14 @@ struct SampleLogBins {
   }
 };
 __device__ __forceinline__ SampleLogBins sample_log_bins(float zmax, float zmin, double y) {
-  const float d = fminf(zmax - zmin, (float)fmin(fmax(54.0 / y, 1e-36), 3e38));
+  const float d = fminf(zmax - zmin, (float)fmin(fmax(62.0 / y, 1e-36), 3e38));
   return SampleLogBins{zmax, d > 0.f && zmax < INFINITY ? fminf(255.f / d, 3e38f) : 0.f};
 }
 
 struct SampleState {                   // of a row
   float zmax, zmin;
   unsigned first;                      // lowest index of the largest logit
+  int down;                            // of its masses
   int kb;                              // the bin that top-k cuts; kSampleBins: none
   unsigned want;                       // codes kept of it
   int b0, b1;                          // bins that the last cut falls into; kSampleBins: no cut
@@ -1293,6 +1317,7 @@ struct SampleLong {
   int most;                            // members that a row's list holds (with more the last kernel searches the row itself)
   unsigned long long* best;            // [row][chunk] key of the largest logit << 32 | ~lowest index that holds it
   unsigned* least;                     // [row][chunk] ~key of the smallest logit that is not -inf
+  float* sum;                          // [row][chunk] sum of 2^(log2 e - the chunk's largest), roughly
   int* floor;                          // [row][chunk] first bin with a code that min-p cuts
   unsigned long long* mass;            // [row][chunk][bin]
   unsigned* count;
@@ -1319,10 +1344,19 @@ __device__ __forceinline__ void sample_load_chunk(const SampleArgs& a, const T* 
   }
 }
 
+// 2^((z - top) log2(e) / T) in 32 bits, never below what it stands for by more than 2^-14 of itself: the difference in halves (that of two fp32
+// may be infinite), y2 = twice the factor (a tiny one may be 0, a huge one is cut off), and 1 where that is no number (0 inf, inf - inf)
+__device__ __forceinline__ float sample_rough(float z, float top, float y2) {
+  return __builtin_amdgcn_exp2f(fminf(fmaf(z, 0.5f, -0.5f * top) * y2, 0.f));
+}
+__device__ __forceinline__ float sample_rough_factor(double y) { return 2.f * (float)fmin(y, 1.5e38); }
+
 template <typename T>
 __global__ void __launch_bounds__(kSampleChunkThreads) sample_range_kernel(SampleArgs a, SampleLong l) {
   __shared__ unsigned sh[3][kSampleChunkThreads / 64];
+  __shared__ float sh_sum[kSampleChunkThreads / 64];
   const long r = blockIdx.x / l.chunks;
+  const SampleRow set = sample_row(a, l.row0 + r);
   const int c = blockIdx.x - (int)(r * l.chunks), i0 = c * kSampleChunk, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   float z[kSampleChunkIpt], hi = -INFINITY, lo = INFINITY;
   sample_load_chunk(a, reinterpret_cast<const T*>(a.logits) + (l.row0 + r) * a.stride, i0, z);
@@ -1344,13 +1378,25 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_range_kernel(Sampl
     sh[2][w] = least;
   }
   __syncthreads();
+  const bool in = lane < kSampleChunkThreads / 64;
+  const unsigned t = in ? sh[0][lane] : 0u, all = sample_wave_max(t);
+  // the chunk's sum next to its largest logit: every row's masses are scaled by its own
+  float sum = 0.f;
+  if (!set.greedy) {
+    const float best = sample_unkey(all), y2 = sample_rough_factor(set.y);
+#pragma unroll
+    for (int j = 0; j < kSampleChunkIpt; ++j) sum += sample_rough(z[j], best, y2);
+    sum = sample_wave_sum(sum);
+    if (lane == 0) sh_sum[w] = sum;
+    __syncthreads();
+  }
   if (w == 0) {
-    const bool in = lane < kSampleChunkThreads / 64;
-    const unsigned t = in ? sh[0][lane] : 0u, all = sample_wave_max(t);
+    sum = sample_wave_sum(in && !set.greedy ? sh_sum[lane] : 0.f);
     const unsigned i = sample_wave_max(in && t == all ? sh[1][lane] : 0u), s = sample_wave_max(in ? sh[2][lane] : 0u);
     if (lane == 0) {
       l.best[r * l.chunks + c] = (unsigned long long)all << 32 | i;
       l.least[r * l.chunks + c] = s;
+      l.sum[r * l.chunks + c] = sum;
     }
   }
 }
@@ -1358,37 +1404,45 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_range_kernel(Sampl
 struct SampleRange {
   float zmax, zmin;
   unsigned first;
+  int down;
 };
-// the row's range from its chunks'; every thread.  Ends with a barrier.
-__device__ __forceinline__ SampleRange sample_range(const SampleLong& l, long r, unsigned* sh) {
+// the row's range from its chunks', and how far its masses go down: the row's sum is below 2^(down + 1) times the largest, so that of the masses
+// below 2^62.  y: log2(e) / T.  Every thread.  Ends with a barrier.  (In the same order in every kernel: the same number.)
+__device__ __forceinline__ SampleRange sample_range(const SampleLong& l, long r, double y, unsigned* sh) {
   if (threadIdx.x < 64) {
     const int lane = threadIdx.x;
-    unsigned top = 0, at = 0, least = 0;
+    const float y2 = sample_rough_factor(y);
+    unsigned top = kSampleKeyMasked, at = 0, least = 0;
+    float sum = 0.f;   // next to `top`
     for (int c = lane; c < l.chunks; c += 64) {
       const unsigned long long b = l.best[r * l.chunks + c];
       const unsigned t = (unsigned)(b >> 32);
+      const float was = sample_unkey(top), z = sample_unkey(t), best = fmaxf(was, z);
       at = t > top ? (unsigned)b : (t == top ? max(at, (unsigned)b) : at);
       top = max(top, t);
       least = max(least, l.least[r * l.chunks + c]);
+      sum = sum * sample_rough(was, best, y2) + l.sum[r * l.chunks + c] * sample_rough(z, best, y2);
     }
     const unsigned all = sample_wave_max(top);
     at = sample_wave_max(top == all ? at : 0u);
     least = sample_wave_max(least);
+    sum = sample_wave_sum(sum * sample_rough(sample_unkey(top), sample_unkey(all), y2));
     if (lane == 0) {
       sh[0] = all;
       sh[1] = ~least;
       sh[2] = ~at;
+      sh[3] = (unsigned)max((int)(__float_as_uint(sum * 1.01f) >> 23) - 127, 0);
     }
   }
   __syncthreads();
-  return SampleRange{sample_unkey(sh[0]), sample_unkey(sh[1]), sh[2]};
+  return SampleRange{sample_unkey(sh[0]), sample_unkey(sh[1]), sh[2], (int)sh[3]};
 }
 
 template <typename T>
 __global__ void __launch_bounds__(kSampleChunkThreads) sample_bins_kernel(SampleArgs a, SampleLong l) {
   __shared__ unsigned long long bin_mass[kSampleBins];
   __shared__ unsigned bin_count[kSampleBins];
-  __shared__ unsigned sh[3];
+  __shared__ unsigned sh[4];
   __shared__ int floor;
   static_assert(kSampleBins == kSampleChunkThreads, "a thread owns a bin");
   const long r = blockIdx.x / l.chunks;
@@ -1399,20 +1453,20 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_bins_kernel(Sample
   bin_mass[tid] = 0;
   bin_count[tid] = 0;
   if (tid == 0) floor = kSampleBins;
-  const SampleRange g = sample_range(l, r, sh);   // (its barrier: the bins are cleared)
+  const SampleRange g = sample_range(l, r, set.y, sh);   // (its barrier: the bins are cleared)
   if (g.zmax == -INFINITY || set.greedy) return;
-  const SampleMass mass(g.zmax, set.y, a.F);
+  const SampleMass mass(g.zmax, set.y, g.down);
   const SampleLogBins bins = sample_log_bins(g.zmax, g.zmin, set.y);
   const bool by_count = set.k < a.V, by_floor = set.m > 0.0;
   int first = kSampleBins;
 #pragma unroll
   for (int j = 0; j < kSampleChunkIpt; ++j) {
     const int b = bins.of(z[j]);
-    const double e = mass.e(z[j]);
+    const SampleMass::Power e = mass.power(z[j]);
     const unsigned long long q = mass.whole(e);
     if (by_count && z[j] > -INFINITY) atomicAdd(&bin_count[b], 1u);
     if (q) atomicAdd(&bin_mass[b], q);
-    if (by_floor) first = min(first, e >= set.m || z[j] == -INFINITY ? kSampleBins : b);
+    if (by_floor) first = min(first, mass.value(e) >= set.m || z[j] == -INFINITY ? kSampleBins : b);
     if (j & 1) __builtin_amdgcn_sched_barrier(0);
   }
   if (first < kSampleBins) atomicMin(&floor, first);
@@ -1427,16 +1481,16 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_bins_kernel(Sample
 // 47; with bins, cuts and members all the same 32 and 67).
 template <typename T>
 __global__ void __launch_bounds__(kSampleChunkThreads) sample_mass_kernel(SampleArgs a, SampleLong l) {
-  __shared__ unsigned sh[3];
+  __shared__ unsigned sh[4];
   __shared__ unsigned long long part[kSampleChunkThreads / 64];
   const long r = blockIdx.x / l.chunks;
   const int c = blockIdx.x - (int)(r * l.chunks), lane = threadIdx.x & 63;
   const SampleRow set = sample_row(a, l.row0 + r);
   float z[kSampleChunkIpt];
   sample_load_chunk(a, reinterpret_cast<const T*>(a.logits) + (l.row0 + r) * a.stride, c * kSampleChunk, z);
-  const SampleRange g = sample_range(l, r, sh);
+  const SampleRange g = sample_range(l, r, set.y, sh);
   if (g.zmax == -INFINITY || set.greedy) return;
-  const SampleMass mass(g.zmax, set.y, a.F);
+  const SampleMass mass(g.zmax, set.y, g.down);
   unsigned long long sum = 0;
 #pragma unroll
   for (int j = 0; j < kSampleChunkIpt; ++j) {
@@ -1485,15 +1539,16 @@ __global__ void __launch_bounds__(1024) sample_cuts_kernel(SampleArgs a, SampleL
   constexpr int NT = 1024;
   __shared__ SampleBlock<NT> blk;
   __shared__ SampleState st;
-  __shared__ unsigned sh[3];
+  __shared__ unsigned sh[4];
   const int tid = threadIdx.x;
   const long r = blockIdx.x;
   const SampleRow set = sample_row(a, l.row0 + r);
-  const SampleRange g = sample_range(l, r, sh);
+  const SampleRange g = sample_range(l, r, set.y, sh);
   if (tid == 0) {
     st.zmax = g.zmax;
     st.zmin = g.zmin;
     st.first = g.first;
+    st.down = g.down;
     st.kb = st.b0 = st.b1 = st.fb = kSampleBins;
     st.want = 0;
     st.n_members = 0;
@@ -1682,7 +1737,7 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
   __shared__ unsigned m_where[kSampleMembers];
   __shared__ unsigned long long chunk[kSampleMaxChunks];
   __shared__ unsigned chunk_ties[kSampleMaxChunks];
-  __shared__ unsigned key_range[2], sh_range[3];
+  __shared__ unsigned key_range[2], sh_range[4];
   __shared__ int sh_chunk;
   __shared__ unsigned sh_tied;
   __shared__ unsigned long long sh_before;
@@ -1691,10 +1746,11 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
   const SampleRow set = sample_row(a, row);
   SampleState st{};
   if (l.uncut) {
-    const SampleRange g = sample_range(l, r, sh_range);
+    const SampleRange g = sample_range(l, r, set.y, sh_range);
     st.zmax = g.zmax;
     st.zmin = g.zmin;
     st.first = g.first;
+    st.down = g.down;
     st.kb = st.b0 = st.b1 = st.fb = kSampleBins;
   } else {
     st = l.state[r];
@@ -1706,7 +1762,7 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
     }
     return;
   }
-  const SampleMass mass(st.zmax, set.y, a.F);
+  const SampleMass mass(st.zmax, set.y, st.down);
   const SampleLogBins bins = sample_log_bins(st.zmax, st.zmin, set.y);
   const T* logits = reinterpret_cast<const T*>(a.logits) + row * a.stride;
   const bool listed = st.n_members <= l.most, held = st.n_members <= kSampleMembers;   // (else the row itself is the list)

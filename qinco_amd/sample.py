@@ -81,8 +81,9 @@ def sample_codes(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, c
     `top_k`, of these every one with less than `top_p` of their mass before it (the first always), of these those with e_i >= `min_p`;
     the code is the lowest kept index at which the kept mass, summed in index order, exceeds u times its total.  top_k <= 0 or >= V,
     top_p >= 1 and min_p <= 0 switch a cut off.  temperature 0 takes the largest logit, the lowest index among equals (log probability
-    0).  -inf and NaN are never drawn; a row with nothing to draw answers -1 with log probability -inf.  Decisions are taken in 64 bits:
-    the same inputs give the same codes, whatever else is in the batch.
+    0).  -inf and NaN are never drawn; a row with nothing to draw answers -1 with log probability -inf.  The same inputs give the same
+    codes, whatever else is in the batch.  Masses and sums are held in 62 bits of the row's total: top_p and u decide as in exact arithmetic
+    unless they lie within 2^-43 of a border (V <= 20480; 2^-39 at 2^20 codes, 2^-35 at 2^24).
 
     temperature, top_p, min_p (float32) and top_k (int32) may be tensors (n,) with a value per row; there a temperature <= 0 is 0."""
     lib = _lib.load()

@@ -775,3 +775,68 @@ def test_together_with_the_search_and_the_look_up_decoder():
     moved = first.gather(codes.to(torch.uint8))
     assert bool((moved[:, 0].diff().int() >= 0).all())
     knn.close(), dec.close()
+
+
+# ------------------------------------------------------------------------------------------------ far tails, long rows, many rows
+def tail_border(V, e, x):
+    """One code of mass 1 at index 0, V - 1 of mass e behind it (exact, a Fraction): the code that a share x of the total falls on."""
+    at = (x * (1 + (V - 1) * e) - 1) / e                      # tail masses behind the peak's
+    return 0 if at < 0 else 1 + int(at)
+
+
+@gpu
+@pytest.mark.parametrize("V,gap", [(60, 33.0), (100, 34.0), (200, 35.0), (500, 35.0), (600, 37.0), (1500, 36.5), (4099, 35.0), (10240, 35.0), (20480, 33.5), (20480, 27.0), (20481, 33.5), (70001, 32.0), (1 << 20, 30.0),
+                                   ((1 << 22) + 1, 27.0), (1 << 24, 28.0), (1 << 24, 27.0)])
+def test_sample_flat_tails_far_below_the_largest_logit(V, gap):
+    """A tail whose codes have 2^-39 to 2^-54 of the largest one's mass each is drawn as often as its share of the row says.  Against whole
+    fractions.  A code's mass is held to 2^-44 of itself (the exponential) and a step of at most 2.25 2^-61 of the row's total (up to 512 codes of
+    2^-62 for each power of two in V), products with u and p to 2^-52: the code drawn is that many tail masses off at most."""
+    import torch
+    from fractions import Fraction as Fr
+    from decimal import Decimal, localcontext
+    from qinco_amd import sample_codes
+    with localcontext() as ctx:
+        ctx.prec = 60
+        e = Fr(Decimal(-gap).exp())
+    total, tail = 1 + (V - 1) * e, (V - 1) * e
+    step = Fr(9, 1 << 63) if V > 512 else Fr(1, 1 << (62 - (V - 1).bit_length()))
+    off = math.ceil((V * step + Fr(1, 1 << 51)) * total / e + V * Fr(1, 1 << 44) + 1)
+    assert off < V / 5                                        # (else the case says little)
+    z = torch.full((1, V), -gap, device="cuda")
+    z[0, 0] = 0.0
+    u = [0.3, 1.0 - float(tail / 2), 1.0 - float(tail / 5), 1.0 - float(tail * 4 / 5), 1.0 - float(tail * 2)]
+    for n in (5, 300, 2500) if V <= 20480 else (5,):          # (many rows go another way)
+        uu = torch.tensor(u, dtype=torch.float64, device="cuda").repeat(n // 5)
+        zz = z.expand(n, V)
+        for s in (dict(), dict(min_p=1e-30), dict(top_k=V - 1)):
+            count = V - (1 if "top_k" in s else 0)            # top-k drops the last of the equal ones
+            codes, logp = sample_codes(zz, uu, return_logp=True, **s)
+            want = [tail_border(count, e, Fr(x)) for x in u]
+            assert want[0] == want[4] == 0 and all(V // 8 < w < V for w in want[1:4])
+            codes, logp = codes.view(-1, 5), logp.view(-1, 5)
+            assert bool((codes == codes[:1]).all()) and bool((logp == logp[:1]).all())
+            got = codes[0].tolist()
+            assert got[0] == got[4] == 0 and all(abs(g - w) <= off for g, w in zip(got, want)), (s, got, want, off)
+            share = math.log1p(float((count - 1) * e))
+            assert abs(float(logp[0, 0]) + share) <= 2.0 ** -24 * share + 2.0 ** -44 + V * float(step)
+            assert abs(float(logp[0, 1]) + gap + share) <= 2.0 ** -23 * gap
+        keep = 1.0 - float(tail / 2)                          # top-p cuts the tail in the middle
+        got = sample_codes(zz, torch.full((n,), 1.0 - 2.0 ** -53, dtype=torch.float64, device="cuda"), top_p=keep)
+        assert bool((got == got[0]).all()) and abs(int(got[0]) - tail_border(V, e, Fr(keep))) <= 2 * off
+
+
+@gpu
+@pytest.mark.parametrize("V,dtype", [((1 << 22) + 1, "float32"), (1 << 24, "bfloat16")])
+def test_sample_longest_rows(V, dtype):
+    """Against the plain statement, whose own sums in 64 bits are good to V 2^-53 of the total."""
+    import torch
+    from qinco_amd import sample_codes
+    g = torch.Generator("cuda").manual_seed(V)
+    z = (torch.randn(2, V, generator=g, device="cuda") * 2.5).to(getattr(torch, dtype))
+    z[1, : V // 3] = -float("inf")
+    z[1, V // 2] = float("nan")
+    check_sample(z, torch.rand(2, generator=g, device="cuda"))
+    check_sample(z, torch.rand(2, generator=g, device="cuda"), T=0.7, k=1000, p=0.9, m=1e-3)
+    z[0, V - 1] = 100.0
+    z[1, V - 2:] = 100.0
+    assert sample_codes(z, torch.rand(2, generator=g, device="cuda"), temperature=0.0).tolist() == [V - 1, V - 2]
