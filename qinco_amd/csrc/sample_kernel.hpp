@@ -168,6 +168,13 @@ struct SampleMass {
   }
 };
 
+// A logit that no code of mass is at or below: 62 powers of two under the largest one, and one fp32 further down.  A top-k that reaches codes
+// without mass changes nothing, so they are not counted, nor sought in their bin (which most of a row can share).
+__device__ __forceinline__ float sample_massless(float zmax, double y) {
+  const double z = (zmax < INFINITY ? (double)zmax : 1.7e308) - 62.0 * sample_reciprocal(y);
+  return sample_unkey(sample_key((float)fmax(z, -3.40282346638528859812e38)) - 1);   // (below the lowest fp32: -inf)
+}
+
 // smallest whole number that is at least p * total (and at least 1): "mass before < p * total" is "mass before < this"
 __device__ __forceinline__ unsigned long long sample_bound(double p, unsigned long long total) {
   const unsigned long long v = (unsigned long long)ceil(p * (double)total);
@@ -362,6 +369,7 @@ __global__ void __launch_bounds__(kSampleGroupThreads) sample_group_kernel(Sampl
   if (by_count || by_mass) {
     const float zmin = sample_unkey(~sample_row_max<G>(~sample_key(lo)));
     const SampleBins bins = sample_bins(zmax, zmin, set.y, 64);
+    const float massless = sample_massless(zmax, set.y);
 #pragma unroll
     for (int j = 0; j < PB; ++j) {
       s.mass[l * PB + j] = 0;
@@ -371,7 +379,7 @@ __global__ void __launch_bounds__(kSampleGroupThreads) sample_group_kernel(Sampl
 #pragma unroll
     for (int j = 0; j < R; ++j) {
       const int b = bins.of(z[j]);
-      if (z[j] > -INFINITY) atomicAdd(&s.count[b], 1u);
+      if (z[j] > massless) atomicAdd(&s.count[b], 1u);
       if (q[j]) atomicAdd(&s.mass[b], q[j]);
     }
     sample_wave_sync();
@@ -389,7 +397,7 @@ __global__ void __launch_bounds__(kSampleGroupThreads) sample_group_kernel(Sampl
     auto members = [&](int b) {
       unsigned in = 0;
 #pragma unroll
-      for (int j = 0; j < R; ++j) in |= (unsigned)(z[j] > -INFINITY && bins.of(z[j]) == b) << j;
+      for (int j = 0; j < R; ++j) in |= (unsigned)(z[j] > massless && bins.of(z[j]) == b) << j;
       const unsigned n = __builtin_popcount(in), run = sample_row_scan<G>(n);
       unsigned to = run - n;
       if (in) {
@@ -595,7 +603,7 @@ struct SampleWaveRow {
     int n = 0;
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      const bool in = z[j] > -INFINITY && bins.of(z[j]) == b;
+      const bool in = q[j] && bins.of(z[j]) == b;
       const unsigned long long at = __ballot(in);
       const int to = n + (int)__builtin_popcountll(at & ((1ull << lane) - 1));
       if (in && to < 64) {
@@ -659,7 +667,7 @@ __global__ void __launch_bounds__(64 * kSampleRowWaves, 5) sample_wave_kernel(Sa
     sample_wave_sync();
 #pragma unroll
     for (int j = 0; j < R; ++j) {
-      if (w.z[j] > -INFINITY) {
+      if (w.q[j]) {
         const int b = bins.of(w.z[j]);
         atomicAdd(&s.count[b], 1u);
         atomicAdd(&s.mass[b], w.q[j]);
@@ -1047,14 +1055,14 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a, long 
     mass.scale(max(17 - __builtin_clz((unsigned)__builtin_amdgcn_readfirstlane((int)upper) + (unsigned)V), 0));
     each([&](int j, float) { q[j] >>= mass.down; });
   };
-  float t = -INFINITY;
+  float t = sample_massless(zmax, set.y);
   unsigned r = 0;
   const bool by_mass = set.p < 1.0;
-  if (by_mass) weigh(-INFINITY);
+  if (by_mass) weigh(t);
   if (set.k < V || by_mass) {
     const SampleBins bins = sample_bins(zmax, sample_unkey(~klo), set.y, kSampleBins);
     each([&](int j, float x) {
-      if (x > -INFINITY) {
+      if (x > t) {
         const int b = bins.of(x);
         atomicAdd(&bin_count[b], 1u);
         if (by_mass && q[j]) atomicAdd(&bin_mass[b], q[j]);
@@ -1157,7 +1165,7 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a, long 
         unsigned long long before;
         const unsigned key = sample_search<NT>(blk, found, part, first, last, want, before, [&](auto f) {
           each([&](int j, float x) {
-            if (x > -INFINITY && bins.of(x) == kb) f(sample_key(x), [] { return 1ull; });
+            if (x > t && bins.of(x) == kb) f(sample_key(x), [] { return 1ull; });
           });
         });
         t = sample_unkey(key);
@@ -1464,8 +1472,10 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_bins_kernel(Sample
     const int b = bins.of(z[j]);
     const SampleMass::Power e = mass.power(z[j]);
     const unsigned long long q = mass.whole(e);
-    if (by_count && z[j] > -INFINITY) atomicAdd(&bin_count[b], 1u);
-    if (q) atomicAdd(&bin_mass[b], q);
+    if (q) {
+      if (by_count) atomicAdd(&bin_count[b], 1u);
+      atomicAdd(&bin_mass[b], q);
+    }
     if (by_floor) first = min(first, mass.value(e) >= set.m || z[j] == -INFINITY ? kSampleBins : b);
     if (j & 1) __builtin_amdgcn_sched_barrier(0);
   }
@@ -1599,6 +1609,7 @@ __global__ void __launch_bounds__(1024) sample_cuts_kernel(SampleArgs a, SampleL
   __syncthreads();
   if (tid < 6) {   // the ends of the members' logits: the bins are monotone, so each is found bit by bit over the keys
     const SampleLogBins bins = sample_log_bins(g.zmax, g.zmin, set.y);
+    const unsigned massless = sample_key(sample_massless(g.zmax, set.y));
     const int which = tid >> 1;
     const int x = which == 0 ? st.b0 : which == 1 ? st.kb : st.fb, y = which == 0 ? st.b1 : x;
     unsigned key = 0;   // tid even: the largest key whose bin is behind y (lo is the one above it); odd: the largest whose bin is x or behind it
@@ -1610,7 +1621,7 @@ __global__ void __launch_bounds__(1024) sample_cuts_kernel(SampleArgs a, SampleL
     }
     const bool none = x >= kSampleBins || (which == 2 && st.fb >= st.b0);
     if (tid & 1) st.hi[which] = none ? -INFINITY : sample_unkey(key);
-    else st.lo[which] = none ? INFINITY : sample_unkey(max(key, kSampleKeyMasked) + 1);
+    else st.lo[which] = none ? INFINITY : sample_unkey(max(key, massless) + 1);
   }
   __syncthreads();
   if (tid == 0) l.state[r] = st;
@@ -1767,6 +1778,7 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
   const T* logits = reinterpret_cast<const T*>(a.logits) + row * a.stride;
   const bool listed = st.n_members <= l.most, held = st.n_members <= kSampleMembers;   // (else the row itself is the list)
   const int n = listed ? st.n_members : a.V;
+  const float massless = sample_massless(st.zmax, set.y);
   chunk[tid] = listed && tid < l.chunks ? l.chunk_mass[r * l.chunks + tid] : 0ull;
   chunk_ties[tid] = 0;
   if (tid == 0) {
@@ -1786,7 +1798,7 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
       for (int i = tid; i < n; i += NT) {
         const float z = listed ? l.m_z[r * l.most + i] : sample_logit(logits, i, a.V);
         const unsigned at = listed ? l.m_where[r * l.most + i] : (unsigned)(i / kSampleChunk) << 15 | 1u;
-        if (z > -INFINITY) f(z, at & 0x7FFFu, at >> 15);
+        if (z > massless) f(z, at & 0x7FFFu, at >> 15);
       }
     }
   };
@@ -1810,7 +1822,7 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_finish_kernel(Samp
   }
   __syncthreads();
   const unsigned kmin = key_range[0], kmax = key_range[1];
-  float t = -INFINITY;
+  float t = massless;
   unsigned ties = 0;   // codes kept of those at t
   unsigned long long qt = 0, before, all = 0;
   unsigned none, none_all;

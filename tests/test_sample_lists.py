@@ -840,3 +840,35 @@ def test_sample_longest_rows(V, dtype):
     z[0, V - 1] = 100.0
     z[1, V - 2:] = 100.0
     assert sample_codes(z, torch.rand(2, generator=g, device="cuda"), temperature=0.0).tolist() == [V - 1, V - 2]
+
+
+@gpu
+@pytest.mark.parametrize("V", [60, 200, 500, 3000, 20000, 70001, 1 << 20])
+def test_sample_top_k_among_codes_without_mass(V):
+    """Where the k-th code is too far below the largest to have any mass, top-k changes nothing, and costs a long row nothing either: it is not
+    sought among the many codes that share its bin."""
+    import torch
+    from qinco_amd import sample_codes
+    g = torch.Generator("cuda").manual_seed(V)
+    z = torch.randn(3, V, generator=g, device="cuda") * 2.5
+    z[1, V // 3] = 100.0                                                       # one code far above the rest, all different
+    z[2] = (z[2] * 4).round()
+    u = torch.rand(3, generator=g, device="cuda", dtype=torch.float64)
+    for T in (0.02, 0.3):
+        for k in (2, 40, V // 3, V - 1):
+            check_sample(z, u, T=T, k=k)
+            check_sample(z, u, T=T, k=k, p=0.7)
+    if V <= 20480:
+        return
+
+    def least(**s):
+        times = []
+        for _ in range(10):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            sample_codes(z[1:2], u[1:2], **s)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+    assert least(top_k=V // 2) < 4 * least(min_p=1e-30)
