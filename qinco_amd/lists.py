@@ -3,11 +3,13 @@
 `group_rows` sorts the entries of (n, k) list ids by list: the IVF column of a code matrix (k = 1, filling an index, reference
 qinco/search/search_utils.py:121-162) or the k nearest centroids of `KnnSearcher.search` (multi-probe, a router).  `RowGroups.gather`
 carries rows into that order, `RowGroups.combine` brings them back with weights; both have gradients.  All of it can be captured into a graph
-(`check=False`); a captured backward pass wants leaves that no eager graph holds at the same time, as torch's own operators do.
+(`check=False`); a captured backward pass wants leaves that no eager graph holds at the same time, as torch's own operators do.  Forward-mode
+and second derivatives are refused.
 """
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -54,6 +56,14 @@ def group_rows(lists, n_lists: int, check: bool = True) -> "RowGroups":
     return groups
 
 
+def _no_tangents(*tensors):
+    """Forward-mode derivatives are refused: a library call would answer its values without them."""
+    if forward_ad._current_level >= 0:                 # (between dual levels there are none)
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise NotImplementedError("gather and combine have no forward-mode derivatives")
+
+
 class RowGroups:
     """Entries in list order (int32 CUDA tensors):
       order   (n k,)         entry row * k + slot in each place; -1 behind the last place in use
@@ -95,6 +105,7 @@ class RowGroups:
         """x (n, D) of any type, also code rows -> (n k, D): row order[s] // k at place s, zeros behind the last place in use.
         The gradient is the sum over a row's places, in 32 bits, rounded once (float32, float16, bfloat16)."""
         x = self._rows(x, self.n, "x")
+        _no_tangents(x)
         if x.requires_grad and torch.is_grad_enabled():
             row_type(x, "x that requires a gradient")
             return _Gather.apply(x, self)
@@ -110,6 +121,7 @@ class RowGroups:
             if on_device(weights, "weights").shape != (self.n, self.k) or weights.dtype not in (torch.float32, y.dtype) or weights.device != y.device:
                 raise ValueError(f"weights must be ({self.n}, {self.k}) float32 or {y.dtype} on {y.device}, got {tuple(weights.shape)} {weights.dtype}")
             weights = as_stored(weights).contiguous()
+        _no_tangents(y, weights)
         if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
             return _Combine.apply(y, weights, self)
         return self._combine(y, weights)
@@ -142,10 +154,12 @@ class RowGroups:
 
 
 def _gather_grad(ctx, dout):
+    _no_tangents(dout)
     return ctx.groups._combine(unit_rows(dout), None), None
 
 
 def _combine_grad(ctx, dout):
+    _no_tangents(dout)
     dout = unit_rows(dout)
     if not ctx.weighted:
         return ctx.groups._gather(dout), None, None

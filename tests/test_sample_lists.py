@@ -872,3 +872,39 @@ def test_sample_top_k_among_codes_without_mass(V):
             times.append(a.elapsed_time(b))
         return min(times)
     assert least(top_k=V // 2) < 4 * least(min_p=1e-30)
+
+
+# ------------------------------------------------------------------------------------------------ derivatives and traces (no GPU: without the calls)
+@pytest.fixture
+def no_calls(monkeypatch):
+    """Host tensors go through the Python side; the library calls are left out."""
+    from qinco_amd import lists, sample
+    for m in (lists, sample):
+        monkeypatch.setattr(m, "on_device", lambda t, what: t)
+        monkeypatch.setattr(m, "on_its_device", lambda index, call, *args: None)
+    return lists
+
+
+def host_groups(lists, n=4, k=2):
+    import torch
+    place = torch.arange(n * k, dtype=torch.int32)
+    return lists.RowGroups(place, place.view(n, k), torch.tensor([0, n * k], dtype=torch.int32))
+
+
+def test_forward_mode_derivatives_are_refused(no_calls):
+    import torch
+    import torch.autograd.forward_ad as fa
+    g = host_groups(no_calls)
+    x, y, w = torch.randn(4, 3), torch.randn(8, 3), torch.rand(4, 2)
+    with fa.dual_level():
+        dual = lambda t: fa.make_dual(t, torch.ones_like(t))                   # noqa: E731
+        for call in (lambda: g.gather(dual(x)), lambda: g.gather(dual(x.cfloat())), lambda: g.combine(dual(y)), lambda: g.combine(dual(y), w), lambda: g.combine(y, dual(w)),
+                     lambda: g.combine(dual(y.T.contiguous().T), w)):
+            for mode in (torch.enable_grad, torch.no_grad):
+                with mode(), pytest.raises(NotImplementedError):
+                    call()
+        assert g.gather(x).shape == (8, 3) and g.gather(x.int()).shape == (8, 3) and g.combine(y, w).shape == (4, 3)   # nothing to lose
+        for out, leaves in ((g.gather(x.requires_grad_()), x), (g.combine(y.requires_grad_()), y), (g.combine(y, w.requires_grad_()), (y, w))):
+            torch.autograd.grad(out, leaves, torch.ones_like(out), retain_graph=True)
+            with pytest.raises(NotImplementedError):                           # ... of a backward pass
+                torch.autograd.grad(out, leaves, dual(torch.ones_like(out)))
