@@ -13,7 +13,7 @@ from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .sample import _TYPES, as_stored, on_device, on_its_device, row_type, unit_rows
+from .sample import _TYPES, as_stored, being_traced, not_traced, on_device, on_its_device, row_type, unit_rows
 
 MAX_LISTS = 1 << 24
 _IDS = {torch.int64: _lib.CODE_I64, torch.int32: _lib.CODE_I32, torch.uint8: _lib.CODE_U8}
@@ -24,6 +24,7 @@ def group_rows(lists, n_lists: int, check: bool = True) -> "RowGroups":
     is); an id < 0 has no list.  Returns the entries (row * k + slot) in list order, stable: RowGroups.  Asynchronous on the current
     stream, except for check: wait and raise IndexError if an id is >= n_lists; check=False leaves such an entry without a list."""
     lib = _lib.load()
+    not_traced("group_rows")
     on_device(lists, "lists")
     if lists.dim() not in (1, 2):
         raise ValueError(f"lists must be (n,) or (n, k), got {tuple(lists.shape)}")
@@ -109,7 +110,7 @@ class RowGroups:
         if x.requires_grad and torch.is_grad_enabled():
             row_type(x, "x that requires a gradient")
             return _Gather.apply(x, self)
-        return self._gather(x)
+        return _Gather.apply(x, self) if being_traced() else self._gather(x)   # (a trace holds the function, with these groups)
 
     def combine(self, y, weights=None):
         """y (n k, D) float32 / float16 / bfloat16 in list order -> (n, D): sum_j weights[r, j] y[place[r, j]] over the entries that have
@@ -122,7 +123,7 @@ class RowGroups:
                 raise ValueError(f"weights must be ({self.n}, {self.k}) float32 or {y.dtype} on {y.device}, got {tuple(weights.shape)} {weights.dtype}")
             weights = as_stored(weights).contiguous()
         _no_tangents(y, weights)
-        if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
+        if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)) or being_traced():
             return _Combine.apply(y, weights, self)
         return self._combine(y, weights)
 

@@ -6,6 +6,7 @@ A prior over the codes of a residual quantiser answers with K logits per step (o
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 
 import numpy as np
@@ -48,14 +49,26 @@ def unit_rows(t):
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
+_recording = functools.partial(torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY)
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 # the handle of a device's current stream without a Stream object around it (2 us of a call of 12), where this torch has it
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
+being_traced = torch._C._get_tracing_state    # (torch.jit.trace: not None; torch.jit.is_tracing takes five times as long to say so)
+
+
+def not_traced(what: str) -> None:
+    """torch.jit.trace records torch's own operators alone: the trace would answer the memory that a library call is to fill."""
+    if being_traced() is not None:
+        raise RuntimeError(f"{what} cannot be traced by torch.jit")
+
+
 def on_its_device(index: int, call, *args) -> None:
     """One library call on the current stream of device `index` (its last argument), with that device current: kernels are launched on a
-    stream of the current device."""
+    stream of the current device.  Not while torch.fx records operators (make_fx), which has no way to see the call."""
+    if _recording() is not None:
+        raise RuntimeError("qinco_amd's operators on tensors cannot be recorded by torch.fx")
     if _current_device() == index:
         rc = call(*args, _raw_stream(index))
     else:
@@ -87,6 +100,7 @@ def sample_codes(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, c
 
     temperature, top_p, min_p (float32) and top_k (int32) may be tensors (n,) with a value per row; there a temperature <= 0 is 0."""
     lib = _lib.load()
+    not_traced("sample_codes")
     shape = on_device(logits, "logits").shape
     if len(shape) != 2 or shape[1] < 1:
         raise ValueError(f"logits must be (n, V) with V >= 1, got {tuple(shape)}")

@@ -908,3 +908,50 @@ def test_forward_mode_derivatives_are_refused(no_calls):
             torch.autograd.grad(out, leaves, torch.ones_like(out), retain_graph=True)
             with pytest.raises(NotImplementedError):                           # ... of a backward pass
                 torch.autograd.grad(out, leaves, dual(torch.ones_like(out)))
+
+
+def test_traces_hold_the_calls_or_are_refused(no_calls):
+    """A trace of what torch itself records would answer uninitialised memory."""
+    import torch
+    from qinco_amd import sample
+    g = host_groups(no_calls)
+    x, y, w = torch.randn(4, 3), torch.randn(8, 3), torch.rand(4, 2)
+
+    def trace(f, *args):
+        return torch.jit.trace(f, args, check_trace=False)
+    for f, args, name in ((g.gather, (x,), "_Gather"), (g.gather, (x.to(torch.uint8),), "_Gather"), (g.combine, (y,), "_Combine"), (g.combine, (y, w), "_Combine")):
+        for mode in (torch.enable_grad, torch.no_grad):
+            with mode():
+                t = trace(lambda *a: f(*a), *args)
+            assert "^" + name in str(t.graph) and t(*args).shape == f(*args).shape
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        trace(lambda a: no_calls.group_rows(a, 4).order, torch.zeros(5, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        trace(lambda a: sample.sample_codes(a, torch.rand(4)), x)
+
+
+def test_recording_by_fx_is_refused():
+    import torch
+    from torch.fx.experimental.proxy_tensor import make_fx
+    from qinco_amd import lists, sample
+    calls = []
+
+    def record(a):
+        sample.on_its_device(0, lambda *args: calls.append(args))
+        return a * 2
+    with pytest.raises(RuntimeError, match="torch.fx"):
+        make_fx(record)(torch.ones(3))
+    assert lists.on_its_device is sample.on_its_device and not calls
+
+
+@gpu
+def test_traced_gather_and_combine_answer_what_they_answer():
+    import torch
+    g = torch.Generator("cuda").manual_seed(31)
+    gr = make_groups(g, 40, 3, 9, True)
+    x, y, w = torch.randn(40, 12, generator=g, device="cuda"), torch.randn(120, 12, generator=g, device="cuda"), torch.rand(40, 3, generator=g, device="cuda")
+    run = lambda a, b, c: (gr.gather(a) * 2, gr.gather(a.to(torch.uint8)), gr.combine(b), gr.combine(b, c))      # noqa: E731
+    traced = torch.jit.trace(run, (x.abs(), y, w))
+    for _ in range(3):
+        x, y, w = x.roll(1, 0).abs(), y.roll(1, 0), w.roll(1, 0)
+        assert all(torch.equal(a, b) for a, b in zip(traced(x, y, w), run(x, y, w)))
