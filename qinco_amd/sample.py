@@ -98,7 +98,11 @@ def sample_codes(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, c
     codes, whatever else is in the batch.  Masses and sums are held in 62 bits of the row's total: top_p and u decide as in exact arithmetic
     unless they lie within 2^-43 of a border (V <= 20480; 2^-39 at 2^20 codes, 2^-35 at 2^24).
 
-    temperature, top_p, min_p (float32) and top_k (int32) may be tensors (n,) with a value per row; there a temperature <= 0 is 0."""
+    temperature, top_p, min_p (float32) and top_k (int32) may be tensors (n,) with a value per row; there a temperature <= 0 or NaN is 0, a
+    min_p above 1 is 1, and NaN switches a cut off.
+
+    The log probabilities are values: no derivative goes through them, whether the logits require one or carry a tangent.  For a gradient
+    take torch.log_softmax(logits / temperature, 1) at the codes (of what is kept, where something is cut)."""
     lib = _lib.load()
     not_traced("sample_codes")
     shape = on_device(logits, "logits").shape

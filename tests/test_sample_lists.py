@@ -955,3 +955,40 @@ def test_traced_gather_and_combine_answer_what_they_answer():
     for _ in range(3):
         x, y, w = x.roll(1, 0).abs(), y.roll(1, 0), w.roll(1, 0)
         assert all(torch.equal(a, b) for a, b in zip(traced(x, y, w), run(x, y, w)))
+
+
+def test_log_probabilities_carry_no_derivative(no_calls):
+    """As the docstring says, in both modes; the codes neither."""
+    import torch
+    import torch.autograd.forward_ad as fa
+    from qinco_amd.sample import sample_codes
+    z, u = torch.randn(4, 8), torch.rand(4)
+    codes, logp = sample_codes(z.requires_grad_(), u, temperature=torch.ones(4, requires_grad=True), return_logp=True)
+    assert not logp.requires_grad and not codes.requires_grad
+    with fa.dual_level():
+        assert fa.unpack_dual(sample_codes(fa.make_dual(z.detach(), torch.ones(4, 8)), u, return_logp=True)[1]).tangent is None
+    assert "no derivative" in sample_codes.__doc__
+
+
+@gpu
+@pytest.mark.parametrize("V", [50, 200, 500, 3000, 30000])
+def test_sample_settings_per_row_that_are_no_settings(V):
+    """NaN, infinities and a min_p above 1 in the arrays: what the docstring says they are."""
+    import torch
+    from qinco_amd import sample_codes
+    g = torch.Generator("cuda").manual_seed(V)
+    z = torch.randn(12, V, generator=g, device="cuda")
+    u = torch.rand(12, generator=g, device="cuda")
+    nan, inf = math.nan, math.inf
+    row = lambda v, dt=torch.float32: torch.tensor(v, dtype=dt, device="cuda")                                   # noqa: E731
+    odd = dict(temperature=row([nan, -inf, -0.0, 1.0] + [0.5] * 8), top_p=row([0.5] * 4 + [nan, inf, -inf, -1.0] + [1.0] * 4),
+               min_p=row([0.01] * 8 + [nan, -inf, inf, 7.0]), top_k=row([V + 1, -(1 << 31), (1 << 31) - 1, 0] * 3, torch.int32))
+    same = dict(temperature=row([0.0, 0.0, 0.0, 1.0] + [0.5] * 8), top_p=row([0.5] * 4 + [1.0, 1.0, 0.0, 0.0] + [1.0] * 4),
+                min_p=row([0.01] * 8 + [0.0, 0.0, 1.0, 1.0]), top_k=row([0] * 12, torch.int32))
+    a, b = sample_codes(z, u, return_logp=True, **odd), sample_codes(z, u, return_logp=True, **same)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    first = z.argmax(1)                                       # (all different)
+    assert torch.equal(a[0][[0, 1, 2, 6, 7, 10, 11]], first[[0, 1, 2, 6, 7, 10, 11]])
+    z[:, ::3] = -inf
+    hot = sample_codes(z, u, temperature=torch.full((12,), inf, device="cuda"))        # every finite logit as likely
+    assert torch.equal(hot, sample_codes(torch.where(z > -inf, 0.0, z), u))
