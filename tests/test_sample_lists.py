@@ -992,3 +992,68 @@ def test_sample_settings_per_row_that_are_no_settings(V):
     z[:, ::3] = -inf
     hot = sample_codes(z, u, temperature=torch.full((12,), inf, device="cuda"))        # every finite logit as likely
     assert torch.equal(hot, sample_codes(torch.where(z > -inf, 0.0, z), u))
+
+
+@gpu
+@pytest.mark.parametrize("n,V,dtype", [(2900, 20481, "float16"), (90, 1 << 20, "float32")])
+def test_sample_more_long_rows_than_one_batch_holds(n, V, dtype):
+    """The workspace holds some 1300 rows of 20481 codes, some 70 of 2^20: what is drawn does not depend on where a batch ends."""
+    import torch
+    from qinco_amd import sample_codes
+    g = torch.Generator("cuda").manual_seed(n)
+    z = (torch.randn(n, V, generator=g, device="cuda") * 2.5).to(getattr(torch, dtype))
+    z[n // 2] = -float("inf")
+    u = torch.rand(n, generator=g, device="cuda", dtype=torch.float64)
+    T = torch.rand(n, generator=g, device="cuda") + 0.2
+    T[::7] = 0.0
+    for s in (dict(), dict(top_k=40, top_p=0.9, min_p=0.01)):
+        codes, logp = sample_codes(z, u, temperature=T, return_logp=True, **s)
+        for a in range(0, n, 60):                                              # every row in a batch of its own neighbourhood
+            b = min(a + 60, n)
+            c, l = sample_codes(z[a:b], u[a:b], temperature=T[a:b], return_logp=True, **s)
+            assert torch.equal(c, codes[a:b]) and torch.equal(l, logp[a:b])
+        assert int(codes[n // 2]) == -1 and torch.equal(z[::7].gather(1, codes[::7, None])[:, 0], z[::7].amax(1))
+    rows = [0, 1, n // 2, n - 2, n - 1]
+    check_sample(z[rows], u[rows].contiguous(), T=T[rows].cpu().numpy(), k=40, p=0.9, m=0.01)
+
+
+@gpu
+@pytest.mark.parametrize("V", [60, 200, 500, 3000, 30000])
+def test_sample_rows_behind_four_giga_elements(V):
+    """Rows 2^23 elements apart: the last ones begin behind 2^32 elements."""
+    import torch
+    from qinco_amd import sample_codes
+    g = torch.Generator("cuda").manual_seed(V)
+    n, stride = 520, 1 << 23
+    store = torch.empty((n - 1) * stride + V, dtype=torch.bfloat16, device="cuda")
+    z = store.as_strided((n, V), (stride, 1))
+    near = (torch.randn(n, V, generator=g, device="cuda") * 2.5).bfloat16()
+    z.copy_(near)
+    u = torch.rand(n, generator=g, device="cuda")
+    for s in (dict(), dict(top_k=30, top_p=0.9)):
+        assert torch.equal(sample_codes(z, u, **s), sample_codes(near, u, **s))
+
+
+@gpu
+def test_gather_and_combine_behind_two_to_the_32_elements():
+    """More than 2^32 elements of one byte (rows of an odd number of bytes: moved byte by byte) and of two, in both directions."""
+    import torch
+    from qinco_amd import group_rows
+    n, k, D = 2_200_000, 2, 1001
+    assert n * k * D > 1 << 32
+    r = torch.arange(n, device="cuda")
+    gr = group_rows(torch.stack([r, r], 1), n)                                  # row r in places 2 r, 2 r + 1
+    x = torch.randint(0, 256, (n, D), device="cuda", dtype=torch.uint8)
+    out = gr.gather(x)
+    assert torch.equal(out[::2], x) and torch.equal(out[1::2], x)
+    del x
+    y = out.to(torch.bfloat16)
+    del out
+    w = torch.tensor([[1.0, -0.5]], device="cuda").expand(n, 2).contiguous()
+    got = gr.combine(y, w)
+    assert torch.equal(got, y[::2] * 0.5)
+    dy, dw = gr._combine_grad(got, y, w, True, True)
+    assert torch.equal(dy[::2], got) and torch.equal(dy[1::2], got * -0.5)
+    for i in (0, n // 2, n - 1):
+        want = float((got[i].double() * y[2 * i].double()).sum())
+        assert abs(float(dw[i, 0]) - want) <= D * 2.0 ** -24 * want and float(dw[i, 0]) == float(dw[i, 1])
