@@ -1057,3 +1057,40 @@ def test_gather_and_combine_behind_two_to_the_32_elements():
     for i in (0, n // 2, n - 1):
         want = float((got[i].double() * y[2 * i].double()).sum())
         assert abs(float(dw[i, 0]) - want) <= D * 2.0 ** -24 * want and float(dw[i, 0]) == float(dw[i, 1])
+
+
+@gpu
+@pytest.mark.parametrize("V,n", [(60, 64), (60, 4096), (120, 64), (120, 4096), (250, 64), (250, 4096), (500, 64), (1000, 64), (1000, 512), (2048, 64), (2048, 512), (4099, 64), (4099, 512),
+                                 (10000, 64), (10000, 512), (20480, 64), (70001, 64), (1 << 20, 64), (1 << 22, 64)])
+def test_sample_draws_and_cuts_within_the_stated_distance_of_a_border(V, n):
+    """u, and top_p, next to the borders between codes, as far from them as the stated bound, against sums of 64-bit mantissas."""
+    import torch
+    from qinco_amd import sample_codes
+    rs = np.random.RandomState(V)
+    near = 2.0 ** -52 + 2.0 ** -44 + (V * 2.0 ** -53 if V <= 512 else 2.25 * V * 2.0 ** -61)
+    for T, spread in ((1.0, 2.5), (0.37, 4.0), (3.0, 0.5)):
+        z = (rs.randn(V) * spread).astype(np.float32)
+        top = np.longdouble(z.max())
+        e = np.exp((z.astype(np.longdouble) - top) / np.longdouble(T))
+        heavy = np.flatnonzero(e / e.sum() > 16 * near)
+        dev = torch.from_numpy(z).cuda().expand(n, V)
+        # draws: above and below the border behind code i
+        run = np.cumsum(e) / e.sum()
+        i = rs.choice(heavy[:-1], n // 2)
+        u = np.concatenate([run[i] - near, run[i] + near]).astype(np.float64)
+        for s in (dict(), dict(min_p=1e-30)):
+            got = sample_codes(dev, torch.from_numpy(u).cuda(), temperature=T, **s).cpu().numpy()
+            assert np.all((run[got] + near > u) & (run[got] - e[got] / e.sum() - near <= u))
+            assert np.array_equal(got[: n // 2], i)                                    # (heavy codes: just before their end)
+        # top-p: the codes kept are the first r by logit; u = 0 draws the lowest kept index, u -> 1 the highest
+        order = np.argsort(-z, kind="stable")
+        before = np.cumsum(e[order]) / e.sum()
+        for r in rs.choice(np.flatnonzero(e[order] / e.sum() > 16 * near)[:-1], 8):
+            for p, kept in ((before[r] - near, r + 1), (before[r] + near, r + 2)):
+                if not 0 < p < 1:
+                    continue
+                ends = torch.tensor([0.0, 1.0 - 2.0 ** -53], dtype=torch.float64, device="cuda").repeat(n // 2)
+                got = sample_codes(dev, ends, temperature=T, top_p=float(p)).cpu().numpy()
+                share = e[np.sort(order[:kept])] / e[order[:kept]].sum()
+                if share[-1] > near:
+                    assert np.all(got[0::2] == order[:kept].min()) and np.all(got[1::2] == order[:kept].max()), (T, r, p)
