@@ -315,7 +315,8 @@ enum { QINCO_T_F32 = 0, QINCO_T_F16 = 1, QINCO_T_BF16 = 2 };
  * inputs give the same codes, whatever the launch, and p and u decide as in exact arithmetic unless they lie within 2^-43 of a border
  * (V <= 20480; 2^-39 at 2^20 codes, 2^-35 at 2^24).
  * The settings: arrays of one value per row, or NULL and the scalar.  top_k <= 0 or >= V, top_p >= 1, min_p <= 0 switch a cut off.
- * workspace: qinco_sample_workspace(n, V) bytes of device memory that no other running call uses.  Device pointers, asynchronous. */
+ * workspace: qinco_sample_workspace(n, V) bytes of device memory, aligned to 16, that no other running call uses.  Device pointers,
+ * asynchronous. */
 typedef struct {
   int32_t struct_bytes;            /* sizeof(qinco_sample_params) */
   int32_t top_k;
@@ -336,7 +337,7 @@ QINCO_API int qinco_sample_codes(const void* logits, int dtype, int64_t row_stri
  *   place   (n, k)         slot of each entry; -1 if it has no list (id < 0)
  *   offsets (n_lists + 1)  first slot of each list; offsets[n_lists] = slots in use
  *   bad     nullable       set to 1 if an id is >= n_lists (never cleared here); such an entry counts as having no list
- * 1 <= n_lists <= 2^24, n k < 2^31.  workspace: qinco_group_workspace(n k, n_lists) bytes.  Device pointers, asynchronous. */
+ * 1 <= n_lists <= 2^24, n k < 2^31.  workspace: qinco_group_workspace(n k, n_lists) bytes, aligned to 16.  Device pointers, asynchronous. */
 QINCO_API int64_t qinco_group_workspace(int64_t entries, int64_t n_lists);
 QINCO_API int qinco_group_rows(const void* lists, int code_dtype, int64_t row_stride, int64_t n, int32_t k, int64_t n_lists, int32_t* order,
                                int32_t* place, int32_t* offsets, int32_t* bad, void* workspace, int64_t workspace_bytes, void* stream);

@@ -23,6 +23,9 @@ static int bits_of(uint64_t v) {   // bits that hold 0 .. v - 1
 
 static bool known(int dtype) { return dtype == QINCO_T_F32 || dtype == QINCO_T_F16 || dtype == QINCO_T_BF16; }
 
+// a workspace holds whole numbers of 64 bits and takes atomics: at an odd address these would fault
+static bool aligned(const void* ws) { return reinterpret_cast<uintptr_t>(ws) % 16 == 0; }
+
 // ---------------------------------------------------------------------------------------------
 // sampling
 // ---------------------------------------------------------------------------------------------
@@ -191,6 +194,7 @@ extern "C" int qinco_sample_codes(const void* logits, int dtype, int64_t row_str
   const SamplePlan p = sample_plan(n, V);
   if (p.bytes > 0 && (!workspace || workspace_bytes < p.bytes))
     return fail(QINCO_ERR_INVALID, "qinco_sample_codes: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)p.bytes);
+  if (p.bytes > 0 && !aligned(workspace)) return fail(QINCO_ERR_INVALID, "qinco_sample_codes: workspace not aligned to 16 bytes");
   const int lv = bits_of((uint64_t)V);
   SampleArgs a{logits, (long)row_stride, (long)n, (int)V, u, u_is_f64 != 0, params->temperature_rows, params->temperature, params->top_k_rows,
                params->top_k, params->top_p_rows, params->top_p, params->min_p_rows, params->min_p, codes_out,
@@ -284,6 +288,7 @@ extern "C" int qinco_group_rows(const void* lists, int code_dtype, int64_t row_s
   const GroupPlan p = group_plan(N, n_lists);
   if (!workspace || workspace_bytes < p.words * 4)
     return fail(QINCO_ERR_INVALID, "qinco_group_rows: workspace of %lld bytes, %lld needed", (long long)workspace_bytes, (long long)p.words * 4);
+  if (!aligned(workspace)) return fail(QINCO_ERR_INVALID, "qinco_group_rows: workspace not aligned to 16 bytes");
   hipStream_t st = reinterpret_cast<hipStream_t>(stream);
   unsigned* ws = reinterpret_cast<unsigned*>(workspace);
   const unsigned E = (unsigned)n_lists;

@@ -1094,3 +1094,17 @@ def test_sample_draws_and_cuts_within_the_stated_distance_of_a_border(V, n):
                 share = e[np.sort(order[:kept])] / e[order[:kept]].sum()
                 if share[-1] > near:
                     assert np.all(got[0::2] == order[:kept].min()) and np.all(got[1::2] == order[:kept].max()), (T, r, p)
+
+
+def test_workspaces_at_odd_addresses_are_refused(lib):
+    """Decided on the host, before anything is launched: their 64-bit words and atomics would not be aligned."""
+    from qinco_amd import _lib
+    P = _lib.QincoSampleParams
+    params = P(struct_bytes=C.sizeof(P), temperature=1.0, top_p=0.5)
+    buf = (C.c_char * 64)()
+    at = (C.addressof(buf) + 15) // 16 * 16
+    for off in (1, 2, 4, 8):
+        assert lib.qinco_sample_codes(at, 0, 30000, 2, 30000, at, 0, C.byref(params), at, 0, None, at + off, 1 << 40, None) == -1
+        assert b"qinco_sample_codes" in lib.qinco_last_error() and b"aligned" in lib.qinco_last_error()
+        assert lib.qinco_group_rows(at, 0, 1, 4, 1, 8, at, at, at, None, at + off, 1 << 40, None) == -1
+        assert b"qinco_group_rows" in lib.qinco_last_error() and b"aligned" in lib.qinco_last_error()
