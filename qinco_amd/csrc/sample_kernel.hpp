@@ -1053,7 +1053,11 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a, long 
     if (lane == 0) atomicAdd(&upper, sum);
     __syncthreads();
     mass.scale(max(17 - __builtin_clz((unsigned)__builtin_amdgcn_readfirstlane((int)upper) + (unsigned)V), 0));
-    each([&](int j, float) { q[j] >>= mass.down; });
+#pragma unroll
+    for (int j = 0; j < R; j += PAIR)
+      if (j < steps)
+#pragma unroll
+        for (int e = 0; e < PAIR; ++e) q[j + e] >>= mass.down;
   };
   float t = sample_massless(zmax, set.y);
   unsigned r = 0;
