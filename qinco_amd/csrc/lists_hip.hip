@@ -151,14 +151,15 @@ static void launch_sample_block(const SampleArgs& a, hipStream_t st) {
   sample_launches(a.n, 1, NT, [&](dim3 grid, long r0) { hipLaunchKernelGGL((sample_block_kernel<T, NT, R>), grid, dim3(NT), 0, st, a, r0); });
 }
 
-// By the length of a row, and where the rows alone do not fill the card with more lanes to each (a row's code depends on neither).  Each
-// border with both sides measured, all three cuts on, fp32.  65536 rows of 64 23 us with 16 lanes each; of 128 36 us with 16 lanes, 65 with 32;
-// of 256 67 us with 32, 78 with 64.  With a wave each or fewer lanes, one row of 128 or 256 4.7 and 6.4 us, 2048 rows of 256 6.7 and 7.8, 4096
-// 8.9 and 8.6; 2048 of 128 6.3 and 7.7, 8192 12.5 and 8.6.  16384 of 512 36 us with a wave each, 75 with four, of 520 86 and 85; 8000 of 2000
-// 70 us with 8 codes per thread, 83 with 20; of 4099 127 us with 256 threads, 171 with 512; of 10240 274 with 512 threads, 384 with 256, 435
-// with 1024; one row of 20480 19 us with a workgroup, 44 split over several, 1000 of them 87 and 216.  One row of 2000 7.5 us with 512
-// threads, 9.0 with 256, 300 of them 9.7 and 9.4; one of 4099 10.2 and 13.6; one of 10240 13.7 with 1024 threads, 15.0 with 512, 300 of them
-// 27 and 21.
+// By the length of a row, and where the rows alone do not fill the card with more lanes to each (a row's code depends on neither).  Both sides of
+// each border measured, all three cuts on, fp32.  65536 rows of 64 24 us with 4 codes per lane, 35 with 8; of 128 38 us with 16 lanes, 68 with
+// 32; of 256 70 us with 32, 81 with 64.  With a wave each or fewer lanes, one row of 128 or 256 4.8 and 6.5 us, 2048 rows of 256 6.9 and 7.8,
+// 4096 9.0 and 8.7; 2048 of 128 6.3 and 7.8, 8192 13.0 and 8.6.  16384 of 512 38 us with a wave each, 82 with four; of 1000 97 us with 4 codes
+// per thread, 113 with 8; 8000 of 2000 75 us with 8, 89 with 20; of 4099 136 us with 256 threads, 182 with 512; of 10240 289 us with 512 threads,
+// 474 with 1024; one row of 20480 21 us with a workgroup, 43 split over several, 1000 of them 97 and 190.  Few rows, 512 and 256 threads: of 2000
+// one 7.8 and 9.1 us, 256 8.5 and 9.9, 500 10.5 and 11.0, 700 12.6 and 12.1, 1000 16.6 and 13.6; of 4099 one 10.8 and 13.9, 256 11.6 and 14.8, 500
+// 14.6 and 16.8, 700 22.0 and 19.3, 1000 26 and 22; 1024 and 512 threads, of 10240 one 14.9 and 15.6, 256 16.1 and 17.1, 300 29 and 22.  (So up to
+// 6144 codes the border of one row per CU comes early: at two the larger workgroups are still 5 to 15 % ahead.)
 template <typename T>
 static int launch_sample(const SampleArgs& a, const SamplePlan& p, char* ws, hipStream_t st) {
   if (a.V > kSampleLongV) return launch_sample_long<T>(a, p, ws, st);

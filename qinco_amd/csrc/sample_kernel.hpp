@@ -616,6 +616,7 @@ struct SampleWaveRow {
   }
 };
 
+// (Five waves per SIMD asked for: left alone the compiler takes 104 registers for 8 codes per lane instead of 88, 16384 x 512 42 us instead of 39.)
 template <typename T, int R>
 __global__ void __launch_bounds__(64 * kSampleRowWaves, 5) sample_wave_kernel(SampleArgs a, long row0) {
   __shared__ SampleWaveLds lds[kSampleRowWaves];
@@ -939,10 +940,10 @@ __device__ __forceinline__ void sample_draw(const SampleArgs& a, long row, const
 // One workgroup per row, V <= NT R, the row and its masses in registers: thread t holds codes t steps ... t steps + steps - 1.  The codes of
 // the bin that a cut falls into are listed, and up to 64 of them compared by one wave, a lane each; more (heavy ties) are searched in bins.
 // One scan over the threads, of the mass above t and of the codes at t, gives the total and the thread that the draw falls on.  Every
-// exponential is taken once (of what top-k keeps alone, where nothing else wants them) and kept: with the row in LDS, taking them anew in
-// each pass, 8000 rows of 4099 fp16 went in 138 us without a cut and 206 with all three; so they go in 80 and 126, and one row of 10240
-// in 13 instead of 36.  Bound by instructions: 74 vector ones per code without a cut, 111 with all three, issued four fifths of the time.
-// (Loads of 16 bytes for two-byte types, eight codes, are worth 1 us of the 80.)
+// exponential is taken once (of what top-k keeps alone, where nothing else wants them) and kept: 8000 rows of 4099 fp16 go in 88 us without
+// a cut, 110 with a top-k of 40 and 133 with all three, one row of 10240 in 15; with the row in LDS and the exponentials taken anew in each pass
+// they took two thirds longer.  Bound by instructions: 86, 97 and 125 vector ones per 64 codes, issued 0.90, 0.79 and 0.85 of the time.  (Loads of
+// 16 bytes for two-byte types, eight codes, are worth 1 us of the 88.)
 template <typename T, int NT, int R>
 __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a, long row0) {
   constexpr int PB = kSampleBins / NT, PAIR = 2;
@@ -1288,8 +1289,8 @@ __global__ void __launch_bounds__(NT, 4) sample_block_kernel(SampleArgs a, long 
 // ---------------------------------------------------------------------------------------------------------------------
 constexpr int kSampleChunkThreads = 1024, kSampleChunkIpt = 16, kSampleChunk = kSampleChunkThreads * kSampleChunkIpt;
 constexpr int kSampleMaxChunks = 1024;          // V <= 2^24
-constexpr int kSampleFewChunks = 4;             // up to which the bins are summed where the cuts are found (500 rows of 50000: 154 us, 169
-                                                // with a launch of its own; one row of 130000, eight chunks, 39 and 37)
+constexpr int kSampleFewChunks = 4;             // up to which the bins are summed where the cuts are found (500 rows of 50000, all cuts: 150
+                                                // us, 164 with a launch of its own; one row of 130000, eight chunks, 46 and 45)
 constexpr int kSampleHere = 2048;               // members of a chunk listed one by one; with more, equal ones as one
 constexpr int kSampleMembers = 4096;            // members of a row that the last kernel holds in LDS
 
@@ -1491,8 +1492,8 @@ __global__ void __launch_bounds__(kSampleChunkThreads) sample_bins_kernel(Sample
   if (tid == 0) l.floor[r * l.chunks + c] = floor;
 }
 
-// Where no row has a cut the mass of every chunk is all that the last kernel needs: three launches (one row of 50000 fp32 21 us, 16 of 2^20
-// 47; with bins, cuts and members all the same 32 and 67).
+// Where no row has a cut the mass of every chunk is all that the last kernel needs: three launches (one row of 50000 fp32 22 us, 16 of 2^20
+// 50; with bins, cuts and members all the same 33 and 73).
 template <typename T>
 __global__ void __launch_bounds__(kSampleChunkThreads) sample_mass_kernel(SampleArgs a, SampleLong l) {
   __shared__ unsigned sh[4];
