@@ -13,7 +13,7 @@ from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
-from .sample import _TYPES, as_stored, being_traced, not_traced, on_device, on_its_device, row_type, unit_rows
+from .sample import _TYPES, as_stored, being_traced, on_device, on_its_device, recording, refuse_trace, row_type, unit_rows
 
 MAX_LISTS = 1 << 24
 _IDS = {torch.int64: _lib.CODE_I64, torch.int32: _lib.CODE_I32, torch.uint8: _lib.CODE_U8}
@@ -24,7 +24,8 @@ def group_rows(lists, n_lists: int, check: bool = True) -> "RowGroups":
     is); an id < 0 has no list.  Returns the entries (row * k + slot) in list order, stable: RowGroups.  Asynchronous on the current
     stream, except for check: wait and raise IndexError if an id is >= n_lists; check=False leaves such an entry without a list."""
     lib = _lib.load()
-    not_traced("group_rows")
+    if being_traced() or recording() is not None:
+        refuse_trace("group_rows")
     on_device(lists, "lists")
     if lists.dim() not in (1, 2):
         raise ValueError(f"lists must be (n,) or (n, k), got {tuple(lists.shape)}")
@@ -59,10 +60,9 @@ def group_rows(lists, n_lists: int, check: bool = True) -> "RowGroups":
 
 def _no_tangents(*tensors):
     """Forward-mode derivatives are refused: a library call would answer its values without them."""
-    if forward_ad._current_level >= 0:                 # (between dual levels there are none)
-        for t in tensors:
-            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
-                raise NotImplementedError("gather and combine have no forward-mode derivatives")
+    for t in tensors:
+        if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("gather and combine have no forward-mode derivatives")
 
 
 class RowGroups:
@@ -106,26 +106,38 @@ class RowGroups:
         """x (n, D) of any type, also code rows -> (n k, D): row order[s] // k at place s, zeros behind the last place in use.
         The gradient is the sum over a row's places, in 32 bits, rounded once (float32, float16, bfloat16)."""
         x = self._rows(x, self.n, "x")
-        _no_tangents(x)
+        if recording() is not None:
+            refuse_trace("gather")
+        if forward_ad._current_level >= 0:             # (between dual levels there are no tangents)
+            _no_tangents(x)
+        traced = being_traced()                        # (a trace holds the function, with these groups)
         if x.requires_grad and torch.is_grad_enabled():
             row_type(x, "x that requires a gradient")
-            return _Gather.apply(x, self)
-        return _Gather.apply(x, self) if being_traced() else self._gather(x)   # (a trace holds the function, with these groups)
+            return _Gather.apply(x, self, traced)
+        return _Gather.apply(x, self, True) if traced else self._gather(x)
 
     def combine(self, y, weights=None):
         """y (n k, D) float32 / float16 / bfloat16 in list order -> (n, D): sum_j weights[r, j] y[place[r, j]] over the entries that have
         a list (zeros for a row without one), in 32 bits in the order of j, rounded once.  weights (n, k) float32 or y's type; None: ones.
         Rows of y behind the last place in use and weights of entries without a list are not read; their gradients are zeros."""
+        y, weights = self._combine_args(y, weights)
+        if recording() is not None:
+            refuse_trace("combine")
+        if forward_ad._current_level >= 0:
+            _no_tangents(y, weights)
+        traced = being_traced()
+        if traced or torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)):
+            return _Combine.apply(y, weights, self, traced)
+        return self._combine(y, weights)
+
+    def _combine_args(self, y, weights):
         y = self._rows(y, self.n * self.k, "y")
         row_type(y, "y")
         if weights is not None:
             if on_device(weights, "weights").shape != (self.n, self.k) or weights.dtype not in (torch.float32, y.dtype) or weights.device != y.device:
                 raise ValueError(f"weights must be ({self.n}, {self.k}) float32 or {y.dtype} on {y.device}, got {tuple(weights.shape)} {weights.dtype}")
             weights = as_stored(weights).contiguous()
-        _no_tangents(y, weights)
-        if torch.is_grad_enabled() and (y.requires_grad or (weights is not None and weights.requires_grad)) or being_traced():
-            return _Combine.apply(y, weights, self)
-        return self._combine(y, weights)
+        return y, weights
 
     # -- the library calls; arguments are checked already, rows in unit_rows' form
     def _gather(self, x):
@@ -155,18 +167,20 @@ class RowGroups:
 
 
 def _gather_grad(ctx, dout):
-    _no_tangents(dout)
-    return ctx.groups._combine(unit_rows(dout), None), None
+    if forward_ad._current_level >= 0:
+        _no_tangents(dout)
+    return ctx.groups._combine(unit_rows(dout), None), None, None
 
 
 def _combine_grad(ctx, dout):
-    _no_tangents(dout)
+    if forward_ad._current_level >= 0:
+        _no_tangents(dout)
     dout = unit_rows(dout)
     if not ctx.weighted:
-        return ctx.groups._gather(dout), None, None
+        return ctx.groups._gather(dout), None, None, None
     y, weights = ctx.saved_tensors
-    need_dy, need_dw, _ = ctx.needs_input_grad
-    return (*ctx.groups._combine_grad(dout, y, weights, need_dy, need_dw), None)
+    need_dy, need_dw = ctx.needs_input_grad[:2]
+    return (*ctx.groups._combine_grad(dout, y, weights, need_dy, need_dw), None, None)
 
 
 # Second derivatives are refused.  once_differentiable() costs as much as the rest of a small backward call, and without create_graph (the
@@ -174,11 +188,12 @@ def _combine_grad(ctx, dout):
 _gather_grad_once, _combine_grad_once = once_differentiable(_gather_grad), once_differentiable(_combine_grad)
 
 
+# traced: a trace goes on from here, with tensors that nothing has looked at
 class _Gather(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, groups):
+    def forward(ctx, x, groups, traced):
         ctx.groups = groups
-        return groups._gather(x)
+        return groups._gather(groups._rows(x, groups.n, "x") if traced else x)
 
     @staticmethod
     def backward(ctx, dout):
@@ -187,7 +202,9 @@ class _Gather(torch.autograd.Function):
 
 class _Combine(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y, weights, groups):
+    def forward(ctx, y, weights, groups, traced):
+        if traced:
+            y, weights = groups._combine_args(y, weights)
         ctx.groups, ctx.weighted = groups, weights is not None
         if weights is not None:
             ctx.save_for_backward(y, weights)

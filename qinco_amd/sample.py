@@ -49,26 +49,25 @@ def unit_rows(t):
     return t if t.stride(1) == 1 or t.shape[1] == 1 else t.contiguous()
 
 
-_recording = functools.partial(torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY)
 _current_device = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
 # the handle of a device's current stream without a Stream object around it (2 us of a call of 12), where this torch has it
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-being_traced = torch._C._get_tracing_state    # (torch.jit.trace: not None; torch.jit.is_tracing takes five times as long to say so)
+being_traced = torch.jit.is_tracing
+# torch.fx's recorder, None where there is none
+recording = functools.partial(torch._C._get_dispatch_mode, torch._C._TorchDispatchModeKey.PROXY)
 
 
-def not_traced(what: str) -> None:
-    """torch.jit.trace records torch's own operators alone: the trace would answer the memory that a library call is to fill."""
-    if being_traced() is not None:
-        raise RuntimeError(f"{what} cannot be traced by torch.jit")
+def refuse_trace(what: str) -> None:
+    """torch.fx's recorder (make_fx) and torch.jit.trace see torch's own operators alone: what they make of a call would answer the memory that the
+    library fills."""
+    raise RuntimeError(f"{what} cannot be recorded by torch.fx" if recording() is not None else f"{what} cannot be traced by torch.jit")
 
 
 def on_its_device(index: int, call, *args) -> None:
     """One library call on the current stream of device `index` (its last argument), with that device current: kernels are launched on a
-    stream of the current device.  Not while torch.fx records operators (make_fx), which has no way to see the call."""
-    if _recording() is not None:
-        raise RuntimeError("qinco_amd's operators on tensors cannot be recorded by torch.fx")
+    stream of the current device."""
     if _current_device() == index:
         rc = call(*args, _raw_stream(index))
     else:
@@ -104,7 +103,8 @@ def sample_codes(logits, u, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, c
     The log probabilities are values: no derivative goes through them, whether the logits require one or carry a tangent.  For a gradient
     take torch.log_softmax(logits / temperature, 1) at the codes (of what is kept, where something is cut)."""
     lib = _lib.load()
-    not_traced("sample_codes")
+    if being_traced() or recording() is not None:
+        refuse_trace("sample_codes")
     shape = on_device(logits, "logits").shape
     if len(shape) != 2 or shape[1] < 1:
         raise ValueError(f"logits must be (n, V) with V >= 1, got {tuple(shape)}")

@@ -930,18 +930,18 @@ def test_traces_hold_the_calls_or_are_refused(no_calls):
         trace(lambda a: sample.sample_codes(a, torch.rand(4)), x)
 
 
-def test_recording_by_fx_is_refused():
+def test_recording_by_fx_is_refused(no_calls):
     import torch
     from torch.fx.experimental.proxy_tensor import make_fx
-    from qinco_amd import lists, sample
-    calls = []
-
-    def record(a):
-        sample.on_its_device(0, lambda *args: calls.append(args))
-        return a * 2
-    with pytest.raises(RuntimeError, match="torch.fx"):
-        make_fx(record)(torch.ones(3))
-    assert lists.on_its_device is sample.on_its_device and not calls
+    from qinco_amd import sample
+    g = host_groups(no_calls)
+    x, w = torch.randn(4, 3), torch.rand(4, 2)
+    for leaf in (x, x.clone().requires_grad_()):
+        for f in (g.gather, lambda a: g.combine(a.repeat(2, 1)), lambda a: g.combine(a.repeat(2, 1), w), lambda a: sample.sample_codes(a, torch.rand(4)),
+                  lambda a: no_calls.group_rows((a > 0).to(torch.int64), 4).order):
+            f(leaf)
+            with pytest.raises(RuntimeError, match="torch.fx"):
+                make_fx(lambda a: f(a))(leaf)
 
 
 @gpu
@@ -1108,3 +1108,43 @@ def test_workspaces_at_odd_addresses_are_refused(lib):
         assert b"qinco_sample_codes" in lib.qinco_last_error() and b"aligned" in lib.qinco_last_error()
         assert lib.qinco_group_rows(at, 0, 1, 4, 1, 8, at, at, at, None, at + off, 1 << 40, None) == -1
         assert b"qinco_group_rows" in lib.qinco_last_error() and b"aligned" in lib.qinco_last_error()
+
+
+@pytest.mark.parametrize("needs_grad", [False, True])
+def test_traces_look_at_the_tensors_they_get(no_calls, monkeypatch, needs_grad):
+    """What was looked at while tracing says nothing of the tensors that a trace gets later: other rows, types and strides."""
+    import torch
+    seen = []
+    monkeypatch.setattr(no_calls, "on_its_device", lambda index, call, *args: seen.append(args))
+    g = host_groups(no_calls)
+    x, y, w = torch.randn(4, 3), torch.randn(8, 3), torch.rand(4, 2)
+    gather = torch.jit.trace(lambda a: g.gather(a), (x.requires_grad_(needs_grad),), check_trace=False)
+    combine = torch.jit.trace(lambda a, b: g.combine(a, b), (y.requires_grad_(needs_grad), w), check_trace=False)
+    for bad in (x[:3], x[0], torch.randn(5, 3)):
+        with pytest.raises(Exception, match="x must be"):
+            gather(bad)
+    for a, b in ((y[:7], w), (y, w[:3]), (y, w.double()), (y.double(), w), (y, torch.rand(2, 4))):
+        with pytest.raises(Exception, match="must be"):
+            combine(a, b)
+    seen.clear()
+    wide = torch.randn(9, 4)
+    assert gather(wide.T).shape == (8, 9) and seen[0][1] == 9 * 4                       # rows of 9 elements next to each other
+    seen.clear()
+    combine(torch.randn(9, 8).T, torch.rand(2, 4).T)
+    assert seen[0][2:4] == (9, 9)
+
+
+@gpu
+def test_traces_with_other_rows_than_they_were_made_with():
+    import torch
+    g = torch.Generator("cuda").manual_seed(33)
+    gr = make_groups(g, 40, 3, 9, True)
+    x, y, w = torch.randn(40, 12, generator=g, device="cuda"), torch.randn(120, 12, generator=g, device="cuda"), torch.rand(40, 3, generator=g, device="cuda")
+    run = lambda a, b, c: (gr.gather(a), gr.combine(b, c))                                        # noqa: E731
+    traced = torch.jit.trace(run, (x, y, w))
+    for D in (1, 7, 130):
+        a, b = torch.randn(D, 40, generator=g, device="cuda").T, torch.randn(D, 120, generator=g, device="cuda").T.bfloat16()
+        got, want = traced(a, b, w.T.contiguous().T), run(a, b, w)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    with pytest.raises(Exception, match="x must be"):
+        traced(x[:39], y, w)
