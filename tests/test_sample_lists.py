@@ -1148,3 +1148,21 @@ def test_traces_with_other_rows_than_they_were_made_with():
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     with pytest.raises(Exception, match="x must be"):
         traced(x[:39], y, w)
+
+
+@gpu
+@pytest.mark.parametrize("V", [200, 500, 3000, 30000, 300000])
+def test_sample_logits_over_the_whole_range_at_huge_temperatures(V):
+    """Differences that fp32 does not hold, at temperatures that bring them back to size 1."""
+    import torch
+    g = torch.Generator("cuda").manual_seed(V)
+    z = torch.full((5, V), -3.0e38, device="cuda")
+    z[0, V // 2] = 3.0e38
+    z[1] = (torch.rand(V, generator=g, device="cuda") * 2 - 1) * 3.4e38
+    z[2, ::2] = 3.0e38
+    z[3, : V // 2] = -float("inf")
+    z[3, V - 1] = 3.4e38
+    z[4, V // 3] = float("inf")
+    for T in (1e38, 3e38, 1e39, 1e42, 1e45, 1e300):
+        for s in (dict(), dict(p=0.7), dict(k=V // 3, p=0.9, m=0.3)):
+            check_sample(z, torch.rand(5, generator=g, device="cuda", dtype=torch.float64), T=T, **s)
